@@ -117,6 +117,61 @@ int check_q(const cvsa_query_desc_t* qd, const KvView& kv, bool need_q, QView* o
   return CVSA_OK;
 }
 
+int check_ragged(const cvsa_ragged_desc_t* rd, RaggedView* out) {
+  if (!rd) return fail(CVSA_ERR_INVALID, "ragged descriptor is NULL");
+  if (rd->batch < 0 || rd->num_tokens < 0 || rd->num_seqs < 0 || rd->max_pages <= 0)
+    return fail(CVSA_ERR_INVALID, "ragged shape (batch=%d tokens=%d seqs=%d pages=%d)", rd->batch,
+                rd->num_tokens, rd->num_seqs, rd->max_pages);
+  if (rd->batch > 0 && (!rd->cu_tokens || !rd->block_tables || !rd->context_lens))
+    return fail(CVSA_ERR_INVALID, "cu_tokens/block_tables/context_lens is NULL");
+  if (!rd->seq_ids && rd->num_seqs < rd->batch)
+    return fail(CVSA_ERR_INVALID, "%d sequences but %d table rows", rd->batch, rd->num_seqs);
+  out->cu = rd->cu_tokens;
+  out->seq_ids = rd->seq_ids;
+  out->starts = rd->start_positions;
+  out->tables = rd->block_tables;
+  out->lens = rd->context_lens;
+  out->B = rd->batch;
+  out->T = rd->num_tokens;
+  out->num_seqs = rd->num_seqs;
+  out->W = rd->max_pages;
+  return CVSA_OK;
+}
+
+int check_chunk(const cvsa_chunk_attend_t* a, const KvView& kv, const RaggedView& rg,
+                ChunkView* out) {
+  if (!a) return fail(CVSA_ERR_INVALID, "arguments are NULL");
+  if (!valid_dtype(a->dtype)) return fail(CVSA_ERR_INVALID, "q dtype %d unknown", a->dtype);
+  if (a->num_q_heads <= 0 || a->num_q_heads % kv.hkv != 0)
+    return fail(CVSA_ERR_INVALID, "num_q_heads=%d is not a positive multiple of num_kv_heads=%d",
+                a->num_q_heads, kv.hkv);
+  if (rg.T > 0 && (!a->q || !a->out)) return fail(CVSA_ERR_INVALID, "q/out is NULL");
+  if (!(a->scale > 0.f) || a->scale > 3.0e38f)
+    return fail(CVSA_ERR_INVALID, "scale must be positive and finite");
+  if (a->window < 0 || (a->window > 0 && !a->causal))
+    return fail(CVSA_ERR_INVALID, "window must be >= 0, and 0 without causal");
+  const int eb = dtype_bytes(a->dtype);
+  if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) % 16 ||
+      (a->q_stride_token * eb) % 16 || (a->q_stride_head * eb) % 16 ||
+      (a->out_stride_token * eb) % 16 || (a->out_stride_head * eb) % 16)
+    return fail(CVSA_ERR_INVALID, "q/out rows must be 16-byte aligned");
+  out->q = a->q;
+  out->out = a->out;
+  out->lse = a->lse;
+  out->dtype = a->dtype;
+  out->hq = a->num_q_heads;
+  out->q_st = a->q_stride_token;
+  out->q_sh = a->q_stride_head;
+  out->o_st = a->out_stride_token;
+  out->o_sh = a->out_stride_head;
+  out->scale = a->scale;
+  out->causal = a->causal != 0;
+  out->window = a->window;
+  if (!chunk_attend_supported(kv, *out))
+    return fail(CVSA_ERR_UNSUPPORTED, "chunk_attend built for head_dim 64/128/256, G<=64");
+  return CVSA_OK;
+}
+
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // Largest page count the select kernel can hold in shared memory.
@@ -994,6 +1049,123 @@ int cvsa_paged_gather(const cvsa_kv_desc_t* kvd, const int32_t* block_table_row,
   return cuda_status(launch_paged_gather(kv, block_table_row, n_pages, k_out, v_out, dev_error,
                                          (cudaStream_t)stream),
                      "gather launch");
+}
+
+int cvsa_paged_reserve(int32_t block_size, const int32_t* cu_tokens, const int32_t* seq_ids,
+                       int32_t batch, int32_t num_seqs, int32_t* block_tables, int32_t max_pages,
+                       int32_t* context_lens, int32_t* pages_allocated, const int32_t* free_list,
+                       int32_t free_list_len, int32_t* free_head, int32_t* start_positions,
+                       int32_t* dev_error, void* stream) {
+  if (block_size <= 0 || batch < 0 || num_seqs < 0 || max_pages <= 0 || free_list_len < 0)
+    return fail(CVSA_ERR_INVALID, "bad shape");
+  if (batch == 0) return CVSA_OK;
+  if (!cu_tokens || !block_tables || !context_lens || !pages_allocated || !free_list ||
+      !free_head)
+    return fail(CVSA_ERR_INVALID, "NULL pointer");
+  return cuda_status(launch_paged_reserve(cu_tokens, seq_ids, batch, num_seqs, block_size,
+                                          block_tables, max_pages, context_lens, pages_allocated,
+                                          free_list, free_list_len, free_head, start_positions,
+                                          dev_error, (cudaStream_t)stream),
+                     "reserve launch");
+}
+
+int cvsa_rope_append(const cvsa_kv_desc_t* kvd, const cvsa_ragged_desc_t* rgd,
+                     const cvsa_rope_append_t* args, int32_t* dev_error, void* stream) {
+  KvView kv;
+  RaggedView rg;
+  int st = check_kv(kvd, &kv);
+  if (st) return st;
+  st = check_ragged(rgd, &rg);
+  if (st) return st;
+  if (!args) return fail(CVSA_ERR_INVALID, "arguments are NULL");
+  if (!valid_dtype(args->dtype)) return fail(CVSA_ERR_INVALID, "dtype %d unknown", args->dtype);
+  const int hq = args->num_q_heads;
+  if (hq < 0 || (args->q && hq == 0) || (!args->q && hq != 0 && rg.T > 0))
+    return fail(CVSA_ERR_INVALID, "num_q_heads=%d does not fit q", args->num_q_heads);
+  if (rg.T > 0 && (!args->k || !args->v || (hq && !args->q_out)))
+    return fail(CVSA_ERR_INVALID, "k/v/q_out is NULL");
+  if ((args->q_norm || args->k_norm) && args->norm_dtype != args->dtype &&
+      args->norm_dtype != CVSA_DTYPE_F32)
+    return fail(CVSA_ERR_INVALID, "norm weights must have the tokens' dtype or float32");
+  if ((args->q_norm || args->k_norm) && !(args->eps >= 0.f))
+    return fail(CVSA_ERR_INVALID, "eps must be >= 0");
+  if (!rope_append_supported(kv))
+    return fail(CVSA_ERR_UNSUPPORTED, "rope_append built for head_dim 64/128/256");
+  if (args->cos_sin && (args->rot_dim <= 0 || args->rot_dim > kv.d || args->rot_dim % 32 ||
+                        args->max_positions <= 0))
+    return fail(CVSA_ERR_INVALID,
+                "rot_dim=%d must be a multiple of 32 up to head_dim, max_positions=%d positive",
+                args->rot_dim, args->max_positions);
+  const int eb = dtype_bytes(args->dtype);
+  auto aligned = [&](const void* p, int64_t st_tok, int64_t st_head) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (st_tok * eb) % 16 == 0 &&
+           (st_head * eb) % 16 == 0;
+  };
+  if (!aligned(args->k, args->k_stride_token, args->k_stride_head) ||
+      !aligned(args->v, args->v_stride_token, args->v_stride_head) ||
+      (hq && (!aligned(args->q, args->q_stride_token, args->q_stride_head) ||
+              !aligned(args->q_out, args->q_out_stride_token, args->q_out_stride_head))) ||
+      (reinterpret_cast<uintptr_t>(args->cos_sin) | reinterpret_cast<uintptr_t>(args->q_norm) |
+       reinterpret_cast<uintptr_t>(args->k_norm)) % 16)
+    return fail(CVSA_ERR_INVALID, "q/k/v/q_out rows, cos_sin and weights must be 16-byte aligned");
+  if ((int64_t)rg.T * (hq + 2 * (int64_t)kv.hkv) >= (int64_t(1) << 31))
+    return fail(CVSA_ERR_UNSUPPORTED, "num_tokens * heads above 2^31");
+  if (rg.B == 0 || rg.T == 0) return CVSA_OK;
+  RopeView r;
+  r.q = args->q;
+  r.k = args->k;
+  r.v = args->v;
+  r.q_out = args->q_out;
+  r.dtype = args->dtype;
+  r.hq = hq;
+  r.q_st = args->q_stride_token;
+  r.q_sh = args->q_stride_head;
+  r.k_st = args->k_stride_token;
+  r.k_sh = args->k_stride_head;
+  r.v_st = args->v_stride_token;
+  r.v_sh = args->v_stride_head;
+  r.qo_st = args->q_out_stride_token;
+  r.qo_sh = args->q_out_stride_head;
+  r.cos_sin = args->cos_sin;
+  r.max_positions = args->max_positions;
+  r.rot = args->cos_sin ? args->rot_dim : 0;
+  r.interleaved = args->interleaved;
+  r.q_norm = args->q_norm;
+  r.k_norm = args->k_norm;
+  r.norm_f32 = args->norm_dtype == CVSA_DTYPE_F32;
+  r.eps = args->eps;
+  return cuda_status(launch_rope_append(rg, kv, r, dev_error, (cudaStream_t)stream),
+                     "rope_append launch");
+}
+
+size_t cvsa_chunk_attend_workspace_size(const cvsa_kv_desc_t* kvd, const cvsa_ragged_desc_t* rgd,
+                                        const cvsa_chunk_attend_t* args) {
+  KvView kv;
+  RaggedView rg;
+  ChunkView c;
+  if (check_kv(kvd, &kv) || check_ragged(rgd, &rg) || check_chunk(args, kv, rg, &c)) return 0;
+  return chunk_attend_workspace_bytes(kv, rg, c);
+}
+
+int cvsa_chunk_attend(const cvsa_kv_desc_t* kvd, const cvsa_ragged_desc_t* rgd,
+                      const cvsa_chunk_attend_t* args, int32_t* dev_error, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  KvView kv;
+  RaggedView rg;
+  ChunkView c;
+  int st = check_kv(kvd, &kv);
+  if (st) return st;
+  st = check_ragged(rgd, &rg);
+  if (st) return st;
+  st = check_chunk(args, kv, rg, &c);
+  if (st) return st;
+  if (rg.B == 0 || rg.T == 0) return CVSA_OK;
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 ||
+      workspace_bytes < chunk_attend_workspace_bytes(kv, rg, c))
+    return fail(CVSA_ERR_WORKSPACE, "workspace NULL, misaligned or below %zu bytes",
+                chunk_attend_workspace_bytes(kv, rg, c));
+  return cuda_status(launch_chunk_attend(kv, rg, c, workspace, dev_error, (cudaStream_t)stream),
+                     "chunk_attend launch");
 }
 
 }  // extern "C"

@@ -1,0 +1,443 @@
+// Attention of a ragged batch of new tokens over the paged cache: the general
+// kernel (any mix of fp32, bf16, f16) and the merge of split items.
+//
+// Row (token t, query head h) at position p sees keys [lo, hi): hi = p + 1
+// (causal) or the context length, lo = max(0, p - window + 1) or 0.
+//   s_j = scale * q . k_j,  out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),
+//   lse = m + log sum_j e^(s_j - m); a row without a key: out 0, lse -inf.
+// One pass over the keys with a running (m, l, o); a tile that raises m scales
+// l and o once. Masked entries are excluded by selection, never by arithmetic,
+// so values of keys a row does not see cannot reach it, NaN and infinities
+// included.
+//
+// General kernel: one CTA walks its range of items (chunk_plan.cuh), 64 query
+// rows against tiles of 64 keys on the CUDA cores in fp32, each thread a 4 x 4
+// block of scores and 4 x D/16 of the output. It is bound by fp32 FMA issue
+// and serves fp32 caches, mixed types and 256-wide heads; 16-bit caches with
+// 64- and 128-wide heads run in chunk_attend_tc.cu.
+#include <type_traits>
+
+#include "chunk_plan.cuh"
+#include "cvsa_common.cuh"
+#include "cvsa_internal.h"
+#include "cvsa_launch.cuh"
+
+namespace cvsa {
+namespace {
+
+constexpr int kRows = 64, kKeys = 64, kThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct GenArgs {
+  RaggedView rg;
+  KvView kv;
+  ChunkView c;
+  ChunkGeo g;
+  float scale2;        // scale * log2(e)
+  int min_units;
+  float* parts;
+  ChunkMergeDesc* desc;
+  int32_t* dev_err;
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void load_row_piece(const T* src, float* dst) {  // 4 elements
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(src);
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(src);
+    float f[4];
+    if constexpr (std::is_same<T, __half>::value) {
+      f16x2_to_f2(w.x, f[0], f[1]);
+      f16x2_to_f2(w.y, f[2], f[3]);
+    } else {
+      bf16x2_to_f2(w.x, f[0], f[1]);
+      bf16x2_to_f2(w.y, f[2], f[3]);
+    }
+    *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
+  }
+}
+
+template <int D>
+struct GenSmem {
+  float q[kRows][D + 4];
+  float k[kKeys][D + 4];
+  float v[kKeys][D + 4];
+  float p[kRows][kKeys + 4];
+  int64_t key_off[kKeys];   // element offset of a key's row in the pools
+  int8_t key_ok[kKeys];
+  ChunkPlanSmem<kThreads> plan;
+};
+
+template <typename T, typename C, int D>
+__global__ void __launch_bounds__(kThreads) chunk_general_kernel(GenArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  GenSmem<D>& sm = *reinterpret_cast<GenSmem<D>*>(smem_raw);
+  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
+  const int cta = blockIdx.x;
+  const ChunkRange rng = chunk_range<kThreads>(a.rg, a.g, sm.plan, cta, gridDim.x, a.min_units,
+                                               a.dev_err);
+  if (tid == 0) a.desc[cta].parts = 0;
+  __syncthreads();
+  ChunkWalk walk(rng);
+  ChunkItem it;
+  const int G = a.g.G;
+  while (walk.next(a.rg, a.g, it)) {
+    const int rows = (it.t1 - it.t0) * G;
+    // query rows: token t0 + r / G, head h * G + r % G
+    for (int e = tid; e < kRows * (D / 4); e += kThreads) {
+      const int r = e / (D / 4), c = e % (D / 4);
+      float f[4] = {0.f, 0.f, 0.f, 0.f};
+      if (r < rows) {
+        const T* src = reinterpret_cast<const T*>(a.c.q) +
+                       (int64_t)(it.q.tok0 + it.t0 + r / G) * a.c.q_st +
+                       (int64_t)(it.h * G + r % G) * a.c.q_sh + c * 4;
+        load_row_piece<T, D>(src, f);
+      }
+      *reinterpret_cast<float4*>(&sm.q[r][c * 4]) = make_float4(f[0], f[1], f[2], f[3]);
+    }
+    int lo[4], hi[4];
+    float m[4], l[4], o[4][D / 16];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int r = ty * 4 + x;
+      const int pos = it.q.start + it.t0 + r / G;
+      hi[x] = r >= rows ? 0 : a.g.causal ? max(0, min(it.q.ctx, pos + 1)) : it.q.ctx;
+      lo[x] = a.g.window > 0 ? max(0, pos - a.g.window + 1) : 0;
+      m[x] = neg_inf();
+      l[x] = 0.f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) o[x][d] = 0.f;
+    }
+    const int tiles = chunk_tiles(it.lo, it.hi, kKeys);
+    for (int k = it.k0; k < min(it.k1, tiles); ++k) {
+      const int base = (it.tile0 + k) * kKeys;
+      __syncthreads();  // the previous tile's reads are done
+      if (tid < kKeys) {
+        const int key = base + tid;
+        bool ok = key >= it.lo && key < it.hi;
+        int64_t off = 0;
+        if (ok) {
+          const int blk = a.rg.tables[(int64_t)it.q.slot * a.rg.W + key / a.kv.bs];
+          ok = blk >= 0 && blk < a.kv.num_blocks;
+          if (!ok) set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);
+          off = ok ? blk * a.kv.sb + (key % a.kv.bs) * a.kv.st + it.h * a.kv.sh : 0;
+        }
+        sm.key_off[tid] = off;
+        sm.key_ok[tid] = ok;
+      }
+      __syncthreads();
+      for (int e = tid; e < kKeys * (D / 4); e += kThreads) {
+        const int r = e / (D / 4), c = e % (D / 4);
+        float fk[4] = {0.f, 0.f, 0.f, 0.f}, fv[4] = {0.f, 0.f, 0.f, 0.f};
+        if (sm.key_ok[r]) {
+          const int64_t off = sm.key_off[r] + c * 4;
+          load_row_piece<C, D>(reinterpret_cast<const C*>(a.kv.k) + off, fk);
+          load_row_piece<C, D>(reinterpret_cast<const C*>(a.kv.v) + off, fv);
+        }
+        *reinterpret_cast<float4*>(&sm.k[r][c * 4]) = make_float4(fk[0], fk[1], fk[2], fk[3]);
+        *reinterpret_cast<float4*>(&sm.v[r][c * 4]) = make_float4(fv[0], fv[1], fv[2], fv[3]);
+      }
+      __syncthreads();
+      float s[4][4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) s[x][y] = 0.f;
+#pragma unroll 4
+      for (int d = 0; d < D; d += 4) {
+        float4 qa[4], kb[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) qa[x] = *reinterpret_cast<float4*>(&sm.q[ty * 4 + x][d]);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) kb[y] = *reinterpret_cast<float4*>(&sm.k[tx + 16 * y][d]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            s[x][y] = fmaf(qa[x].x, kb[y].x, s[x][y]);
+            s[x][y] = fmaf(qa[x].y, kb[y].y, s[x][y]);
+            s[x][y] = fmaf(qa[x].z, kb[y].z, s[x][y]);
+            s[x][y] = fmaf(qa[x].w, kb[y].w, s[x][y]);
+          }
+      }
+      bool cut = false;  // some row of the block does not see every key of the tile
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float mx = m[x];
+        bool see[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int c = tx + 16 * y, key = base + c;
+          see[y] = key >= lo[x] && key < hi[x] && sm.key_ok[c];
+          cut |= !see[y];
+          s[x][y] = see[y] ? s[x][y] * a.scale2 : neg_inf();
+          if (see[y]) mx = fmaxf(mx, s[x][y]);
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+        const float ref = mx == neg_inf() ? 0.f : mx;
+        const float fix = exp2f(m[x] - ref);  // 0 while the row has seen no key
+        float sum = 0.f;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float p = see[y] ? exp2f(s[x][y] - ref) : 0.f;
+          sum += p;
+          // an unseen key is marked by a negative weight
+          sm.p[ty * 4 + x][tx + 16 * y] = see[y] ? p : -1.f;
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        l[x] = l[x] * fix + sum;
+        m[x] = mx;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) o[x][d] *= fix;
+      }
+      cut = __syncthreads_or(cut);
+#pragma unroll 2
+      for (int c = 0; c < kKeys; ++c) {
+        float p[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) p[x] = sm.p[ty * 4 + x][c];
+        float v[D / 16];
+#pragma unroll
+        for (int y = 0; y < D / 64; ++y)
+          *reinterpret_cast<float4*>(v + 4 * y) =
+              *reinterpret_cast<float4*>(&sm.v[c][tx * 4 + 64 * y]);
+        if (!cut) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) o[x][d] = fmaf(p[x], v[d], o[x][d]);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+              o[x][d] = p[x] >= 0.f || p[x] != p[x] ? fmaf(p[x], v[d], o[x][d]) : o[x][d];
+        }
+      }
+    }
+    // whole items are finished here, pieces go to a partial slot
+    const bool whole = it.k0 == 0 && it.k1 == it.units;
+    if (whole) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int r = ty * 4 + x;
+        if (r >= rows) continue;
+        const int64_t tok = it.q.tok0 + it.t0 + r / G;
+        const int head = it.h * G + r % G;
+        const float inv = l[x] == 0.f ? 0.f : 1.f / l[x];
+        T* dst = reinterpret_cast<T*>(a.c.out) + tok * a.c.o_st + head * a.c.o_sh;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+          dst[(d / 4) * 64 + tx * 4 + d % 4] =
+              Elem<T>::from_f(l[x] == 0.f ? 0.f : o[x][d] * inv);
+        if (a.c.lse && tx == 0)
+          a.c.lse[tok * a.c.hq + head] = l[x] == 0.f ? neg_inf() : (m[x] + log2f(l[x])) * kLn2;
+      }
+    } else {
+      float* part = a.parts + (size_t)chunk_slot(it, rng.u0, cta) * chunk_slot_floats(kRows, D);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int r = ty * 4 + x;
+        if (r >= rows) continue;
+        if (tx == 0) {
+          part[r] = m[x];
+          part[kRows + r] = l[x];
+        }
+        float4* po = reinterpret_cast<float4*>(part + 2 * kRows);
+#pragma unroll
+        for (int y = 0; y < D / 64; ++y)
+          po[(size_t)(tx + 16 * y) * kRows + r] =
+              make_float4(o[x][4 * y], o[x][4 * y + 1], o[x][4 * y + 2], o[x][4 * y + 3]);
+      }
+      if (tid == 0 && it.k0 == 0) {
+        ChunkMergeDesc d;
+        d.parts = (int)((it.first + it.units - 1) / rng.per_cta) - cta + 1;
+        d.tok = it.q.tok0 + it.t0;
+        d.rows = rows;
+        d.head = it.h;
+        a.desc[cta] = d;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, typename C>
+cudaError_t launch_general_d(const GenArgs& a, int ctas, cudaStream_t s) {
+  auto go = [&](auto kernel, size_t smem) -> cudaError_t {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)smem);
+    if (e != cudaSuccess) return e;
+    kernel<<<ctas, kThreads, smem, s>>>(a);
+    return cudaGetLastError();
+  };
+  switch (a.kv.d) {
+    case 64: return go(chunk_general_kernel<T, C, 64>, sizeof(GenSmem<64>));
+    case 128: return go(chunk_general_kernel<T, C, 128>, sizeof(GenSmem<128>));
+    case 256: return go(chunk_general_kernel<T, C, 256>, sizeof(GenSmem<256>));
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+template <typename T>
+cudaError_t launch_general_c(const GenArgs& a, int ctas, cudaStream_t s) {
+  switch (a.kv.dtype) {
+    case CVSA_DTYPE_BF16: return launch_general_d<T, __nv_bfloat16>(a, ctas, s);
+    case CVSA_DTYPE_F16: return launch_general_d<T, __half>(a, ctas, s);
+    default: return launch_general_d<T, float>(a, ctas, s);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// merge of split items
+// ---------------------------------------------------------------------------
+// Block (x, y): rows [32 x, 32 x + 32) of the item that begins in CTA y's range
+// and leaves it. Lanes own rows, warps own float4 columns. Parts are summed in
+// CTA order. Most blocks find no item and leave at once.
+constexpr int kMaxCtas = 256;
+
+struct MergeArgs {
+  const float* parts;
+  const ChunkMergeDesc* desc;
+  ChunkView c;
+  int rows, G, d;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) chunk_merge_kernel(MergeArgs a) {
+  __shared__ float w[kMaxCtas][32];  // weight of each part, then of the output
+  __shared__ float red[8][32];
+  pdl_wait();
+  const int cta = blockIdx.y;
+  const ChunkMergeDesc ds = a.desc[cta];
+  const int r0 = blockIdx.x * 32;
+  if (ds.parts == 0 || r0 >= ds.rows) return;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int r = r0 + lane;
+  const size_t slot_floats = chunk_slot_floats(a.rows, a.d);
+  auto slot = [&](int p) {
+    return a.parts + (size_t)(p == 0 ? 2 * cta + 1 : 2 * (cta + p)) * slot_floats;
+  };
+  const bool live = r < ds.rows;
+  float mx = neg_inf();
+  for (int p = wid; p < ds.parts; p += 8) {
+    const float m = live ? slot(p)[r] : neg_inf();
+    w[p][lane] = m;
+    mx = fmaxf(mx, m);
+  }
+  red[wid][lane] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) mx = fmaxf(mx, red[i][lane]);
+  __syncthreads();
+  const float ref = mx == neg_inf() ? 0.f : mx;
+  float l = 0.f;
+  for (int p = wid; p < ds.parts; p += 8) {
+    const float e = exp2f(w[p][lane] - ref);
+    w[p][lane] = e;
+    l += live ? e * slot(p)[a.rows + r] : 0.f;
+  }
+  red[wid][lane] = l;
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) l += red[i][lane];
+  if (!live) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t tok = ds.tok + r / a.G;
+  const int head = ds.head * a.G + r % a.G;
+  T* dst = reinterpret_cast<T*>(a.c.out) + tok * a.c.o_st + head * a.c.o_sh;
+  for (int c = wid; c < a.d / 4; c += 8) {
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int p = 0; p < ds.parts; ++p) {
+      const float4 v = reinterpret_cast<const float4*>(slot(p) + 2 * a.rows)[(size_t)c * a.rows + r];
+      const float e = w[p][lane];
+      // a part whose rows saw no key holds o = 0 and weighs 0
+      o.x = fmaf(e, v.x, o.x);
+      o.y = fmaf(e, v.y, o.y);
+      o.z = fmaf(e, v.z, o.z);
+      o.w = fmaf(e, v.w, o.w);
+    }
+    if (l == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<float4*>(dst + c * 4) =
+          make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    else
+      *reinterpret_cast<uint2*>(dst + c * 4) =
+          make_uint2(Mma<T>::pack(o.x * inv, o.y * inv), Mma<T>::pack(o.z * inv, o.w * inv));
+  }
+  if (a.c.lse && wid == 0)
+    a.c.lse[tok * a.c.hq + head] = l == 0.f ? neg_inf() : (mx + log2f(l)) * kLn2;
+}
+
+// ---------------------------------------------------------------------------
+// workspace: [merge descriptors][partial slots]
+// ---------------------------------------------------------------------------
+constexpr size_t kDescBytes = ((kMaxCtas * sizeof(ChunkMergeDesc) + 255) / 256) * 256;
+
+int chunk_ctas() { return num_sms() < kMaxCtas ? num_sms() : kMaxCtas; }
+
+ChunkGeo general_geo(const KvView& kv, const ChunkView& c) {
+  ChunkGeo g;
+  g.bs = kv.bs;
+  g.hkv = kv.hkv;
+  g.G = c.hq / kv.hkv;
+  g.P = kRows / g.G;
+  g.KT = kKeys;
+  g.causal = c.causal;
+  g.window = c.window;
+  return g;
+}
+
+}  // namespace
+
+bool chunk_attend_supported(const KvView& kv, const ChunkView& c) {
+  return (kv.d == 64 || kv.d == 128 || kv.d == 256) && c.hq / kv.hkv <= kRows;
+}
+
+size_t chunk_attend_workspace_bytes(const KvView& kv, const RaggedView& rg, const ChunkView& c) {
+  return kDescBytes + 2 * (size_t)chunk_ctas() * chunk_slot_floats(kRows, kv.d) * 4;
+}
+
+cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const ChunkView& c,
+                                void* ws, int32_t* dev_err, cudaStream_t s) {
+  const int ctas = chunk_ctas();
+  GenArgs a;
+  a.rg = rg;
+  a.kv = kv;
+  a.c = c;
+  a.g = general_geo(kv, c);
+  a.scale2 = c.scale * kLog2e;
+  a.min_units = 2;
+  a.desc = reinterpret_cast<ChunkMergeDesc*>(ws);
+  a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kDescBytes);
+  a.dev_err = dev_err;
+  cudaError_t e;
+  switch (c.dtype) {
+    case CVSA_DTYPE_BF16: e = launch_general_c<__nv_bfloat16>(a, ctas, s); break;
+    case CVSA_DTYPE_F16: e = launch_general_c<__half>(a, ctas, s); break;
+    default: e = launch_general_c<float>(a, ctas, s); break;
+  }
+  if (e != cudaSuccess) return e;
+  MergeArgs m;
+  m.parts = a.parts;
+  m.desc = a.desc;
+  m.c = c;
+  m.rows = kRows;
+  m.G = a.g.G;
+  m.d = kv.d;
+  const dim3 grid((kRows + 31) / 32, ctas);
+  switch (c.dtype) {
+    case CVSA_DTYPE_BF16:
+      return launch_k(chunk_merge_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, true, m);
+    case CVSA_DTYPE_F16:
+      return launch_k(chunk_merge_kernel<__half>, grid, dim3(256), 0, s, true, m);
+    default: return launch_k(chunk_merge_kernel<float>, grid, dim3(256), 0, s, true, m);
+  }
+}
+
+}  // namespace cvsa

@@ -247,4 +247,48 @@ cudaError_t launch_paged_append(const KvView& kv, const void* k_new, const void*
 cudaError_t launch_paged_gather(const KvView& kv, const int32_t* row, int n_pages, void* k_out,
                                 void* v_out, int32_t* dev_err, cudaStream_t s);
 
+// ---- ragged batches of new tokens (rope_append.cu, chunk_attend.cu) ----
+struct RaggedView {
+  const int32_t* cu;       // [B + 1] token offsets
+  const int32_t* seq_ids;  // [B] rows of the tables, or null (row b)
+  const int32_t* starts;   // [B] first new position (-1: refused), or null (length - count)
+  const int32_t* tables;   // [num_seqs, W]
+  const int32_t* lens;     // [num_seqs], with the new tokens
+  int B, T, num_seqs, W;
+};
+
+// ---- rope_append.cu ----
+struct RopeView {
+  const void* q; const void* k; const void* v;
+  void* q_out;
+  int dtype, hq;           // hq = 0: no queries
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh;  // element strides: token, head
+  const float* cos_sin;    // [max_positions, rot]: cosines, then sines; or null
+  int max_positions, rot, interleaved;
+  const void* q_norm; const void* k_norm;  // [head_dim] or null
+  int norm_f32;            // weights are float32 (else dtype)
+  float eps;
+};
+cudaError_t launch_paged_reserve(const int32_t* cu, const int32_t* seq_ids, int B, int num_seqs,
+                                 int bs, int32_t* tables, int W, int32_t* lens,
+                                 int32_t* pages_alloc, const int32_t* free_list, int free_len,
+                                 int32_t* free_head, int32_t* starts, int32_t* dev_err,
+                                 cudaStream_t s);
+bool rope_append_supported(const KvView& kv);
+cudaError_t launch_rope_append(const RaggedView& rg, const KvView& kv, const RopeView& r,
+                               int32_t* dev_err, cudaStream_t s);
+
+// ---- chunk_attend.cu (any supported type), chunk_attend_tc.cu (16-bit, tensor cores) ----
+struct ChunkView {
+  const void* q; void* out; float* lse;   // lse [T, hq] or null
+  int dtype, hq;
+  int64_t q_st, q_sh, o_st, o_sh;         // element strides: token, head
+  float scale;
+  int causal, window;                     // window 0: none
+};
+size_t chunk_attend_workspace_bytes(const KvView& kv, const RaggedView& rg, const ChunkView& c);
+bool chunk_attend_supported(const KvView& kv, const ChunkView& c);
+cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const ChunkView& c,
+                                void* ws, int32_t* dev_err, cudaStream_t s);
+
 }  // namespace cvsa

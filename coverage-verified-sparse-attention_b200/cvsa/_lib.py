@@ -32,8 +32,8 @@ NUM_COUNTERS = 8
 EV_SCORE_BEGIN, EV_SCORE_END, EV_SELECT_BEGIN, EV_SELECT_END, EV_ATTEND_BEGIN, EV_ATTEND_END = (
     range(6))
 NUM_EVENTS = 6
-DEV_ERR_BLOCK_RANGE, DEV_ERR_PAGE_RANGE, DEV_ERR_POOL, DEV_ERR_TABLE_FULL, DEV_ERR_TIMEOUT = (
-    1, 2, 4, 8, 16)
+(DEV_ERR_BLOCK_RANGE, DEV_ERR_PAGE_RANGE, DEV_ERR_POOL, DEV_ERR_TABLE_FULL, DEV_ERR_TIMEOUT,
+ DEV_ERR_RAGGED) = (1, 2, 4, 8, 16, 32)
 
 _TORCH_TO_DT = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
 
@@ -94,6 +94,41 @@ class PeerDesc(ctypes.Structure):
     ]
 
 
+class RaggedDesc(ctypes.Structure):
+    _fields_ = [
+        ("cu_tokens", ctypes.c_void_p), ("seq_ids", ctypes.c_void_p),
+        ("start_positions", ctypes.c_void_p), ("block_tables", ctypes.c_void_p),
+        ("context_lens", ctypes.c_void_p), ("batch", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32), ("num_seqs", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+    ]
+
+
+class RopeAppend(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("num_q_heads", ctypes.c_int32),
+        ("q_stride_token", ctypes.c_int64), ("q_stride_head", ctypes.c_int64),
+        ("k_stride_token", ctypes.c_int64), ("k_stride_head", ctypes.c_int64),
+        ("v_stride_token", ctypes.c_int64), ("v_stride_head", ctypes.c_int64),
+        ("q_out_stride_token", ctypes.c_int64), ("q_out_stride_head", ctypes.c_int64),
+        ("cos_sin", ctypes.c_void_p), ("max_positions", ctypes.c_int32),
+        ("rot_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+        ("norm_dtype", ctypes.c_int32), ("q_norm", ctypes.c_void_p),
+        ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float),
+    ]
+
+
+class ChunkAttend(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32), ("num_q_heads", ctypes.c_int32),
+        ("q_stride_token", ctypes.c_int64), ("q_stride_head", ctypes.c_int64),
+        ("out_stride_token", ctypes.c_int64), ("out_stride_head", ctypes.c_int64),
+        ("scale", ctypes.c_float), ("causal", ctypes.c_int32), ("window", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
 _SIGS = {
@@ -143,6 +178,15 @@ _SIGS = {
     "cvsa_paged_append": ([ctypes.POINTER(KvDesc), _P, _P, _I, _P, _P, _I, _P, _P, _P, _I, _P, _P,
                            _P], ctypes.c_int),
     "cvsa_paged_gather": ([ctypes.POINTER(KvDesc), _P, _I, _P, _P, _P, _P], ctypes.c_int),
+    "cvsa_paged_reserve": ([_I, _P, _P, _I, _I, _P, _I, _P, _P, _P, _I, _P, _P, _P, _P],
+                           ctypes.c_int),
+    "cvsa_rope_append": ([ctypes.POINTER(KvDesc), ctypes.POINTER(RaggedDesc),
+                          ctypes.POINTER(RopeAppend), _P, _P], ctypes.c_int),
+    "cvsa_chunk_attend_workspace_size": ([ctypes.POINTER(KvDesc), ctypes.POINTER(RaggedDesc),
+                                          ctypes.POINTER(ChunkAttend)], ctypes.c_size_t),
+    "cvsa_chunk_attend": ([ctypes.POINTER(KvDesc), ctypes.POINTER(RaggedDesc),
+                           ctypes.POINTER(ChunkAttend), _P, _P, ctypes.c_size_t, _P],
+                          ctypes.c_int),
     "cvsa_sparse_decode_noalloc": ([ctypes.POINTER(QueryDesc), ctypes.POINTER(KvDesc), _P, _I, _P,
                                     _P, _P, _P, _P, _I, _P], ctypes.c_int),
 }
@@ -255,6 +299,38 @@ def query_desc(q: Optional[torch.Tensor], block_tables: torch.Tensor,
                          block_tables.data_ptr(), context_lens.data_ptr())
     return QueryDesc(None, DTYPE_BF16, B, num_q_heads or 1, W, block_tables.data_ptr(),
                      context_lens.data_ptr())
+
+
+def ragged_desc(num_tokens: int, cu_tokens: torch.Tensor, block_tables: torch.Tensor,
+                context_lens: torch.Tensor, seq_ids: Optional[torch.Tensor],
+                start_positions: Optional[torch.Tensor]) -> RaggedDesc:
+    """The packed new tokens of a batch and the tables of the sequences they belong to."""
+    for t in (cu_tokens, block_tables, context_lens, seq_ids, start_positions):
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            raise ValueError("cu_tokens, block_tables, context_lens, seq_ids and "
+                             "start_positions must be contiguous int32")
+    if block_tables.dim() != 2 or cu_tokens.dim() != 1 or cu_tokens.shape[0] < 1:
+        raise ValueError("block_tables must be [num_seqs, max_pages], cu_tokens [batch + 1]")
+    B = cu_tokens.shape[0] - 1
+    S, W = block_tables.shape
+    if context_lens.shape != (S,):
+        raise ValueError("context_lens must be [num_seqs]")
+    for t in (seq_ids, start_positions):
+        if t is not None and t.shape != (B,):
+            raise ValueError("seq_ids and start_positions must be [batch]")
+    return RaggedDesc(cu_tokens.data_ptr(), ptr(seq_ids), ptr(start_positions),
+                      block_tables.data_ptr(), context_lens.data_ptr(), B, num_tokens, S, W)
+
+
+def token_rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    """A [num_tokens, heads, head_dim] view the kernels can read: 16-byte rows (copied if not)."""
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [num_tokens, heads, head_dim]")
+    eb = t.element_size()
+    if t.numel() and (t.stride(2) != 1 or t.data_ptr() % 16 or (t.stride(0) * eb) % 16
+                      or (t.stride(1) * eb) % 16 or t.stride(0) < 0 or t.stride(1) < 0):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
 
 
 class Workspace:

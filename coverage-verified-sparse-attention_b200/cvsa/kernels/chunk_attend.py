@@ -1,0 +1,57 @@
+"""Attention of a ragged batch of new tokens over the paged cache.
+
+`chunk_attention` serves a prompt, a chunk of one, drafted tokens to verify,
+or one token for each sequence, in any mix: sequence b owns tokens
+cu_tokens[b]..cu_tokens[b + 1] of q, and they attend to everything the
+sequence has cached up to themselves (csrc/chunk_attend_tc.cu,
+csrc/chunk_attend.cu). The reference computes prompts in the model library
+(eval/latency_benchmark.py:376-420) and has no counterpart.
+"""
+
+from typing import Optional
+
+import torch
+
+from cvsa import _lib
+
+
+def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_tables: torch.Tensor, context_lens: torch.Tensor,
+                    cu_tokens: torch.Tensor, causal: bool = True, window: int = 0,
+                    scale: Optional[float] = None, seq_ids: Optional[torch.Tensor] = None,
+                    start_positions: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                    dev_error: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale q K^T) V per new token and query head, [T, H_q, D] in q's dtype.
+
+    q [T, H_q, D]; the pools, tables [num_seqs, max_pages] and lengths
+    [num_seqs] are those of the decode step, with the new tokens already in
+    (`rope_append`); scale defaults to D^-0.5. causal: a token sees its
+    sequence up to itself, of which the last `window` keys if window > 0;
+    otherwise all of it. lse, if given, is a float32 [T, H_q] tensor to fill
+    with the log-sum-exp of each row's scaled scores (for a merge with
+    attention over other keys). A row that sees no key gives 0 and -inf.
+    """
+    dev = _lib.require_cuda(q, k_cache, v_cache, block_tables, context_lens, cu_tokens, seq_ids,
+                            start_positions, out, lse, dev_error)
+    q = _lib.token_rows(q, "q")
+    T, Hq, D = q.shape
+    if k_cache.dim() != 4 or k_cache.shape[3] != D:
+        raise ValueError("q's head_dim does not match the cache")
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError("out must have q's shape and dtype and contiguous rows")
+    if lse is not None and (lse.shape != (T, Hq) or lse.dtype != torch.float32
+                            or not lse.is_contiguous()):
+        raise ValueError("lse must be a contiguous float32 [T, H_q]")
+    kvd = _lib.kv_desc(k_cache, v_cache)
+    rg = _lib.ragged_desc(T, cu_tokens, block_tables, context_lens, seq_ids, start_positions)
+    args = _lib.ChunkAttend(q.data_ptr(), out.data_ptr(), _lib.ptr(lse), _lib.dtype_code(q.dtype),
+                            Hq, q.stride(0), q.stride(1), out.stride(0), out.stride(1),
+                            D ** -0.5 if scale is None else scale, int(causal), window)
+    lib = _lib.load()
+    ws = _lib.WORKSPACE.get(lib.cvsa_chunk_attend_workspace_size(kvd, rg, args), dev, "chunk")
+    _lib.check(lib.cvsa_chunk_attend(kvd, rg, args, _lib.ptr(dev_error), ws.data_ptr(),
+                                     ws.numel(), _lib.stream_ptr(dev)), "cvsa_chunk_attend")
+    return out

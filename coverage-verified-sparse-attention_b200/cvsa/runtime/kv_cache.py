@@ -157,6 +157,35 @@ class SequenceKVManager:
         ids = self._seq_ids[:k.shape[0]] if seq_ids is None else seq_ids.to(torch.int32)
         self._append(k, v, ids)
 
+    def reserve(self, cu_tokens: torch.Tensor,
+                seq_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Grow sequence seq_ids[b] (default b) by cu_tokens[b + 1] - cu_tokens[b] tokens.
+
+        Pops the pages they need and advances the context lengths, on the
+        device. Returns the start positions [batch] for `rope_append` and
+        `chunk_attention`; a sequence that does not fit (its table or the pool)
+        keeps its state and gets -1, and `cache.check()` raises."""
+        c = self.cache
+        dev = _lib.require_cuda(cu_tokens, seq_ids, c.k_cache)
+        cu = cu_tokens.to(torch.int32).contiguous()
+        if cu.dim() != 1 or cu.shape[0] < 1:
+            raise ValueError("cu_tokens must be [batch + 1]")
+        n = cu.shape[0] - 1
+        if seq_ids is not None:
+            seq_ids = seq_ids.to(torch.int32).contiguous()
+            if seq_ids.shape != (n,):
+                raise ValueError("seq_ids must be [batch]")
+        elif n > self.batch_size:
+            raise ValueError(f"{n} sequences but {self.batch_size} table rows")
+        starts = torch.empty((n,), dtype=torch.int32, device=dev)
+        _lib.check(_lib.load().cvsa_paged_reserve(
+            self.block_size, cu.data_ptr(), _lib.ptr(seq_ids), n, self.batch_size,
+            self.block_tables.data_ptr(), self.max_pages, self.context_lens.data_ptr(),
+            self.pages_allocated.data_ptr(), c.free_list.data_ptr(), c.free_list.numel(),
+            c.free_head.data_ptr(), starts.data_ptr(), c.dev_error.data_ptr(),
+            _lib.stream_ptr(dev)), "cvsa_paged_reserve")
+        return starts
+
     def _append(self, k, v, ids):
         c = self.cache
         _lib.require_cuda(k, v, c.k_cache)

@@ -64,7 +64,9 @@ enum {
   CVSA_DEV_ERR_PAGE_RANGE = 2,  /* a page index outside [0, max_pages) */
   CVSA_DEV_ERR_POOL = 4,        /* append: free list exhausted */
   CVSA_DEV_ERR_TABLE_FULL = 8,  /* append: sequence longer than the table */
-  CVSA_DEV_ERR_TIMEOUT = 16     /* a bounded wait (async copy, peer rank) gave up */
+  CVSA_DEV_ERR_TIMEOUT = 16,    /* a bounded wait (async copy, peer rank) gave up */
+  CVSA_DEV_ERR_RAGGED = 32      /* a ragged batch's offsets, table rows, lengths or
+                                   positions out of range */
 };
 
 /* Paged KV pool: [num_blocks, block_size, num_kv_heads, head_dim].
@@ -509,6 +511,104 @@ int cvsa_paged_append(const cvsa_kv_desc_t* kv, const void* k_new, const void* v
 int cvsa_paged_gather(const cvsa_kv_desc_t* kv, const int32_t* block_table_row,
                       int32_t n_pages, void* k_out, void* v_out, int32_t* dev_error,
                       void* stream);
+
+/* ---- new tokens of a ragged batch (no counterpart in the reference, whose
+ * prompts run in the model library, eval/latency_benchmark.py:376-420) -------
+ * A prompt, a chunk of one, drafted tokens to verify, or one token for each
+ * sequence: the batch's new tokens are packed in one array, sequence b owning
+ * tokens cu_tokens[b] .. cu_tokens[b + 1]. All arrays are on the device and
+ * no call reads them on the host, so the calls can be captured in a CUDA
+ * graph; tokens at or past cu_tokens[batch] (padding) are not touched. A
+ * sequence may appear once in a batch. Per layer:
+ *   cvsa_paged_reserve -> cvsa_rope_append -> cvsa_chunk_attend.
+ * Entries out of range never trap: they set CVSA_DEV_ERR_RAGGED or
+ * CVSA_DEV_ERR_BLOCK_RANGE in *dev_error (nullable) and the token, row or key
+ * is skipped. */
+typedef struct cvsa_ragged_desc {
+  const int32_t* cu_tokens;       /* [batch + 1], non-decreasing, from 0 */
+  const int32_t* seq_ids;         /* [batch] rows of the tables, or NULL: row b */
+  const int32_t* start_positions; /* [batch] position of the first new token, -1: the
+                                     sequence was refused (cvsa_paged_reserve) and is
+                                     skipped; or NULL: length - number of new tokens */
+  const int32_t* block_tables;    /* [num_seqs, max_pages] */
+  const int32_t* context_lens;    /* [num_seqs], counting the new tokens */
+  int32_t batch;
+  int32_t num_tokens;             /* rows of the packed arrays (>= cu_tokens[batch]) */
+  int32_t num_seqs;
+  int32_t max_pages;
+} cvsa_ragged_desc_t;
+
+/* Pages for the new tokens: sequence b's length grows by its number of new
+ * tokens; pages starting at or past its old length and past pages_allocated
+ * are popped from the free list in batch order and written to its table.
+ * A sequence is granted all its pages or none: one that would pass its table
+ * (CVSA_DEV_ERR_TABLE_FULL) or the free list (CVSA_DEV_ERR_POOL; then no later
+ * sequence of the batch gets new pages either) keeps its state.
+ * start_positions [batch] (nullable): the old length, or -1 if refused.
+ * The batched form of kv_cache.py:53-62 and :102-131. */
+int cvsa_paged_reserve(int32_t block_size, const int32_t* cu_tokens, const int32_t* seq_ids,
+                       int32_t batch, int32_t num_seqs, int32_t* block_tables,
+                       int32_t max_pages, int32_t* context_lens, int32_t* pages_allocated,
+                       const int32_t* free_list, int32_t free_list_len, int32_t* free_head,
+                       int32_t* start_positions, int32_t* dev_error, void* stream);
+
+typedef struct cvsa_rope_append {
+  const void* q;          /* [num_tokens, num_q_heads, head_dim] or NULL */
+  const void* k;          /* [num_tokens, num_kv_heads, head_dim] */
+  const void* v;
+  void* q_out;            /* like q; may be q itself with q's strides */
+  int32_t dtype;          /* of q, k, v, q_out; the pool may have another */
+  int32_t num_q_heads;    /* 0 without q */
+  int64_t q_stride_token, q_stride_head;       /* element strides; head_dim is contiguous */
+  int64_t k_stride_token, k_stride_head;
+  int64_t v_stride_token, v_stride_head;
+  int64_t q_out_stride_token, q_out_stride_head;
+  const float* cos_sin;   /* [max_positions, rot_dim]: rot_dim / 2 cosines, then the sines;
+                             NULL: no rotation */
+  int32_t max_positions;
+  int32_t rot_dim;        /* a multiple of 32 up to head_dim; elements past it pass through */
+  int32_t interleaved;    /* pairs (2i, 2i + 1) instead of (i, i + rot_dim / 2) */
+  int32_t norm_dtype;     /* of the weights: dtype or CVSA_DTYPE_F32 */
+  const void* q_norm;     /* [head_dim] weights of the RMS norm of each query row, or NULL */
+  const void* k_norm;     /* the same for key rows */
+  float eps;
+} cvsa_rope_append_t;
+
+/* Norm and rotate the new tokens' queries and keys, write the queries to
+ * q_out and the keys and values to the slots of their positions, in one pass:
+ * x^ = x * rsqrt(mean(x^2) + eps) * w, then each pair (x, y) turned by
+ * (cos, sin) of its position; fp32 throughout, rounded once. Query rows of a
+ * skipped token are 0. The reservation must be made before. */
+int cvsa_rope_append(const cvsa_kv_desc_t* kv, const cvsa_ragged_desc_t* rg,
+                     const cvsa_rope_append_t* args, int32_t* dev_error, void* stream);
+
+typedef struct cvsa_chunk_attend {
+  const void* q;          /* [num_tokens, num_q_heads, head_dim] */
+  void* out;              /* the same shape and dtype */
+  float* lse;             /* [num_tokens, num_q_heads] natural log, or NULL */
+  int32_t dtype;
+  int32_t num_q_heads;
+  int64_t q_stride_token, q_stride_head;
+  int64_t out_stride_token, out_stride_head;
+  float scale;            /* > 0, finite */
+  int32_t causal;         /* 1: a token sees its sequence up to itself; 0: all of it */
+  int32_t window;         /* causal only: keys a token sees, itself included; 0: no limit */
+} cvsa_chunk_attend_t;
+
+size_t cvsa_chunk_attend_workspace_size(const cvsa_kv_desc_t* kv, const cvsa_ragged_desc_t* rg,
+                                        const cvsa_chunk_attend_t* args);
+
+/* Attention of the new tokens over the paged keys and values of their
+ * sequences: out = softmax(scale q K^T) V per token and query head, lse the
+ * log-sum-exp of the scaled scores; a row that sees no key yields 0 and -inf.
+ * Keys a row does not see never reach it, whatever they hold. fp32 softmax
+ * and accumulation; with a 16-bit pool of q's dtype and head_dim 64 or 128
+ * the products run on the tensor cores with the weights rounded to that
+ * dtype. head_dim 64, 128 or 256, up to 64 query heads a KV head, any
+ * block_size. The workspace is not read before it is written. */
+int cvsa_chunk_attend(const cvsa_kv_desc_t* kv, const cvsa_ragged_desc_t* rg,
+                      const cvsa_chunk_attend_t* args, int32_t* dev_error, void* workspace,
+                      size_t workspace_bytes, void* stream);
 
 /* ---- allocation-free decode ------------------------------------------ */
 
