@@ -400,37 +400,45 @@ bool chunk_attend_supported(const KvView& kv, const ChunkView& c) {
 }
 
 size_t chunk_attend_workspace_bytes(const KvView& kv, const RaggedView& rg, const ChunkView& c) {
-  return kDescBytes + 2 * (size_t)chunk_ctas() * chunk_slot_floats(kRows, kv.d) * 4;
+  const int rows = chunk_tc_eligible(kv, c) ? chunk_tc_rows() : kRows;
+  return kDescBytes + 2 * (size_t)chunk_ctas() * chunk_slot_floats(rows, kv.d) * 4;
 }
 
 cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const ChunkView& c,
                                 void* ws, int32_t* dev_err, cudaStream_t s) {
   const int ctas = chunk_ctas();
-  GenArgs a;
-  a.rg = rg;
-  a.kv = kv;
-  a.c = c;
-  a.g = general_geo(kv, c);
-  a.scale2 = c.scale * kLog2e;
-  a.min_units = 2;
-  a.desc = reinterpret_cast<ChunkMergeDesc*>(ws);
-  a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kDescBytes);
-  a.dev_err = dev_err;
+  ChunkMergeDesc* desc = reinterpret_cast<ChunkMergeDesc*>(ws);
+  float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kDescBytes);
+  const bool tc = chunk_tc_eligible(kv, c);
   cudaError_t e;
-  switch (c.dtype) {
-    case CVSA_DTYPE_BF16: e = launch_general_c<__nv_bfloat16>(a, ctas, s); break;
-    case CVSA_DTYPE_F16: e = launch_general_c<__half>(a, ctas, s); break;
-    default: e = launch_general_c<float>(a, ctas, s); break;
+  if (tc) {
+    e = launch_chunk_tc(kv, rg, c, ctas, parts, desc, dev_err, s);
+  } else {
+    GenArgs a;
+    a.rg = rg;
+    a.kv = kv;
+    a.c = c;
+    a.g = general_geo(kv, c);
+    a.scale2 = c.scale * kLog2e;
+    a.min_units = 2;
+    a.desc = desc;
+    a.parts = parts;
+    a.dev_err = dev_err;
+    switch (c.dtype) {
+      case CVSA_DTYPE_BF16: e = launch_general_c<__nv_bfloat16>(a, ctas, s); break;
+      case CVSA_DTYPE_F16: e = launch_general_c<__half>(a, ctas, s); break;
+      default: e = launch_general_c<float>(a, ctas, s); break;
+    }
   }
   if (e != cudaSuccess) return e;
   MergeArgs m;
-  m.parts = a.parts;
-  m.desc = a.desc;
+  m.parts = parts;
+  m.desc = desc;
   m.c = c;
-  m.rows = kRows;
-  m.G = a.g.G;
+  m.rows = tc ? chunk_tc_rows() : kRows;
+  m.G = c.hq / kv.hkv;
   m.d = kv.d;
-  const dim3 grid((kRows + 31) / 32, ctas);
+  const dim3 grid((m.rows + 31) / 32, ctas);
   switch (c.dtype) {
     case CVSA_DTYPE_BF16:
       return launch_k(chunk_merge_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, true, m);

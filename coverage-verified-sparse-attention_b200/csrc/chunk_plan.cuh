@@ -264,4 +264,10 @@ __device__ __forceinline__ int chunk_slot(const ChunkItem& it, long long u0, int
   return 2 * cta + (it.first < u0 ? 0 : 1);
 }
 
+// ---- chunk_attend_tc.cu ----
+bool chunk_tc_eligible(const KvView& kv, const ChunkView& c);
+int chunk_tc_rows();  // query rows of an item at most (a partial slot's rows)
+cudaError_t launch_chunk_tc(const KvView& kv, const RaggedView& rg, const ChunkView& c, int ctas,
+                            float* parts, ChunkMergeDesc* desc, int32_t* dev_err, cudaStream_t s);
+
 }  // namespace cvsa
