@@ -127,71 +127,46 @@ __device__ __forceinline__ bool tile_partial(const ChunkItem& it, const ChunkGeo
 // ---------------------------------------------------------------------------
 // loading warps
 // ---------------------------------------------------------------------------
+// A copy's arrival on its buffer's barrier is left to the hardware
+// (cp.async.mbarrier.arrive), so these warps never wait for their own copies,
+// and the proxy fence the tensor core needs is the MMA thread's: a fence in a
+// thread with copies in flight waits for all of them (2500 cycles a buffer).
+__device__ __forceinline__ void arrive_when_landed(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+
 template <typename T, int D>
 struct Loader {
   using C = Cfg<D>;
   static constexpr int kCh = D / 8;           // 16-byte chunks a row
   static constexpr int kRPI = 32 / kCh;       // rows a warp instruction
-  static constexpr int kLag = 2;              // copy groups in flight behind the newest
   const TcArgs& a;
   TcMeta* m;
   uint32_t base;    // shared memory base
   int w, lane;
-  // copy groups not signalled yet, oldest first
-  uint64_t* bar[kLag + 1];
-  uint32_t chk[kLag + 1];    // 0, or the V stage's address | tile slot + 1
-  int np;
 
   __device__ Loader(const TcArgs& a_, TcMeta* m_, uint32_t base_, int w_, int lane_)
-      : a(a_), m(m_), base(base_), w(w_), lane(lane_), np(0) {}
+      : a(a_), m(m_), base(base_), w(w_), lane(lane_) {}
 
   __device__ __forceinline__ uint32_t dst(uint32_t tile, int row, int ch) const {
     return tile + (ch >> 3) * C::kPanel + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
   }
-
-  // The oldest group has landed: check it if asked, make it visible to the
-  // tensor core, signal.
-  __device__ __forceinline__ void signal_oldest() {
-    cp_async_wait_dyn(np - 1);
-    if (chk[0]) {
-      const uint32_t tile = chk[0] & ~1023u, slot = (chk[0] & 1023u) - 1;
-      bool odd = false;
-      const int ch = lane % kCh;
-      for (int i = 0; i < 32 / kRPI; ++i) {
-        const int row = w * 32 + i * kRPI + lane / kCh;
-        uint32_t x[4];
-        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                     : "r"(dst(tile, row, ch)));
-        constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  // Whether this warp's rows of a V tile hold a value that is not finite.
+  __device__ __forceinline__ bool has_odd(uint32_t tile) const {
+    bool odd = false;
+    const int ch = lane % kCh;
+    for (int i = 0; i < 32 / kRPI; ++i) {
+      const int row = w * 32 + i * kRPI + lane / kCh;
+      uint32_t x[4];
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                   : "r"(dst(tile, row, ch)));
+      constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) odd |= __vcmpgeu2(x[j] & 0x7fff7fffu, kExp) != 0;
-      }
-      odd = __any_sync(0xffffffffu, odd);
-      if (lane == 0) m->v_odd[slot][w] = odd;
+      for (int j = 0; j < 4; ++j) odd |= __vcmpgeu2(x[j] & 0x7fff7fffu, kExp) != 0;
     }
-    fence_proxy_async_smem();
-    mbar_arrive(bar[0]);
-    --np;
-#pragma unroll
-    for (int i = 0; i < kLag; ++i) { bar[i] = bar[i + 1]; chk[i] = chk[i + 1]; }
-  }
-  __device__ __forceinline__ void pushed(uint64_t* full, uint32_t check) {
-    cp_async_commit();
-#pragma unroll
-    for (int i = 0; i <= kLag; ++i)
-      if (i == np) { bar[i] = full; chk[i] = check; }
-    if (++np > kLag) signal_oldest();
-  }
-  __device__ __forceinline__ void flush() {
-    while (np) signal_oldest();
-  }
-  // A buffer to be free. What is in flight is signalled before blocking: the
-  // buffer may be waiting for it.
-  __device__ __forceinline__ bool acquire(uint64_t* bar_empty, uint32_t parity) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar_empty, parity))) return true;
-    flush();
-    return warp_wait(bar_empty, parity, m, a);
+    return __any_sync(0xffffffffu, odd);
   }
   // 32 rows of this warp; `off` is each lane's row offset in elements, < 0: zeros
   __device__ __forceinline__ void copy_rows(uint32_t tile, const void* src, int64_t off) {
@@ -213,7 +188,7 @@ struct Loader {
       if (it.hi <= it.lo) continue;
       const int G = a.g.G;
       // queries
-      if (!acquire(&m->q_empty, (items & 1) ^ 1)) break;
+      if (!warp_wait(&m->q_empty, (items & 1) ^ 1, m, a)) break;
       const int ntok = it.t1 - it.t0;
       const int nq = ntok > a.TQ ? 2 : 1;
       for (int q = 0; q < nq; ++q) {
@@ -225,7 +200,7 @@ struct Loader {
                 (int64_t)(it.h * G + r % G) * a.c.q_sh;
         copy_rows(base + q * C::kQTile, a.c.q, off);
       }
-      pushed(&m->q_full, 0);
+      arrive_when_landed(&m->q_full);
       ++items;
       // keys and values
       const int32_t* table = a.rg.tables + (int64_t)it.q.slot * a.rg.W;
@@ -249,22 +224,32 @@ struct Loader {
         blk = next;
         const uint32_t slot = (op >> 1) % kSlots;
         uint32_t st = op % C::kStages;
-        if (!acquire(&m->kv_empty[st], ((op / C::kStages) & 1) ^ 1)) goto out;
+        if (!warp_wait(&m->kv_empty[st], ((op / C::kStages) & 1) ^ 1, m, a)) goto out;
         const uint32_t bad = __ballot_sync(0xffffffffu, off < 0);
-        if (lane == 0) m->key_bad[slot][w] = bad;
+        if (lane == 0) {
+          m->key_bad[slot][w] = bad;
+          mbar_arrive(&m->kv_full[st]);  // a plain arrival, behind the plain write
+        }
         copy_rows(base + C::kRing + st * C::kStage, a.kv.k, off);
-        pushed(&m->kv_full[st], 0);
+        arrive_when_landed(&m->kv_full[st]);
         ++op;
         st = op % C::kStages;
-        if (!acquire(&m->kv_empty[st], ((op / C::kStages) & 1) ^ 1)) goto out;
-        copy_rows(base + C::kRing + st * C::kStage, a.kv.v, off);
-        const bool check = tile_partial(it, a.g, (it.tile0 + k) * kKT);
-        pushed(&m->kv_full[st], check ? (base + C::kRing + st * C::kStage) | (slot + 1) : 0);
+        if (!warp_wait(&m->kv_empty[st], ((op / C::kStages) & 1) ^ 1, m, a)) goto out;
+        const uint32_t v = base + C::kRing + st * C::kStage;
+        copy_rows(v, a.kv.v, off);
+        if (tile_partial(it, a.g, (it.tile0 + k) * kKT)) {
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          __syncwarp();
+          const bool odd = has_odd(v);
+          if (lane == 0) m->v_odd[slot][w] = odd;
+          mbar_arrive(&m->kv_full[st]);
+        } else {
+          arrive_when_landed(&m->kv_full[st]);
+        }
         ++op;
       }
     }
   out:
-    flush();
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
 };
@@ -319,6 +304,7 @@ __device__ __forceinline__ void mma_role(const TcArgs& a, TcMeta* m, uint32_t ba
           skip = m->v_odd[slot][0] | m->v_odd[slot][1] | m->v_odd[slot][2] | m->v_odd[slot][3];
         }
       }
+      fence_proxy_async_smem();  // the tiles were written through the generic proxy
       tc_fence_after();
       for (int q = 0; q < nq; ++q) {
         if (j > 0) {
@@ -578,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const __grid_cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(&m->kv_full[i], 128);
+      mbar_init(&m->kv_full[i], i % 2 ? 128 : 128 + 4);  // K (even): and the key_bad writers
       mbar_init(&m->kv_empty[i], 1);
     }
     mbar_init(&m->q_full, 128);
