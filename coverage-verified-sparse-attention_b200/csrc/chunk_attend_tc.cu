@@ -255,8 +255,14 @@ struct Loader {
 };
 
 // ---------------------------------------------------------------------------
-// MMA issue (one thread)
+// MMA issue (one warp, one elected lane)
 // ---------------------------------------------------------------------------
+// The whole warp runs the loop, with its trip counts broadcast, so that the
+// compiler keeps descriptors in uniform registers, where the instruction
+// wants them: issued from a single-lane branch each MMA cost about 95 cycles
+// of moves, against the 64 that it runs.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 template <typename T, int D>
 __device__ __forceinline__ void mma_role(const TcArgs& a, TcMeta* m, uint32_t base, uint32_t tmem,
                                          const ChunkRange& rng) {
@@ -265,67 +271,84 @@ __device__ __forceinline__ void mma_role(const TcArgs& a, TcMeta* m, uint32_t ba
   constexpr uint32_t kIdS = mma_idesc(kBf16, kTile, kKT, false);
   constexpr uint32_t kIdO = mma_idesc(kBf16, kTile, D, true);
   const uint32_t ring = base + C::kRing;
+  const uint64_t q_desc = smem_desc(base, 16, 1024), k_desc = smem_desc(ring, 16, 1024),
+                 v_desc = smem_desc(ring, C::kPanel, 1024);
   ChunkWalk walk(rng);
   ChunkItem it;
-  uint32_t op = 0, items = 0, turns[2] = {0, 0};
+  uint32_t op = 0, items = 0, turn0 = 0, turn1 = 0;
   auto scores = [&](int q, uint32_t st) {  // S_q = Q_q K^T
-    const uint32_t d = tmem + q * kKT;
+    if (elect_one()) {
+      const uint32_t d = tmem + q * kKT;
+      const uint64_t qd = q_desc + ((q * C::kQTile) >> 4), kd = k_desc + ((st * C::kStage) >> 4);
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      const uint32_t o = (kk / 4) * C::kPanel + (kk % 4) * 32;
-      mma_ss(d, smem_desc(base + q * C::kQTile + o, 16, 1024),
-             smem_desc(ring + st * C::kStage + o, 16, 1024), kIdS, kk > 0);
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t o = ((kk / 4) * C::kPanel + (kk % 4) * 32) >> 4;
+        mma_ss(d, qd + o, kd + o, kIdS, kk > 0);
+      }
+      mma_commit(smem_u32(&m->s_full[q]));
+      mbar_arrive(&m->s_full[q]);  // orders the loaders' plain writes before the softmax too
     }
-    mma_commit(smem_u32(&m->s_full[q]));
-    mbar_arrive(&m->s_full[q]);  // orders the loaders' plain writes before the softmax too
+    __syncwarp();
   };
   auto outputs = [&](int q, uint32_t st, bool acc) {  // O_q (+)= P_q V
-    const uint32_t d = tmem + 2 * kKT + q * D, p = tmem + q * kKT;
+    if (elect_one()) {
+      const uint32_t d = tmem + 2 * kKT + q * D, p = tmem + q * kKT;
+      const uint64_t vd = v_desc + ((st * C::kStage) >> 4);
 #pragma unroll
-    for (int kk = 0; kk < kKT / 16; ++kk)
-      mma_ts(d, p + kk * 8, smem_desc(ring + st * C::kStage + kk * 2048, C::kPanel, 1024), kIdO,
-             acc || kk > 0);
+      for (int kk = 0; kk < kKT / 16; ++kk)
+        mma_ts(d, p + kk * 8, vd + ((kk * 2048) >> 4), kIdO, acc || kk > 0);
+    }
+    __syncwarp();
+  };
+  auto commit = [&](uint64_t* bar) {
+    if (elect_one()) mma_commit(smem_u32(bar));
+    __syncwarp();
   };
   while (walk.next(a.rg, a.g, it)) {
     if (it.hi <= it.lo) continue;
-    const int nq = it.t1 - it.t0 > a.TQ ? 2 : 1;
-    const int nt = it.k1 - it.k0;
-    if (!wait_for(&m->q_full, items & 1, m, a)) break;
+    const int nq = uniform(it.t1 - it.t0 > a.TQ ? 2 : 1);
+    const int nt = uniform(it.k1 - it.k0);
+    if (!warp_wait(&m->q_full, items & 1, m, a)) break;
     ++items;
     for (int j = 0; j <= nt; ++j) {
       const uint32_t kop = op + 2 * j, vop = kop - 1;
       const uint32_t kst = kop % C::kStages, vst = vop % C::kStages;
-      if (j < nt && !wait_for(&m->kv_full[kst], (kop / C::kStages) & 1, m, a)) goto out;
+      if (j < nt && !warp_wait(&m->kv_full[kst], (kop / C::kStages) & 1, m, a)) goto out;
       bool skip = false;
       if (j > 0) {
-        if (!wait_for(&m->kv_full[vst], (vop / C::kStages) & 1, m, a)) goto out;
+        if (!warp_wait(&m->kv_full[vst], (vop / C::kStages) & 1, m, a)) goto out;
         if (tile_partial(it, a.g, (it.tile0 + it.k0 + j - 1) * kKT)) {
           const uint32_t slot = (vop >> 1) % kSlots;
-          skip = m->v_odd[slot][0] | m->v_odd[slot][1] | m->v_odd[slot][2] | m->v_odd[slot][3];
+          skip = uniform(m->v_odd[slot][0] | m->v_odd[slot][1] | m->v_odd[slot][2] |
+                         m->v_odd[slot][3]);
         }
       }
       fence_proxy_async_smem();  // the tiles were written through the generic proxy
       tc_fence_after();
-      for (int q = 0; q < nq; ++q) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (q >= nq) break;
         if (j > 0) {
-          if (!wait_for(&m->p_full[q], turns[q] & 1, m, a)) goto out;
-          ++turns[q];
+          uint32_t& turn = q ? turn1 : turn0;
+          if (!warp_wait(&m->p_full[q], turn & 1, m, a)) goto out;
+          ++turn;
           tc_fence_after();
           if (!skip) outputs(q, vst, j > 1);
-          if (j == nt) mma_commit(smem_u32(&m->o_full[q]));
+          if (j == nt) commit(&m->o_full[q]);
         }
         if (j < nt) scores(q, kst);
       }
-      if (j < nt) mma_commit(smem_u32(&m->kv_empty[kst]));
-      if (j > 0) mma_commit(smem_u32(&m->kv_empty[vst]));
-      if (j == nt - 1) mma_commit(smem_u32(&m->q_empty));
+      if (j < nt) commit(&m->kv_empty[kst]);
+      if (j > 0) commit(&m->kv_empty[vst]);
+      if (j == nt - 1) commit(&m->q_empty);
     }
     op += 2 * nt;
   }
 out:
   // nothing of this CTA may be in flight when its tensor memory is freed
-  mma_commit(smem_u32(&m->drain));
+  commit(&m->drain);
   mbar_wait_bounded(&m->drain, 0, 1u << 22);
+  __syncwarp();
 }
 
 // ---------------------------------------------------------------------------
@@ -561,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const __grid_cons
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   TcMeta* m = reinterpret_cast<TcMeta*>(smem + C::kMeta);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(&m->kv_full[i], i % 2 ? 128 : 128 + 4);  // K (even): and the key_bad writers
@@ -587,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t base = smem_u32(smem), tmem = m->tmem;
+  const uint32_t base = smem_u32(smem), tmem = __shfl_sync(0xffffffffu, m->tmem, 0);
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     softmax_role<T, D>(a, m, base, tmem, rng, warp / 4);
@@ -596,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc_kernel(const __grid_cons
     Loader<T, D>(a, m, base, warp - 8, lane).run(rng);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 12 && lane == 0) mma_role<T, D>(a, m, base, tmem, rng);
+    if (warp == 12) mma_role<T, D>(a, m, base, tmem, rng);
     __syncwarp();
   }
   tc_fence_before();

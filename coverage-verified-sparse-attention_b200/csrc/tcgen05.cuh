@@ -73,6 +73,15 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const float* r) {
                : "memory");
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 // ---- MMA -----------------------------------------------------------------
 // Shared-memory matrix descriptor, 128-byte swizzle. K-major operand: rows of
 // 64 16-bit elements (128 bytes), 8-row groups `sbo` bytes apart. MN-major
