@@ -167,8 +167,10 @@ int check_chunk(const cvsa_chunk_attend_t* a, const KvView& kv, const RaggedView
   out->scale = a->scale;
   out->causal = a->causal != 0;
   out->window = a->window;
-  if (!chunk_attend_supported(kv, *out))
-    return fail(CVSA_ERR_UNSUPPORTED, "chunk_attend built for head_dim 64/128/256, G<=64");
+  if (!chunk_attend_supported(kv, rg, *out))
+    return fail(CVSA_ERR_UNSUPPORTED,
+                "chunk_attend built for head_dim 64/128/256, G<=64, and fewer than 2^31 key tiles "
+                "over all token groups and heads");
   return CVSA_OK;
 }
 

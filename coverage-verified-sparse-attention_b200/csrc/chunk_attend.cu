@@ -66,7 +66,7 @@ struct GenSmem {
   float p[kRows][kKeys + 4];
   int64_t key_off[kKeys];   // element offset of a key's row in the pools
   int8_t key_ok[kKeys];
-  ChunkPlanSmem<kThreads> plan;
+  ChunkRange range;
 };
 
 template <typename T, typename C, int D>
@@ -75,14 +75,18 @@ __global__ void __launch_bounds__(kThreads) chunk_general_kernel(GenArgs a) {
   GenSmem<D>& sm = *reinterpret_cast<GenSmem<D>*>(smem_raw);
   const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
   const int cta = blockIdx.x;
-  const ChunkRange rng = chunk_range<kThreads>(a.rg, a.g, sm.plan, cta, gridDim.x, a.min_units,
-                                               a.dev_err);
-  if (tid == 0) a.desc[cta].parts = 0;
+  if (tid < 32) {
+    const ChunkRange r = chunk_range(a.rg, a.g, cta, gridDim.x, a.min_units, a.dev_err);
+    if (tid == 0) {
+      sm.range = r;
+      a.desc[cta].parts = 0;
+    }
+  }
   __syncthreads();
-  ChunkWalk walk(rng);
+  ChunkWalk walk(sm.range);
   ChunkItem it;
   const int G = a.g.G;
-  while (walk.next(a.rg, a.g, it)) {
+  while (walk.next(a.rg, a.g, cta, it)) {
     const int rows = (it.t1 - it.t0) * G;
     // query rows: token t0 + r / G, head h * G + r % G
     for (int e = tid; e < kRows * (D / 4); e += kThreads) {
@@ -109,8 +113,7 @@ __global__ void __launch_bounds__(kThreads) chunk_general_kernel(GenArgs a) {
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) o[x][d] = 0.f;
     }
-    const int tiles = chunk_tiles(it.lo, it.hi, kKeys);
-    for (int k = it.k0; k < min(it.k1, tiles); ++k) {
+    for (int k = it.k0; k < it.k1; ++k) {
       const int base = (it.tile0 + k) * kKeys;
       __syncthreads();  // the previous tile's reads are done
       if (tid < kKeys) {
@@ -219,8 +222,7 @@ __global__ void __launch_bounds__(kThreads) chunk_general_kernel(GenArgs a) {
       }
     }
     // whole items are finished here, pieces go to a partial slot
-    const bool whole = it.k0 == 0 && it.k1 == it.units;
-    if (whole) {
+    if (it.whole) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int r = ty * 4 + x;
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(kThreads) chunk_general_kernel(GenArgs a) {
           a.c.lse[tok * a.c.hq + head] = l[x] == 0.f ? neg_inf() : (m[x] + log2f(l[x])) * kLn2;
       }
     } else {
-      float* part = a.parts + (size_t)chunk_slot(it, rng.u0, cta) * chunk_slot_floats(kRows, D);
+      float* part = a.parts + (size_t)(2 * cta + it.slot) * chunk_slot_floats(kRows, D);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int r = ty * 4 + x;
@@ -252,9 +254,9 @@ __global__ void __launch_bounds__(kThreads) chunk_general_kernel(GenArgs a) {
           po[(size_t)(tx + 16 * y) * kRows + r] =
               make_float4(o[x][4 * y], o[x][4 * y + 1], o[x][4 * y + 2], o[x][4 * y + 3]);
       }
-      if (tid == 0 && it.k0 == 0) {
+      if (tid == 0 && it.parts) {
         ChunkMergeDesc d;
-        d.parts = (int)((it.first + it.units - 1) / rng.per_cta) - cta + 1;
+        d.parts = it.parts;
         d.tok = it.q.tok0 + it.t0;
         d.rows = rows;
         d.head = it.h;
@@ -381,7 +383,7 @@ constexpr size_t kDescBytes = ((kMaxCtas * sizeof(ChunkMergeDesc) + 255) / 256) 
 
 int chunk_ctas() { return num_sms() < kMaxCtas ? num_sms() : kMaxCtas; }
 
-ChunkGeo general_geo(const KvView& kv, const ChunkView& c) {
+ChunkGeo general_geo(const KvView& kv, const RaggedView& rg, const ChunkView& c) {
   ChunkGeo g;
   g.bs = kv.bs;
   g.hkv = kv.hkv;
@@ -390,13 +392,17 @@ ChunkGeo general_geo(const KvView& kv, const ChunkView& c) {
   g.KT = kKeys;
   g.causal = c.causal;
   g.window = c.window;
+  g.fixed = 1;
+  g.split = chunk_may_split(rg, kv.bs, kKeys);
   return g;
 }
 
 }  // namespace
 
-bool chunk_attend_supported(const KvView& kv, const ChunkView& c) {
-  return (kv.d == 64 || kv.d == 128 || kv.d == 256) && c.hq / kv.hkv <= kRows;
+bool chunk_attend_supported(const KvView& kv, const RaggedView& rg, const ChunkView& c) {
+  return (kv.d == 64 || kv.d == 128 || kv.d == 256) && c.hq / kv.hkv <= kRows &&
+         chunk_fits(rg, chunk_tc_eligible(kv, c) ? chunk_tc_geo(kv, rg, c)
+                                                 : general_geo(kv, rg, c));
 }
 
 size_t chunk_attend_workspace_bytes(const KvView& kv, const RaggedView& rg, const ChunkView& c) {
@@ -410,6 +416,7 @@ cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const Ch
   ChunkMergeDesc* desc = reinterpret_cast<ChunkMergeDesc*>(ws);
   float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kDescBytes);
   const bool tc = chunk_tc_eligible(kv, c);
+  const bool split = tc ? chunk_tc_geo(kv, rg, c).split : general_geo(kv, rg, c).split;
   cudaError_t e;
   if (tc) {
     e = launch_chunk_tc(kv, rg, c, ctas, parts, desc, dev_err, s);
@@ -418,7 +425,7 @@ cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const Ch
     a.rg = rg;
     a.kv = kv;
     a.c = c;
-    a.g = general_geo(kv, c);
+    a.g = general_geo(kv, rg, c);
     a.scale2 = c.scale * kLog2e;
     a.min_units = 2;
     a.desc = desc;
@@ -430,7 +437,7 @@ cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const Ch
       default: e = launch_general_c<float>(a, ctas, s); break;
     }
   }
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || !split) return e;
   MergeArgs m;
   m.parts = parts;
   m.desc = desc;

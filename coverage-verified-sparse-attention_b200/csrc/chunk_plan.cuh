@@ -3,19 +3,22 @@
 //
 // An item is one KV head of one group of P consecutive new tokens of one
 // sequence (all query heads of the KV head: P * G query rows); it walks the
-// KT-key tiles its rows can see, one unit of work a tile (an item that sees
-// none counts one, so its rows are still written). The items in the order
+// KT-key tiles its rows can see. It counts its tiles plus `fixed` units of work
+// (bringing the queries in and writing the rows out cost about as much as
+// that many tiles: without it the CTA that got a prompt's first groups, of a
+// tile each, took three times as long as the others). The items in the order
 // (sequence, group, head) form one stream of units that is cut into equal
 // contiguous ranges, one a CTA, so the load is even whatever the mix of long
 // and short contexts, and a long cache with few queries is split over all CTAs
 // by the same rule. An item inside one range is finished by its CTA; an item
 // that crosses ranges leaves one partial (m, l, o) a CTA, merged in CTA order
 // by a second kernel. A CTA has at most two such items (its first and its
-// last), so two partial slots each.
+// last), so two partial slots each. When no item can be longer than a few
+// tiles (short tables) a CTA takes the items that begin in its range whole, and
+// there is nothing to merge.
 //
-// Lengths live on the device, so every CTA finds its own range: the threads
-// evaluate the groups of all sequences in parallel (a block scan a thousand
-// groups), which costs about a microsecond and no extra launch.
+// Lengths live on the device, so every CTA finds its own range, one warp of it
+// alone, 32 sequences or groups a step: no launch and no block-wide barrier.
 #pragma once
 
 #include "cvsa_common.cuh"
@@ -28,6 +31,8 @@ struct ChunkGeo {
   int P;        // new tokens a group
   int KT;       // keys a tile
   int causal, window;
+  int fixed;    // units an item counts beside its tiles
+  int split;    // items may cross ranges
 };
 
 struct SeqInfo {
@@ -77,175 +82,161 @@ __device__ __forceinline__ int chunk_tiles(int lo, int hi, int KT) {
 __device__ __forceinline__ int chunk_units(const SeqInfo& q, const ChunkGeo& g, int i) {
   int lo, hi;
   chunk_keys(q, g, i * g.P, min(q.n, (i + 1) * g.P), lo, hi);
-  return max(1, chunk_tiles(lo, hi, g.KT));
+  return chunk_tiles(lo, hi, g.KT) + g.fixed;
 }
 
-// What the CTA at `cta` of `ctas` does: units [u0, u1) of the stream, starting
-// at unit `skip` of item (b, i, h).
+// What a CTA does: units [u0, u1) of the stream, starting at unit `skip` of
+// item (b, i, h). (The host has checked that the units fit 31 bits.)
 struct ChunkRange {
-  long long u0, u1, per_cta;
+  int u0, u1, per_cta;
   int b, i, h, skip;
 };
 
-template <int NT>
-struct ChunkPlanSmem {
-  int incl[NT];            // inclusive sum of the groups of a round's sequences
-  SeqInfo seq[NT];
-  long long warp_sums[NT / 32];
-  long long carry;
-  int total;
-  ChunkRange range;
-};
-
-template <int NT>
-__device__ __forceinline__ long long chunk_scan_incl(long long v, long long* warp_sums) {
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+__device__ __forceinline__ int warp_scan_incl(int v) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long t = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += t;
+    const int t = __shfl_up_sync(0xffffffffu, v, o);
+    if ((int)(threadIdx.x & 31) >= o) v += t;
   }
-  if (lane == 31) warp_sums[wid] = v;
-  __syncthreads();
-  long long before = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 32; ++w) before += w < wid ? warp_sums[w] : 0;
-  __syncthreads();
-  return v + before;
+  return v;
 }
 
-// Runs `visit(pair, b, i, units, incl)` for every group of the batch in
-// stream order, NT at a time, all threads together (units = 0 and b = -1
-// beyond the end; units already times the heads, incl = inclusive sum over
-// the whole stream so far). Returns the stream's total.
-template <int NT, typename Visit>
-__device__ __forceinline__ long long chunk_enumerate(const RaggedView& rg, const ChunkGeo& g,
-                                                     ChunkPlanSmem<NT>& sm, int32_t* dev_err,
-                                                     Visit visit) {
-  const int tid = threadIdx.x;
-  long long base = 0;
-  for (int b0 = 0; b0 < rg.B; b0 += NT) {
-    int ng = 0;
-    if (b0 + tid < rg.B) {
-      const SeqInfo q = chunk_seq(rg, g.bs, b0 + tid, dev_err);
-      sm.seq[tid] = q;
-      ng = chunk_groups(q, g.P);
-    }
-    const long long in = chunk_scan_incl<NT>(ng, sm.warp_sums);
-    sm.incl[tid] = (int)in;
-    __syncthreads();
-    const int total = sm.incl[NT - 1];
-    for (int p0 = 0; p0 < total; p0 += NT) {
-      const int p = p0 + tid;
-      int b = -1, i = 0;
-      long long units = 0;
-      if (p < total) {
-        int lo = 0, hi = NT - 1;
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (sm.incl[mid] > p) hi = mid; else lo = mid + 1;
-        }
-        i = p - (lo ? sm.incl[lo - 1] : 0);
-        b = b0 + lo;
-        units = (long long)chunk_units(sm.seq[lo], g, i) * g.hkv;
-      }
-      const long long incl = base + chunk_scan_incl<NT>(units, sm.warp_sums);
-      visit(b, i, units, incl);
-      if (tid == NT - 1) sm.carry = incl;
-      __syncthreads();
-      base = sm.carry;
-    }
-    __syncthreads();
+// Units of 32 sequences from b0, one a lane (all heads).
+__device__ __forceinline__ int chunk_seq_units(const RaggedView& rg, const ChunkGeo& g, int b0,
+                                               SeqInfo& q, int32_t* dev_err) {
+  const int lane = threadIdx.x & 31;
+  q.n = 0;
+  if (b0 + lane < rg.B) q = chunk_seq(rg, g.bs, b0 + lane, dev_err);
+  const int ng = chunk_groups(q, g.P);
+  int units = ng == 1 ? chunk_units(q, g, 0) : 0;
+  // sequences of several groups: the warp sums the groups of one at a time
+  for (unsigned many = __ballot_sync(0xffffffffu, ng > 1); many; many &= many - 1) {
+    const int src = __ffs(many) - 1;
+    SeqInfo s;
+    s.n = __shfl_sync(0xffffffffu, q.n, src);
+    s.start = __shfl_sync(0xffffffffu, q.start, src);
+    s.ctx = __shfl_sync(0xffffffffu, q.ctx, src);
+    const int groups = chunk_groups(s, g.P);
+    int sum = 0;
+    for (int i = lane; i < groups; i += 32) sum += chunk_units(s, g, i);
+    sum = warp_sum_i(sum);
+    if (lane == src) units = sum;
   }
-  return base;
+  return units * g.hkv;
 }
 
-// The range of CTA `cta`; every thread of the block returns it. Ranges are at
+// The range of CTA `cta`, by a whole warp; every lane returns it. Ranges are at
 // least `min_units` long: a partial costs its write and its read by the merge,
 // which a tile or two do not pay for.
-template <int NT>
-__device__ __forceinline__ ChunkRange chunk_range(const RaggedView& rg, const ChunkGeo& g,
-                                                  ChunkPlanSmem<NT>& sm, int cta, int ctas,
-                                                  int min_units, int32_t* dev_err) {
-  int kb = -1, ki = 0, rounds = 0;
-  long long kunits = 0, kincl = 0;
-  const long long total = chunk_enumerate<NT>(
-      rg, g, sm, cta == 0 ? dev_err : nullptr, [&](int b, int i, long long units, long long incl) {
-        kb = b; ki = i; kunits = units; kincl = incl;
-        ++rounds;
-      });
-  ChunkRange r;
-  r.per_cta = max((long long)min_units, (total + ctas - 1) / ctas);
-  r.u0 = min(total, cta * (long long)r.per_cta);
-  r.u1 = min(total, r.u0 + r.per_cta);
-  r.b = r.i = r.h = r.skip = 0;
-  if (r.u0 >= r.u1) return r;
-  auto find = [&](int b, int i, long long units, long long incl) {
-    if (b >= 0 && incl > r.u0 && incl - units <= r.u0) {
-      ChunkRange f = r;
-      const int per_head = (int)(units / g.hkv);
-      const int off = (int)(r.u0 - (incl - units));
-      f.b = b; f.i = i; f.h = off / per_head; f.skip = off % per_head;
-      sm.range = f;
-    }
-  };
-  if (rounds == 1) {
-    find(kb, ki, kunits, kincl);  // one round held every group: its values are still here
-    __syncthreads();
-  } else {
-    chunk_enumerate<NT>(rg, g, sm, nullptr, find);
+__device__ __forceinline__ ChunkRange chunk_range(const RaggedView& rg, const ChunkGeo& g, int cta,
+                                                  int ctas, int min_units, int32_t* dev_err) {
+  const int lane = threadIdx.x & 31;
+  SeqInfo q = {};
+  ChunkRange r = {};
+  int total = 0, units = 0;
+#pragma unroll 1
+  for (int b0 = 0; b0 < rg.B; b0 += 32) {
+    units = chunk_seq_units(rg, g, b0, q, cta == 0 ? dev_err : nullptr);
+    total += warp_sum_i(units);
   }
-  r = sm.range;
-  __syncthreads();
+  r.per_cta = max(min_units, (total + ctas - 1) / ctas);
+  r.u0 = (int)min((int64_t)total, (int64_t)cta * r.per_cta);
+  r.u1 = min(total, r.u0 + r.per_cta);
+  if (r.u0 >= r.u1) return r;
+  int before = 0;  // units ahead of this step
+#pragma unroll 1
+  for (int b0 = 0; b0 < rg.B; b0 += 32) {
+    if (rg.B > 32) units = chunk_seq_units(rg, g, b0, q, nullptr);  // else still in registers
+    const int incl = warp_scan_incl(units) + before;
+    const unsigned past = __ballot_sync(0xffffffffu, incl > r.u0);
+    if (!past) {
+      before = __shfl_sync(0xffffffffu, incl, 31);
+      continue;
+    }
+    const int src = __ffs(past) - 1;
+    before = __shfl_sync(0xffffffffu, incl - units, src);
+    r.b = b0 + src;
+    SeqInfo s;
+    s.n = __shfl_sync(0xffffffffu, q.n, src);
+    s.start = __shfl_sync(0xffffffffu, q.start, src);
+    s.ctx = __shfl_sync(0xffffffffu, q.ctx, src);
+    const int groups = chunk_groups(s, g.P);
+#pragma unroll 1
+    for (int i0 = 0; i0 < groups; i0 += 32) {
+      const int per_head = i0 + lane < groups ? chunk_units(s, g, i0 + lane) : 0;
+      const int in = warp_scan_incl(per_head * g.hkv) + before;
+      const unsigned here = __ballot_sync(0xffffffffu, in > r.u0);
+      if (!here) {
+        before = __shfl_sync(0xffffffffu, in, 31);
+        continue;
+      }
+      const int at = __ffs(here) - 1;
+      const int ph = __shfl_sync(0xffffffffu, per_head, at);
+      const int off = r.u0 - __shfl_sync(0xffffffffu, in - per_head * g.hkv, at);
+      r.i = i0 + at;
+      r.h = off / ph;
+      r.skip = off - r.h * ph;
+      break;
+    }
+    break;
+  }
   return r;
 }
 
 // A CTA's walk over its items, identical in every thread that runs one.
 struct ChunkItem {
   SeqInfo q;
-  int i, h;
+  int h;
   int t0, t1;        // new tokens of the group
   int lo, hi;        // keys its rows see
   int tile0;         // first key tile of the item
-  int units;         // units of the whole item
-  int k0, k1;        // units of it in this CTA's range
-  long long first;   // stream position of its unit 0
+  int k0, k1;        // tiles of it in this CTA's range, from tile0
+  bool whole;        // all of them
+  int slot;          // partial slot of the CTA (0: begun before its range)
+  int parts;         // when it begins here: CTAs that share it
 };
 
 struct ChunkWalk {
-  long long u, u1;
-  int b, i, h, skip, loaded;
+  int u, b, i, h, skip, loaded;
+  ChunkRange r;
   SeqInfo q;
-  __device__ __forceinline__ explicit ChunkWalk(const ChunkRange& r)
-      : u(r.u0), u1(r.u1), b(r.b), i(r.i), h(r.h), skip(r.skip), loaded(-1) {}
+  __device__ __forceinline__ explicit ChunkWalk(const ChunkRange& r_)
+      : u(r_.u0), b(r_.b), i(r_.i), h(r_.h), skip(r_.skip), loaded(-1), r(r_) {}
   // false at the end of the range
-  __device__ __forceinline__ bool next(const RaggedView& rg, const ChunkGeo& g, ChunkItem& it) {
-    if (u >= u1) return false;
-    if (h == g.hkv) { h = 0; ++i; }
-    for (;;) {
+  __device__ __forceinline__ bool next(const RaggedView& rg, const ChunkGeo& g, int cta,
+                                       ChunkItem& it) {
+    while (u < r.u1) {
+      if (h == g.hkv) { h = 0; ++i; }
       if (loaded != b) {
         q = chunk_seq(rg, g.bs, b, nullptr);
         loaded = b;
       }
-      if (i < chunk_groups(q, g.P)) break;
-      i = 0;
-      if (++b >= rg.B) return false;
+      if (i >= chunk_groups(q, g.P)) {
+        i = 0;
+        if (++b >= rg.B) return false;
+        continue;
+      }
+      it.t0 = i * g.P;
+      it.t1 = min(q.n, it.t0 + g.P);
+      chunk_keys(q, g, it.t0, it.t1, it.lo, it.hi);
+      const int tiles = chunk_tiles(it.lo, it.hi, g.KT), units = tiles + g.fixed;
+      const int k0 = skip, k1 = g.split ? min(units, skip + (r.u1 - u)) : units;
+      const int first = u - skip;
+      u += k1 - k0;
+      skip = 0;
+      it.h = h++;
+      // of another CTA, or nothing but the end of the item's fixed part
+      if (k0 > 0 && (!g.split || k0 >= tiles)) continue;
+      it.q = q;
+      it.tile0 = tiles ? it.lo / g.KT : 0;
+      it.k0 = k0;
+      it.k1 = min(k1, tiles);
+      it.whole = k0 == 0 && k1 >= tiles;
+      it.slot = first < r.u0 ? 0 : 1;
+      it.parts = it.whole || k0 > 0 ? 0 : (first + tiles - 1) / r.per_cta - cta + 1;
+      return true;
     }
-    it.q = q;
-    it.i = i;
-    it.h = h;
-    it.t0 = i * g.P;
-    it.t1 = min(q.n, it.t0 + g.P);
-    chunk_keys(q, g, it.t0, it.t1, it.lo, it.hi);
-    it.tile0 = it.hi > it.lo ? it.lo / g.KT : 0;
-    it.units = max(1, chunk_tiles(it.lo, it.hi, g.KT));
-    it.k0 = skip;
-    it.k1 = (int)min((long long)it.units, skip + (u1 - u));
-    it.first = u - skip;
-    u += it.k1 - it.k0;
-    skip = 0;
-    ++h;
-    return true;
+    return false;
   }
 };
 
@@ -260,12 +251,20 @@ struct ChunkMergeDesc {
 __host__ __device__ constexpr size_t chunk_slot_floats(int rows, int d) {
   return (size_t)rows * (d + 2);
 }
-__device__ __forceinline__ int chunk_slot(const ChunkItem& it, long long u0, int cta) {
-  return 2 * cta + (it.first < u0 ? 0 : 1);
+
+// Whether a call's units fit 31 bits, and whether its items may be split.
+inline bool chunk_fits(const RaggedView& rg, const ChunkGeo& g) {
+  const int64_t tiles = ((int64_t)rg.W * g.bs + g.KT - 1) / g.KT + 1;
+  return ((int64_t)rg.T / g.P + rg.B + 1) * g.hkv * (tiles + g.fixed) < (int64_t(1) << 31);
+}
+inline int chunk_may_split(const RaggedView& rg, int bs, int KT) {
+  // up to four tiles: less than the merge's launch and the partials' way
+  return ((int64_t)rg.W * bs + KT - 1) / KT > 4;
 }
 
 // ---- chunk_attend_tc.cu ----
 bool chunk_tc_eligible(const KvView& kv, const ChunkView& c);
+ChunkGeo chunk_tc_geo(const KvView& kv, const RaggedView& rg, const ChunkView& c);
 int chunk_tc_rows();  // query rows of an item at most (a partial slot's rows)
 cudaError_t launch_chunk_tc(const KvView& kv, const RaggedView& rg, const ChunkView& c, int ctas,
                             float* parts, ChunkMergeDesc* desc, int32_t* dev_err, cudaStream_t s);

@@ -287,7 +287,7 @@ struct ChunkView {
   int causal, window;                     // window 0: none
 };
 size_t chunk_attend_workspace_bytes(const KvView& kv, const RaggedView& rg, const ChunkView& c);
-bool chunk_attend_supported(const KvView& kv, const ChunkView& c);
+bool chunk_attend_supported(const KvView& kv, const RaggedView& rg, const ChunkView& c);
 cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const ChunkView& c,
                                 void* ws, int32_t* dev_err, cudaStream_t s);
 

@@ -307,3 +307,14 @@ def test_long_pool_offsets(cuda):
     P.tables = torch.where(P.tables >= 0, P.tables + (nb - n), P.tables)
     P.k_cache = P.v_cache = k
     check(P)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64)])
+def test_mixed_items_in_one_cta(cuda, dtype, d):
+    """Items of two, one and small single query tiles, with and without keys,
+    follow one another in every CTA's range: far more items than CTAs."""
+    new = [(37 * i * i + 11) % 97 for i in range(60)] + [130, 1, 300, 0, 2, 64, 65]
+    ctx = [n + (53 * i) % 400 for i, n in enumerate(new)]
+    P = Problem(new, ctx, 28, 4, d, dtype=dtype, seed=22)
+    check(P)
+    check(P, window=100)
