@@ -272,6 +272,23 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def raw_stream(index: int) -> int:
+    """The current stream's handle by device index (no stream object is built)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def same_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """Device index shared by all tensors; the errors are require_cuda's."""
+    dev = first.get_device()
+    ok = dev >= 0
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            ok = False
+    if not ok:
+        require_cuda(first, *others)
+    return dev
+
+
 def kv_desc(k_cache: torch.Tensor, v_cache: torch.Tensor) -> KvDesc:
     """[num_blocks, block_size, num_kv_heads, head_dim] pools (kv_cache.py:38-43)."""
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
@@ -305,18 +322,19 @@ def ragged_desc(num_tokens: int, cu_tokens: torch.Tensor, block_tables: torch.Te
                 context_lens: torch.Tensor, seq_ids: Optional[torch.Tensor],
                 start_positions: Optional[torch.Tensor]) -> RaggedDesc:
     """The packed new tokens of a batch and the tables of the sequences they belong to."""
+    i32 = torch.int32
     for t in (cu_tokens, block_tables, context_lens, seq_ids, start_positions):
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+        if t is not None and not (t.dtype is i32 and t.is_contiguous()):
             raise ValueError("cu_tokens, block_tables, context_lens, seq_ids and "
                              "start_positions must be contiguous int32")
-    if block_tables.dim() != 2 or cu_tokens.dim() != 1 or cu_tokens.shape[0] < 1:
+    B = cu_tokens.numel() - 1
+    if block_tables.dim() != 2 or cu_tokens.dim() != 1 or B < 0:
         raise ValueError("block_tables must be [num_seqs, max_pages], cu_tokens [batch + 1]")
-    B = cu_tokens.shape[0] - 1
     S, W = block_tables.shape
-    if context_lens.shape != (S,):
+    if context_lens.dim() != 1 or context_lens.numel() != S:
         raise ValueError("context_lens must be [num_seqs]")
     for t in (seq_ids, start_positions):
-        if t is not None and t.shape != (B,):
+        if t is not None and (t.dim() != 1 or t.numel() != B):
             raise ValueError("seq_ids and start_positions must be [batch]")
     return RaggedDesc(cu_tokens.data_ptr(), ptr(seq_ids), ptr(start_positions),
                       block_tables.data_ptr(), context_lens.data_ptr(), B, num_tokens, S, W)
@@ -326,9 +344,8 @@ def token_rows(t: torch.Tensor, name: str) -> torch.Tensor:
     """A [num_tokens, heads, head_dim] view the kernels can read: 16-byte rows (copied if not)."""
     if t.dim() != 3:
         raise ValueError(f"{name} must be [num_tokens, heads, head_dim]")
-    eb = t.element_size()
-    if t.numel() and (t.stride(2) != 1 or t.data_ptr() % 16 or (t.stride(0) * eb) % 16
-                      or (t.stride(1) * eb) % 16 or t.stride(0) < 0 or t.stride(1) < 0):
+    st, sh, sd = t.stride()
+    if t.numel() and (sd != 1 or t.data_ptr() % 16 or (st | sh) * t.element_size() % 16):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -351,6 +368,16 @@ class Workspace:
             self._bufs[key] = buf
         off = (-buf.data_ptr()) % 256
         return buf[off:]
+
+    def address(self, nbytes: int, device: torch.device, stream: int, tag: str) -> int:
+        """Aligned address of at least nbytes, for calls that pass no tensor on."""
+        key = (device.index, stream, tag)
+        got = self._bufs.get(key)
+        if got is None or got[2] < nbytes:
+            buf = torch.zeros(nbytes + 256, dtype=torch.uint8, device=device)
+            got = (buf, buf.data_ptr() + (-buf.data_ptr()) % 256, nbytes)
+            self._bufs[key] = got
+        return got[1]
 
 
 WORKSPACE = Workspace()

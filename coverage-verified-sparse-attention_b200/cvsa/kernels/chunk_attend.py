@@ -14,6 +14,8 @@ import torch
 
 from cvsa import _lib
 
+_ws_bytes = {}  # workspace bytes by (device, head_dim, dtypes)
+
 
 def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                     block_tables: torch.Tensor, context_lens: torch.Tensor,
@@ -32,26 +34,35 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     with the log-sum-exp of each row's scaled scores (for a merge with
     attention over other keys). A row that sees no key gives 0 and -inf.
     """
-    dev = _lib.require_cuda(q, k_cache, v_cache, block_tables, context_lens, cu_tokens, seq_ids,
-                            start_positions, out, lse, dev_error)
+    dev = _lib.same_device(q, k_cache, v_cache, block_tables, context_lens, cu_tokens, seq_ids,
+                           start_positions, out, lse, dev_error)
     q = _lib.token_rows(q, "q")
-    T, Hq, D = q.shape
+    T, Hq, D = shape = q.shape
     if k_cache.dim() != 4 or k_cache.shape[3] != D:
         raise ValueError("q's head_dim does not match the cache")
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif out.shape != shape or out.dtype != q.dtype or out.stride(2) != 1:
         raise ValueError("out must have q's shape and dtype and contiguous rows")
     if lse is not None and (lse.shape != (T, Hq) or lse.dtype != torch.float32
                             or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous float32 [T, H_q]")
     kvd = _lib.kv_desc(k_cache, v_cache)
     rg = _lib.ragged_desc(T, cu_tokens, block_tables, context_lens, seq_ids, start_positions)
+    qs, os_ = q.stride(), out.stride()
     args = _lib.ChunkAttend(q.data_ptr(), out.data_ptr(), _lib.ptr(lse), _lib.dtype_code(q.dtype),
-                            Hq, q.stride(0), q.stride(1), out.stride(0), out.stride(1),
-                            D ** -0.5 if scale is None else scale, int(causal), window)
-    lib = _lib.load()
-    ws = _lib.WORKSPACE.get(lib.cvsa_chunk_attend_workspace_size(kvd, rg, args), dev, "chunk")
-    _lib.check(lib.cvsa_chunk_attend(kvd, rg, args, _lib.ptr(dev_error), ws.data_ptr(),
-                                     ws.numel(), _lib.stream_ptr(dev)), "cvsa_chunk_attend")
+                            Hq, qs[0], qs[1], os_[0], os_[1],
+                            D ** -0.5 if scale is None else scale, causal, window)
+    lib, stream = _lib.load(), _lib.raw_stream(dev)
+    # the size depends on the head layout alone; 0 for what the call will refuse
+    key = (dev, D, q.dtype, k_cache.dtype)
+    nbytes = _ws_bytes.get(key)
+    if nbytes is None:
+        nbytes = lib.cvsa_chunk_attend_workspace_size(kvd, rg, args)
+        if nbytes:
+            _ws_bytes[key] = nbytes
+    ws = _lib.WORKSPACE.address(nbytes, q.device, stream, "chunk") if nbytes else None
+    st = lib.cvsa_chunk_attend(kvd, rg, args, _lib.ptr(dev_error), ws, nbytes, stream)
+    if st:
+        _lib.check(st, "cvsa_chunk_attend")
     return out

@@ -57,8 +57,8 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     instead of the halves of the rotated part. start_positions and seq_ids as
     returned by / given to `reserve`. `out` may be q itself.
     """
-    dev = _lib.require_cuda(q, k, v, k_cache, v_cache, block_tables, context_lens, cu_tokens,
-                            cos_sin, q_norm, k_norm, seq_ids, start_positions, out, dev_error)
+    dev = _lib.same_device(k, q, v, k_cache, v_cache, block_tables, context_lens, cu_tokens,
+                           cos_sin, q_norm, k_norm, seq_ids, start_positions, out, dev_error)
     T, Hkv, D = k.shape
     if v.shape != k.shape or k_cache.dim() != 4 or tuple(k_cache.shape[2:]) != (Hkv, D):
         raise ValueError("k and v must be [T, H_kv, D] with the cache's H_kv and D")
@@ -72,7 +72,7 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         Hq = q.shape[1]
         q = _lib.token_rows(q, "q")
         if out is None:
-            out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+            out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
             raise ValueError("out must have q's shape and dtype and contiguous rows")
         qs, os_ = q.stride(), out.stride()
@@ -92,11 +92,13 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
             raise ValueError("cos_sin must be a contiguous float32 [max_positions, rot_dim]")
         pos, rot = cos_sin.shape
     rg = _lib.ragged_desc(T, cu_tokens, block_tables, context_lens, seq_ids, start_positions)
+    ks, vs = k.stride(), v.stride()
     args = _lib.RopeAppend(qp, k.data_ptr(), v.data_ptr(), op, _lib.dtype_code(k.dtype), Hq,
-                           qs[0], qs[1], k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                           os_[0], os_[1], _lib.ptr(cos_sin), pos, rot, int(interleaved),
+                           qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
+                           os_[0], os_[1], _lib.ptr(cos_sin), pos, rot, interleaved,
                            _lib.dtype_code(ndt), _lib.ptr(q_norm), _lib.ptr(k_norm), eps)
-    _lib.check(_lib.load().cvsa_rope_append(_lib.kv_desc(k_cache, v_cache), rg, args,
-                                            _lib.ptr(dev_error), _lib.stream_ptr(dev)),
-               "cvsa_rope_append")
+    st = _lib.load().cvsa_rope_append(_lib.kv_desc(k_cache, v_cache), rg, args,
+                                      _lib.ptr(dev_error), _lib.raw_stream(dev))
+    if st:
+        _lib.check(st, "cvsa_rope_append")
     return out
