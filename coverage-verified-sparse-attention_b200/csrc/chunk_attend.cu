@@ -445,7 +445,8 @@ cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const Ch
   m.rows = tc ? chunk_tc_rows() : kRows;
   m.G = c.hq / kv.hkv;
   m.d = kv.d;
-  const dim3 grid((m.rows + 31) / 32, ctas);
+  const int64_t rows = (int64_t)rg.T * m.G;  // of an item, at most
+  const dim3 grid(((rows < m.rows ? (int)rows : m.rows) + 31) / 32, ctas);
   switch (c.dtype) {
     case CVSA_DTYPE_BF16:
       return launch_k(chunk_merge_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, true, m);

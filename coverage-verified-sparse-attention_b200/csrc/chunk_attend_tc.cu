@@ -328,23 +328,7 @@ struct Loader {
         items.done();
         continue;
       }
-      // queries
-      if (!warp_wait(&m->q_empty, (loads & 1) ^ 1, m, a)) break;
-      ++loads;
-      if (joins && !warp_wait(&m->join_free, (joins - 1) & 1, m, a)) break;
       const int lag = it->pair ? 2 : 1;
-      joins += it->pair;
-      for (int q = 0; q < it->nq; ++q) {
-        const int r = w * 32 + lane;
-        const int rows = min(a.TQ, it->ntok - q * a.TQ) * G;
-        int64_t off = -1;
-        if (r < rows)
-          off = (int64_t)(it->tok + q * a.TQ + r / G) * a.c.q_st +
-                (int64_t)(it->h * G + r % G) * a.c.q_sh;
-        copy_rows(base + q * C::kQTile, a.c.q, off);
-      }
-      arrive_when_landed(&m->q_full);
-      // keys and values
       const int lo = it->lo, hi = it->hi;
       const int32_t* table = a.rg.tables + (int64_t)it->slot * a.rg.W;
       const int64_t head = it->h * a.kv.sh;
@@ -384,6 +368,24 @@ struct Loader {
           copy(base + C::kRing + st * C::kStage, a.kv.k, off0, pages & 1);
           arrive_when_landed(&m->kv_full[st]);
           ++op;
+        }
+        if (j == lag - 1) {
+          // the queries, behind the first K tiles: those are on their way while the
+          // item before still holds the queries' memory
+          if (!warp_wait(&m->q_empty, (loads & 1) ^ 1, m, a)) goto out;
+          ++loads;
+          if (joins && !warp_wait(&m->join_free, (joins - 1) & 1, m, a)) goto out;
+          joins += it->pair;
+          for (int q = 0; q < it->nq; ++q) {
+            const int r = w * 32 + lane;
+            const int rows = min(a.TQ, it->ntok - q * a.TQ) * G;
+            int64_t off = -1;
+            if (r < rows)
+              off = (int64_t)(it->tok + q * a.TQ + r / G) * a.c.q_st +
+                    (int64_t)(it->h * G + r % G) * a.c.q_sh;
+            copy_rows(base + q * C::kQTile, a.c.q, off);
+          }
+          arrive_when_landed(&m->q_full);
         }
         if (j >= lag) {
           const uint32_t st = op % C::kStages, slot = (tiles + j - lag) % kSlots;
@@ -709,7 +711,7 @@ __device__ __forceinline__ void softmax_role(const TcArgs& a, TcMeta* m, uint32_
           for (int c = 0; c < kKT; c += 64) {
             float s[64];
             uint32_t p[32];
-              tmem_ld32(ts + c, s);
+            tmem_ld32(ts + c, s);
             tmem_ld32(ts + c + 32, s + 32);
             tmem_wait_ld();
 #pragma unroll
@@ -906,6 +908,7 @@ chunk_tc_kernel(const __grid_constant__ TcArgs a) {
     fence_mbar_init();
     a.desc[blockIdx.x].parts = 0;
   }
+  pdl_launch_dependents();  // the merge's blocks wait for this grid's end on the SMs it leaves
   if (warp == 12) tmem_alloc(smem_u32(&m->tmem), 512);
   tc_fence_before();
   __syncthreads();
