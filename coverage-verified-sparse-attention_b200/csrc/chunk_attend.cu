@@ -58,21 +58,28 @@ __device__ __forceinline__ void load_row_piece(const T* src, float* dst) {  // 4
   }
 }
 
-template <int D>
+// fp32 pools are copied asynchronously into the buffer that the tile after
+// next frees; 256-wide heads (no room for two) and 16-bit pools (converted on
+// the way) are loaded through registers between two barriers.
+template <typename C, int D>
+constexpr int kBufs = sizeof(C) == 4 && D <= 128 ? 2 : 1;
+
+template <typename C, int D>
 struct GenSmem {
   float q[kRows][D + 4];
-  float k[kKeys][D + 4];
-  float v[kKeys][D + 4];
+  float k[kBufs<C, D>][kKeys][D + 4];
+  float v[kBufs<C, D>][kKeys][D + 4];
   float p[kRows][kKeys + 4];
-  int64_t key_off[kKeys];   // element offset of a key's row in the pools
-  int8_t key_ok[kKeys];
+  int64_t key_off[2][kKeys];   // element offset of a key's row in the pools
+  int8_t key_ok[2][kKeys];
   ChunkRange range;
 };
 
 template <typename T, typename C, int D>
-__global__ void __launch_bounds__(kThreads) chunk_general_kernel(GenArgs a) {
+__global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
+chunk_general_kernel(const __grid_constant__ GenArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  GenSmem<D>& sm = *reinterpret_cast<GenSmem<D>*>(smem_raw);
+  GenSmem<C, D>& sm = *reinterpret_cast<GenSmem<C, D>*>(smem_raw);
   const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
   const int cta = blockIdx.x;
   if (tid < 32) {
@@ -113,35 +120,67 @@ __global__ void __launch_bounds__(kThreads) chunk_general_kernel(GenArgs a) {
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) o[x][d] = 0.f;
     }
-    for (int k = it.k0; k < it.k1; ++k) {
-      const int base = (it.tile0 + k) * kKeys;
-      __syncthreads();  // the previous tile's reads are done
-      if (tid < kKeys) {
-        const int key = base + tid;
-        bool ok = key >= it.lo && key < it.hi;
-        int64_t off = 0;
-        if (ok) {
-          const int blk = a.rg.tables[(int64_t)it.q.slot * a.rg.W + key / a.kv.bs];
-          ok = blk >= 0 && blk < a.kv.num_blocks;
-          if (!ok) set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);
-          off = ok ? blk * a.kv.sb + (key % a.kv.bs) * a.kv.st + it.h * a.kv.sh : 0;
-        }
-        sm.key_off[tid] = off;
-        sm.key_ok[tid] = ok;
+    constexpr bool kAsync = kBufs<C, D> == 2;
+    // where the keys of tile k are, to record k % 2
+    auto locate = [&](int k) {
+      if (tid >= kKeys) return;
+      const int key = (it.tile0 + k) * kKeys + tid;
+      bool ok = key >= it.lo && key < it.hi;
+      int64_t off = 0;
+      if (ok) {
+        const int blk = a.rg.tables[(int64_t)it.q.slot * a.rg.W + key / a.kv.bs];
+        ok = blk >= 0 && blk < a.kv.num_blocks;
+        if (!ok) set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);
+        off = ok ? blk * a.kv.sb + (key % a.kv.bs) * a.kv.st + it.h * a.kv.sh : 0;
       }
-      __syncthreads();
+      sm.key_off[k & 1][tid] = off;
+      sm.key_ok[k & 1][tid] = ok;
+    };
+    auto copy = [&](int k) {
       for (int e = tid; e < kKeys * (D / 4); e += kThreads) {
         const int r = e / (D / 4), c = e % (D / 4);
-        float fk[4] = {0.f, 0.f, 0.f, 0.f}, fv[4] = {0.f, 0.f, 0.f, 0.f};
-        if (sm.key_ok[r]) {
-          const int64_t off = sm.key_off[r] + c * 4;
-          load_row_piece<C, D>(reinterpret_cast<const C*>(a.kv.k) + off, fk);
-          load_row_piece<C, D>(reinterpret_cast<const C*>(a.kv.v) + off, fv);
+        const bool ok = sm.key_ok[k & 1][r];
+        const int64_t off = sm.key_off[k & 1][r] + c * 4;
+        const C* kp = reinterpret_cast<const C*>(a.kv.k) + off;
+        const C* vp = reinterpret_cast<const C*>(a.kv.v) + off;
+        if constexpr (kAsync) {
+          const int n = ok ? 16 : 0;  // 0: zeros
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                           smem_u32(&sm.k[k & 1][r][c * 4])), "l"(kp), "r"(n) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                           smem_u32(&sm.v[k & 1][r][c * 4])), "l"(vp), "r"(n) : "memory");
+        } else {
+          float fk[4] = {0.f, 0.f, 0.f, 0.f}, fv[4] = {0.f, 0.f, 0.f, 0.f};
+          if (ok) {
+            load_row_piece<C, D>(kp, fk);
+            load_row_piece<C, D>(vp, fv);
+          }
+          *reinterpret_cast<float4*>(&sm.k[0][r][c * 4]) = make_float4(fk[0], fk[1], fk[2], fk[3]);
+          *reinterpret_cast<float4*>(&sm.v[0][r][c * 4]) = make_float4(fv[0], fv[1], fv[2], fv[3]);
         }
-        *reinterpret_cast<float4*>(&sm.k[r][c * 4]) = make_float4(fk[0], fk[1], fk[2], fk[3]);
-        *reinterpret_cast<float4*>(&sm.v[r][c * 4]) = make_float4(fv[0], fv[1], fv[2], fv[3]);
       }
+      if constexpr (kAsync) cp_async_commit();
+    };
+    if constexpr (kAsync) {  // records of two tiles, the first on its way
+      if (it.k0 < it.k1) locate(it.k0);
+      if (it.k0 + 1 < it.k1) locate(it.k0 + 1);
       __syncthreads();
+      if (it.k0 < it.k1) copy(it.k0);
+    }
+    for (int k = it.k0; k < it.k1; ++k) {
+      const int base = (it.tile0 + k) * kKeys;
+      const int rec = k & 1, buf = kAsync ? k & 1 : 0;
+      if constexpr (kAsync) {
+        cp_async_wait_dyn(0);
+        __syncthreads();  // this tile is there, and the tile before is done with
+        if (k + 1 < it.k1) copy(k + 1);
+      } else {
+        __syncthreads();  // the previous tile's reads are done
+        locate(k);
+        __syncthreads();
+        copy(k);
+        __syncthreads();
+      }
       float s[4][4];
 #pragma unroll
       for (int x = 0; x < 4; ++x)
@@ -153,7 +192,7 @@ __global__ void __launch_bounds__(kThreads) chunk_general_kernel(GenArgs a) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) qa[x] = *reinterpret_cast<float4*>(&sm.q[ty * 4 + x][d]);
 #pragma unroll
-        for (int y = 0; y < 4; ++y) kb[y] = *reinterpret_cast<float4*>(&sm.k[tx + 16 * y][d]);
+        for (int y = 0; y < 4; ++y) kb[y] = *reinterpret_cast<float4*>(&sm.k[buf][tx + 16 * y][d]);
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -172,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) chunk_general_kernel(GenArgs a) {
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
           const int c = tx + 16 * y, key = base + c;
-          see[y] = key >= lo[x] && key < hi[x] && sm.key_ok[c];
+          see[y] = key >= lo[x] && key < hi[x] && sm.key_ok[rec][c];
           cut |= !see[y];
           s[x][y] = see[y] ? s[x][y] * a.scale2 : neg_inf();
           if (see[y]) mx = fmaxf(mx, s[x][y]);
@@ -197,27 +236,33 @@ __global__ void __launch_bounds__(kThreads) chunk_general_kernel(GenArgs a) {
         for (int d = 0; d < D / 16; ++d) o[x][d] *= fix;
       }
       cut = __syncthreads_or(cut);
-#pragma unroll 2
-      for (int c = 0; c < kKeys; ++c) {
-        float p[4];
+      if (kAsync && k + 2 < it.k1) locate(k + 2);  // this tile's record was read before
+#pragma unroll 1
+      for (int c = 0; c < kKeys; c += 4) {
+        float p[4][4];  // four keys at a time: one wide load a row
 #pragma unroll
-        for (int x = 0; x < 4; ++x) p[x] = sm.p[ty * 4 + x][c];
-        float v[D / 16];
+        for (int x = 0; x < 4; ++x)
+          *reinterpret_cast<float4*>(p[x]) = *reinterpret_cast<float4*>(&sm.p[ty * 4 + x][c]);
 #pragma unroll
-        for (int y = 0; y < D / 64; ++y)
-          *reinterpret_cast<float4*>(v + 4 * y) =
-              *reinterpret_cast<float4*>(&sm.v[c][tx * 4 + 64 * y]);
-        if (!cut) {
+        for (int i = 0; i < 4; ++i) {
+          float v[D / 16];
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
+          for (int y = 0; y < D / 64; ++y)
+            *reinterpret_cast<float4*>(v + 4 * y) =
+                *reinterpret_cast<float4*>(&sm.v[buf][c + i][tx * 4 + 64 * y]);
+          if (!cut) {
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d) o[x][d] = fmaf(p[x], v[d], o[x][d]);
-        } else {
+            for (int x = 0; x < 4; ++x)
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
+              for (int d = 0; d < D / 16; ++d) o[x][d] = fmaf(p[x][i], v[d], o[x][d]);
+          } else {
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d)
-              o[x][d] = p[x] >= 0.f || p[x] != p[x] ? fmaf(p[x], v[d], o[x][d]) : o[x][d];
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+              for (int d = 0; d < D / 16; ++d)
+                o[x][d] = p[x][i] >= 0.f || p[x][i] != p[x][i] ? fmaf(p[x][i], v[d], o[x][d])
+                                                               : o[x][d];
+          }
         }
       }
     }
@@ -277,9 +322,9 @@ cudaError_t launch_general_d(const GenArgs& a, int ctas, cudaStream_t s) {
     return cudaGetLastError();
   };
   switch (a.kv.d) {
-    case 64: return go(chunk_general_kernel<T, C, 64>, sizeof(GenSmem<64>));
-    case 128: return go(chunk_general_kernel<T, C, 128>, sizeof(GenSmem<128>));
-    case 256: return go(chunk_general_kernel<T, C, 256>, sizeof(GenSmem<256>));
+    case 64: return go(chunk_general_kernel<T, C, 64>, sizeof(GenSmem<C, 64>));
+    case 128: return go(chunk_general_kernel<T, C, 128>, sizeof(GenSmem<C, 128>));
+    case 256: return go(chunk_general_kernel<T, C, 256>, sizeof(GenSmem<C, 256>));
     default: return cudaErrorInvalidValue;
   }
 }
@@ -299,7 +344,7 @@ cudaError_t launch_general_c(const GenArgs& a, int ctas, cudaStream_t s) {
 // Block (x, y): rows [32 x, 32 x + 32) of the item that begins in CTA y's range
 // and leaves it. Lanes own rows, warps own float4 columns. Parts are summed in
 // CTA order. Most blocks find no item and leave at once.
-constexpr int kMaxCtas = 256;
+constexpr int kMaxCtas = 320;
 
 struct MergeArgs {
   const float* parts;
@@ -381,7 +426,12 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(MergeArgs a) {
 // ---------------------------------------------------------------------------
 constexpr size_t kDescBytes = ((kMaxCtas * sizeof(ChunkMergeDesc) + 255) / 256) * 256;
 
-int chunk_ctas() { return num_sms() < kMaxCtas ? num_sms() : kMaxCtas; }
+// One CTA an SM; the general kernel's two where shared memory and registers
+// hold two (64-wide heads): one hides the other's barriers.
+int chunk_ctas(const KvView& kv, bool tc) {
+  const int n = num_sms() * (!tc && kv.d == 64 ? 2 : 1);
+  return n < kMaxCtas ? n : kMaxCtas;
+}
 
 ChunkGeo general_geo(const KvView& kv, const RaggedView& rg, const ChunkView& c) {
   ChunkGeo g;
@@ -407,15 +457,15 @@ bool chunk_attend_supported(const KvView& kv, const RaggedView& rg, const ChunkV
 
 size_t chunk_attend_workspace_bytes(const KvView& kv, const RaggedView& rg, const ChunkView& c) {
   const int rows = chunk_tc_eligible(kv, c) ? chunk_tc_rows() : kRows;
-  return kDescBytes + 2 * (size_t)chunk_ctas() * chunk_slot_floats(rows, kv.d) * 4;
+  return kDescBytes + 2 * (size_t)chunk_ctas(kv, chunk_tc_eligible(kv, c)) * chunk_slot_floats(rows, kv.d) * 4;
 }
 
 cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const ChunkView& c,
                                 void* ws, int32_t* dev_err, cudaStream_t s) {
-  const int ctas = chunk_ctas();
+  const bool tc = chunk_tc_eligible(kv, c);
+  const int ctas = chunk_ctas(kv, tc);
   ChunkMergeDesc* desc = reinterpret_cast<ChunkMergeDesc*>(ws);
   float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kDescBytes);
-  const bool tc = chunk_tc_eligible(kv, c);
   const bool split = tc ? chunk_tc_geo(kv, rg, c).split : general_geo(kv, rg, c).split;
   cudaError_t e;
   if (tc) {
