@@ -318,3 +318,24 @@ def test_mixed_items_in_one_cta(cuda, dtype, d):
     P = Problem(new, ctx, 28, 4, d, dtype=dtype, seed=22)
     check(P)
     check(P, window=100)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_wait_limit_runs_out_and_recovers(cuda, d):
+    """One poll a wait (about 4 us): the call ends with CVSA_DEV_ERR_TIMEOUT
+    instead of waiting, and the next call with the default limit is as before.
+    With thousands of sequences every CTA's plan takes several times a poll, and
+    the other warps wait for its first item."""
+    P = Problem([1] * 4000, [3 + i % 20 for i in range(4000)], 2, 1, d, seed=23)
+    first, _ = run(P)
+    assert int(P.dev_error.item()) == 0
+    lib = _lib.load()
+    lib.cvsa_set_wait_limit(1)
+    try:
+        run(P)
+    finally:
+        lib.cvsa_set_wait_limit(0)
+    assert int(P.dev_error.item()) == _lib.DEV_ERR_TIMEOUT
+    P.dev_error.zero_()
+    again, _ = run(P)
+    assert torch.equal(again, first) and int(P.dev_error.item()) == 0
