@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from typing import Optional
 
@@ -318,9 +319,14 @@ def query_desc(q: Optional[torch.Tensor], block_tables: torch.Tensor,
                      context_lens.data_ptr())
 
 
-def ragged_desc(num_tokens: int, cu_tokens: torch.Tensor, block_tables: torch.Tensor,
-                context_lens: torch.Tensor, seq_ids: Optional[torch.Tensor],
-                start_positions: Optional[torch.Tensor]) -> RaggedDesc:
+def ragged_desc(**kw) -> RaggedDesc:
+    """RaggedDesc of ragged_fields' arguments."""
+    return RaggedDesc(*ragged_fields(**kw))
+
+
+def ragged_fields(num_tokens: int, cu_tokens: torch.Tensor, block_tables: torch.Tensor,
+                  context_lens: torch.Tensor, seq_ids: Optional[torch.Tensor],
+                  start_positions: Optional[torch.Tensor]) -> tuple:
     """The packed new tokens of a batch and the tables of the sequences they belong to."""
     i32 = torch.int32
     for t in (cu_tokens, block_tables, context_lens, seq_ids, start_positions):
@@ -336,8 +342,39 @@ def ragged_desc(num_tokens: int, cu_tokens: torch.Tensor, block_tables: torch.Te
     for t in (seq_ids, start_positions):
         if t is not None and (t.dim() != 1 or t.numel() != B):
             raise ValueError("seq_ids and start_positions must be [batch]")
-    return RaggedDesc(cu_tokens.data_ptr(), ptr(seq_ids), ptr(start_positions),
-                      block_tables.data_ptr(), context_lens.data_ptr(), B, num_tokens, S, W)
+    return (cu_tokens.data_ptr(), 0 if seq_ids is None else seq_ids.data_ptr(),
+            0 if start_positions is None else start_positions.data_ptr(),
+            block_tables.data_ptr(), context_lens.data_ptr(), B, num_tokens, S, W)
+
+
+class _ArgMemory(threading.local):
+    """Per-thread argument structs of the ragged-batch calls over one buffer, which one
+    pack fills (constructing the three structs field by field costs 5 us a call)."""
+
+    _KV, _RG = "QQiiiiiiqqq", "QQQQQiiii"
+
+    def __init__(self):
+        self.buf = ctypes.create_string_buffer(64 + 56 + 152)
+        self.kv = KvDesc.from_buffer(self.buf, 0)
+        self.rg = RaggedDesc.from_buffer(self.buf, 64)
+        self.chunk = ChunkAttend.from_buffer(self.buf, 120)
+        self.rope = RopeAppend.from_buffer(self.buf, 120)
+        self.pack_chunk = struct.Struct("<" + self._KV + self._RG + "QQQiiqqqqfii").pack_into
+        self.pack_rope = struct.Struct("<" + self._KV + self._RG
+                                       + "QQQQiiqqqqqqqqQiiiiQQf").pack_into
+
+
+ARGS = _ArgMemory()
+
+
+def kv_fields(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple:
+    """KvDesc's fields (kv_desc's checks)."""
+    shape, stride = k_cache.shape, k_cache.stride()
+    if (len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != k_cache.dtype
+            or v_cache.stride() != stride or stride[3] != 1):
+        kv_desc(k_cache, v_cache)  # raises
+    return (k_cache.data_ptr(), v_cache.data_ptr(), dtype_code(k_cache.dtype), *shape, 0,
+            *stride[:3])
 
 
 def token_rows(t: torch.Tensor, name: str) -> torch.Tensor:

@@ -41,28 +41,29 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if k_cache.dim() != 4 or k_cache.shape[3] != D:
         raise ValueError("q's head_dim does not match the cache")
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(shape)
     elif out.shape != shape or out.dtype != q.dtype or out.stride(2) != 1:
         raise ValueError("out must have q's shape and dtype and contiguous rows")
     if lse is not None and (lse.shape != (T, Hq) or lse.dtype != torch.float32
                             or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous float32 [T, H_q]")
-    kvd = _lib.kv_desc(k_cache, v_cache)
-    rg = _lib.ragged_desc(T, cu_tokens, block_tables, context_lens, seq_ids, start_positions)
-    qs, os_ = q.stride(), out.stride()
-    args = _lib.ChunkAttend(q.data_ptr(), out.data_ptr(), _lib.ptr(lse), _lib.dtype_code(q.dtype),
-                            Hq, qs[0], qs[1], os_[0], os_[1],
-                            D ** -0.5 if scale is None else scale, causal, window)
+    qs, os_, mem = q.stride(), out.stride(), _lib.ARGS
+    mem.pack_chunk(mem.buf, 0, *_lib.kv_fields(k_cache, v_cache),
+                   *_lib.ragged_fields(T, cu_tokens, block_tables, context_lens, seq_ids,
+                                       start_positions),
+                   q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                   _lib.dtype_code(q.dtype), Hq, qs[0], qs[1], os_[0], os_[1],
+                   D ** -0.5 if scale is None else scale, causal, window)
     lib, stream = _lib.load(), _lib.raw_stream(dev)
     # the size depends on the head layout alone; 0 for what the call will refuse
     key = (dev, D, q.dtype, k_cache.dtype)
     nbytes = _ws_bytes.get(key)
     if nbytes is None:
-        nbytes = lib.cvsa_chunk_attend_workspace_size(kvd, rg, args)
+        nbytes = lib.cvsa_chunk_attend_workspace_size(mem.kv, mem.rg, mem.chunk)
         if nbytes:
             _ws_bytes[key] = nbytes
     ws = _lib.WORKSPACE.address(nbytes, q.device, stream, "chunk") if nbytes else None
-    st = lib.cvsa_chunk_attend(kvd, rg, args, _lib.ptr(dev_error), ws, nbytes, stream)
+    st = lib.cvsa_chunk_attend(mem.kv, mem.rg, mem.chunk, _lib.ptr(dev_error), ws, nbytes, stream)
     if st:
         _lib.check(st, "cvsa_chunk_attend")
     return out

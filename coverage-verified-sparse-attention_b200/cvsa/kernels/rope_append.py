@@ -65,14 +65,14 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
         raise ValueError("q, k and v dtypes differ")
     k, v = _lib.token_rows(k, "k"), _lib.token_rows(v, "v")
-    Hq, qs, os_, qp, op = 0, (0, 0), (0, 0), None, None
+    Hq, qs, os_, qp, op = 0, (0, 0), (0, 0), 0, 0
     if q is not None:
         if q.dim() != 3 or q.shape[0] != T or q.shape[2] != D:
             raise ValueError("q must be [T, H_q, D]")
         Hq = q.shape[1]
         q = _lib.token_rows(q, "q")
         if out is None:
-            out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+            out = q.new_empty((T, Hq, D))
         elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
             raise ValueError("out must have q's shape and dtype and contiguous rows")
         qs, os_ = q.stride(), out.stride()
@@ -91,14 +91,17 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous():
             raise ValueError("cos_sin must be a contiguous float32 [max_positions, rot_dim]")
         pos, rot = cos_sin.shape
-    rg = _lib.ragged_desc(T, cu_tokens, block_tables, context_lens, seq_ids, start_positions)
-    ks, vs = k.stride(), v.stride()
-    args = _lib.RopeAppend(qp, k.data_ptr(), v.data_ptr(), op, _lib.dtype_code(k.dtype), Hq,
-                           qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
-                           os_[0], os_[1], _lib.ptr(cos_sin), pos, rot, interleaved,
-                           _lib.dtype_code(ndt), _lib.ptr(q_norm), _lib.ptr(k_norm), eps)
-    st = _lib.load().cvsa_rope_append(_lib.kv_desc(k_cache, v_cache), rg, args,
-                                      _lib.ptr(dev_error), _lib.raw_stream(dev))
+    ks, vs, mem = k.stride(), v.stride(), _lib.ARGS
+    mem.pack_rope(mem.buf, 0, *_lib.kv_fields(k_cache, v_cache),
+                  *_lib.ragged_fields(T, cu_tokens, block_tables, context_lens, seq_ids,
+                                      start_positions),
+                  qp, k.data_ptr(), v.data_ptr(), op, _lib.dtype_code(k.dtype), Hq,
+                  qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1],
+                  0 if cos_sin is None else cos_sin.data_ptr(), pos, rot, interleaved,
+                  _lib.dtype_code(ndt), 0 if q_norm is None else q_norm.data_ptr(),
+                  0 if k_norm is None else k_norm.data_ptr(), eps)
+    st = _lib.load().cvsa_rope_append(mem.kv, mem.rg, mem.rope, _lib.ptr(dev_error),
+                                      _lib.raw_stream(dev))
     if st:
         _lib.check(st, "cvsa_rope_append")
     return out

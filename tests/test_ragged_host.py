@@ -143,3 +143,29 @@ def test_rope_table_values():
     ang = 49 * 500.0 ** (-2 * 3 / 32)
     assert abs(float(t[49, 3]) - torch.cos(torch.tensor(ang, dtype=torch.float64))) < 1e-7
     assert abs(float(t[49, 19]) - torch.sin(torch.tensor(ang, dtype=torch.float64))) < 1e-7
+
+
+def test_packed_arguments_are_the_structs():
+    """One pack fills the per-thread structs as their constructors would."""
+    mem = _lib.ARGS
+    kvf = (11, 12, 2, 10, 16, 2, 128, 0, 4096, 256, 128)
+    rgf = (21, 22, 23, 24, 25, 3, 9, 4, 7)
+    chf = (31, 32, 0, 1, 8, 1024, 128, 2048, 256, 0.5, True, 40)
+    rof = (41, 42, 43, 44, 2, 8, 1, 2, 3, 4, 5, 6, 7, 8, 45, 99, 64, True, 0, 46, 47, 0.25)
+
+    def same(got, want):
+        for name, _ in want._fields_:
+            assert getattr(got, name) == getattr(want, name), name
+
+    mem.pack_chunk(mem.buf, 0, *kvf, *rgf, *chf)
+    same(mem.kv, _lib.KvDesc(*kvf))
+    same(mem.rg, _lib.RaggedDesc(*rgf))
+    same(mem.chunk, _lib.ChunkAttend(*chf))
+    mem.pack_rope(mem.buf, 0, *kvf, *rgf, *rof)
+    same(mem.rope, _lib.RopeAppend(*rof))
+    k = torch.zeros(3, 16, 2, 64, dtype=torch.bfloat16)
+    same(_lib.KvDesc(*_lib.kv_fields(k, k)), _lib.kv_desc(k, k))
+    with pytest.raises(ValueError):
+        _lib.kv_fields(k, k.float())
+    with pytest.raises(ValueError):
+        _lib.kv_fields(k.transpose(2, 3), k.transpose(2, 3))
