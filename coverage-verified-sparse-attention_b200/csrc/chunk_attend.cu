@@ -370,6 +370,11 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(MergeArgs a) {
   };
   const bool live = r < ds.rows;
   float mx = neg_inf();
+  constexpr int kMine = 4;  // sums of this warp's first parts, loaded beside the maxima
+  float sums[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i)
+    sums[i] = live && wid + 8 * i < ds.parts ? slot(wid + 8 * i)[a.rows + r] : 0.f;
   for (int p = wid; p < ds.parts; p += 8) {
     const float m = live ? slot(p)[r] : neg_inf();
     w[p][lane] = m;
@@ -382,7 +387,15 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(MergeArgs a) {
   __syncthreads();
   const float ref = mx == neg_inf() ? 0.f : mx;
   float l = 0.f;
-  for (int p = wid; p < ds.parts; p += 8) {
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int p = wid + 8 * i;
+    if (p >= ds.parts) break;
+    const float e = exp2f(w[p][lane] - ref);
+    w[p][lane] = e;
+    l += e * sums[i];
+  }
+  for (int p = wid + 8 * kMine; p < ds.parts; p += 8) {
     const float e = exp2f(w[p][lane] - ref);
     w[p][lane] = e;
     l += live ? e * slot(p)[a.rows + r] : 0.f;

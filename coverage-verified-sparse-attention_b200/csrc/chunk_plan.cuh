@@ -44,25 +44,27 @@ struct SeqInfo {
 // Sequence b; every field ends in range whatever the arrays hold.
 __device__ __forceinline__ SeqInfo chunk_seq(const RaggedView& rg, int bs, int b,
                                              int32_t* dev_err) {
+  // every load before the first check, so that they wait for one another only
+  // where one names the next
   SeqInfo q;
   q.tok0 = rg.cu[b];
   const int end = rg.cu[b + 1];
   q.slot = rg.seq_ids ? rg.seq_ids[b] : b;
+  const bool row_ok = q.slot >= 0 && q.slot < rg.num_seqs;
+  q.ctx = row_ok ? rg.lens[q.slot] : 0;
+  const int start = rg.starts ? rg.starts[b] : 0;
   q.n = end - q.tok0;
-  q.start = q.ctx = 0;
-  if (q.tok0 < 0 || end > rg.T || end < q.tok0 || q.slot < 0 || q.slot >= rg.num_seqs) {
+  q.start = rg.starts ? start : q.ctx - q.n;
+  if (q.tok0 < 0 || end > rg.T || end < q.tok0 || !row_ok) {
     set_dev_error(dev_err, CVSA_DEV_ERR_RAGGED);
-    q.n = 0;
-    q.slot = 0;
+    q.n = q.slot = q.start = q.ctx = 0;
     return q;
   }
-  q.ctx = rg.lens[q.slot];
-  q.start = rg.starts ? rg.starts[b] : q.ctx - q.n;
   if (q.ctx < 0 || q.ctx > (int64_t)rg.W * bs) {
     set_dev_error(dev_err, CVSA_DEV_ERR_RAGGED);
     q.ctx = q.ctx < 0 ? 0 : rg.W * bs;
   }
-  if (rg.starts && q.start < 0) q.start = q.ctx = 0;  // refused: its rows see no key
+  if (rg.starts && start < 0) q.start = q.ctx = 0;  // refused: its rows see no key
   return q;
 }
 
