@@ -166,7 +166,7 @@ int check_chunk(const cvsa_chunk_attend_t* a, const KvView& kv, const RaggedView
   out->o_sh = a->out_stride_head;
   out->scale = a->scale;
   out->causal = a->causal != 0;
-  out->window = a->window;
+  out->window = a->window < (1 << 30) ? a->window : 1 << 30;  // positions less a window fit
   if (!chunk_attend_supported(kv, rg, *out))
     return fail(CVSA_ERR_UNSUPPORTED,
                 "chunk_attend built for head_dim 64/128/256, G<=64, and fewer than 2^31 key tiles "

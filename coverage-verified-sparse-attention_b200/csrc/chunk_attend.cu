@@ -10,11 +10,11 @@
 // so values of keys a row does not see cannot reach it, NaN and infinities
 // included.
 //
-// General kernel: one CTA walks its range of items (chunk_plan.cuh), 64 query
-// rows against tiles of 64 keys on the CUDA cores in fp32, each thread a 4 x 4
-// block of scores and 4 x D/16 of the output. It is bound by fp32 FMA issue
-// and serves fp32 caches, mixed types and 256-wide heads; 16-bit caches with
-// 64- and 128-wide heads run in chunk_attend_tc.cu.
+// General kernel: a CTA walks its range of items (chunk_plan.cuh), 64 or 128
+// query rows against tiles of 64 keys on the CUDA cores in fp32, each thread a
+// block of 4 x 4 or 8 x 4 scores and as many rows by D/16 of the output. It is
+// bound by fp32 FMA issue and serves fp32 caches, mixed types and 256-wide
+// heads; 16-bit caches with 64- and 128-wide heads run in chunk_attend_tc.cu.
 #include <type_traits>
 
 #include "chunk_plan.cuh"
@@ -25,7 +25,15 @@
 namespace cvsa {
 namespace {
 
-constexpr int kRows = 64, kKeys = 64, kThreads = 256;
+constexpr int kKeys = 64, kThreads = 256;
+// Query rows of an item: 64, 4 by 4 scores a thread, or, for 128-wide heads and
+// sequences that fill them, 128, 8 by 4 (a thread's block sets how many FMAs a
+// shared-memory load feeds: 1000 tokens at 8000 keys, fp32, 3.7 ms instead of
+// 4.3; one token of 16 sequences 1.7 ms instead of 1.1).
+int gen_rows(const RaggedView& rg, const KvView& kv, int G) {
+  return kv.d == 128 && (int64_t)rg.T * G >= (int64_t)128 * rg.B ? 128 : 64;
+}
+constexpr int gen_max_rows(int d) { return d == 128 ? 128 : 64; }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct GenArgs {
@@ -58,28 +66,26 @@ __device__ __forceinline__ void load_row_piece(const T* src, float* dst) {  // 4
   }
 }
 
-// fp32 pools are copied asynchronously into the buffer that the tile after
-// next frees; 256-wide heads (no room for two) and 16-bit pools (converted on
-// the way) are loaded through registers between two barriers.
-template <typename C, int D>
-constexpr int kBufs = sizeof(C) == 4 && D <= 128 ? 2 : 1;
-
-template <typename C, int D>
+// K and V have a buffer each: the next K is copied (asynchronously, from an
+// fp32 pool) while the weights and the output are formed, the next V while the
+// next scores are. 16-bit pools are converted on the way, through registers.
+template <int D, int ROWS>
 struct GenSmem {
-  float q[kRows][D + 4];
-  float k[kBufs<C, D>][kKeys][D + 4];
-  float v[kBufs<C, D>][kKeys][D + 4];
-  float p[kRows][kKeys + 4];
+  float q[ROWS][D + 4];
+  float k[kKeys][D + 4];
+  float v[kKeys][D + 4];
+  float p[ROWS][kKeys + 4];
   int64_t key_off[2][kKeys];   // element offset of a key's row in the pools
   int8_t key_ok[2][kKeys];
   ChunkRange range;
 };
 
-template <typename T, typename C, int D>
+template <typename T, typename C, int D, int kRows>
 __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
 chunk_general_kernel(const __grid_constant__ GenArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  GenSmem<C, D>& sm = *reinterpret_cast<GenSmem<C, D>*>(smem_raw);
+  constexpr int kX = kRows / 16;  // rows of a thread
+  GenSmem<D, kRows>& sm = *reinterpret_cast<GenSmem<D, kRows>*>(smem_raw);
   const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
   const int cta = blockIdx.x;
   if (tid < 32) {
@@ -95,6 +101,7 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
   const int G = a.g.G;
   while (walk.next(a.rg, a.g, cta, it)) {
     const int rows = (it.t1 - it.t0) * G;
+    const bool busy = (ty & ~1) * kX < rows;  // a warp none of whose rows exist only copies
     // query rows: token t0 + r / G, head h * G + r % G
     for (int e = tid; e < kRows * (D / 4); e += kThreads) {
       const int r = e / (D / 4), c = e % (D / 4);
@@ -107,11 +114,11 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
       }
       *reinterpret_cast<float4*>(&sm.q[r][c * 4]) = make_float4(f[0], f[1], f[2], f[3]);
     }
-    int lo[4], hi[4];
-    float m[4], l[4], o[4][D / 16];
+    int lo[kX], hi[kX];
+    float m[kX], l[kX], o[kX][D / 16];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int r = ty * 4 + x;
+    for (int x = 0; x < kX; ++x) {
+      const int r = ty * kX + x;
       const int pos = it.q.start + it.t0 + r / G;
       hi[x] = r >= rows ? 0 : a.g.causal ? max(0, min(it.q.ctx, pos + 1)) : it.q.ctx;
       lo[x] = a.g.window > 0 ? max(0, pos - a.g.window + 1) : 0;
@@ -120,7 +127,7 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) o[x][d] = 0.f;
     }
-    constexpr bool kAsync = kBufs<C, D> == 2;
+    constexpr bool kAsync = sizeof(C) == 4;
     // where the keys of tile k are, to record k % 2
     auto locate = [&](int k) {
       if (tid >= kKeys) return;
@@ -136,65 +143,47 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
       sm.key_off[k & 1][tid] = off;
       sm.key_ok[k & 1][tid] = ok;
     };
-    auto copy = [&](int k) {
-      for (int e = tid; e < kKeys * (D / 4); e += kThreads) {
-        const int r = e / (D / 4), c = e % (D / 4);
-        const bool ok = sm.key_ok[k & 1][r];
-        const int64_t off = sm.key_off[k & 1][r] + c * 4;
-        const C* kp = reinterpret_cast<const C*>(a.kv.k) + off;
-        const C* vp = reinterpret_cast<const C*>(a.kv.v) + off;
-        if constexpr (kAsync) {
-          const int n = ok ? 16 : 0;  // 0: zeros
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                           smem_u32(&sm.k[k & 1][r][c * 4])), "l"(kp), "r"(n) : "memory");
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                           smem_u32(&sm.v[k & 1][r][c * 4])), "l"(vp), "r"(n) : "memory");
-        } else {
-          float fk[4] = {0.f, 0.f, 0.f, 0.f}, fv[4] = {0.f, 0.f, 0.f, 0.f};
-          if (ok) {
-            load_row_piece<C, D>(kp, fk);
-            load_row_piece<C, D>(vp, fv);
+    auto copy = [&](int k, const void* pool, float (*to)[D + 4]) {
+      if (k < it.k1) {
+        for (int e = tid; e < kKeys * (D / 4); e += kThreads) {
+          const int r = e / (D / 4), c = e % (D / 4);
+          const bool ok = sm.key_ok[k & 1][r];
+          const C* src = reinterpret_cast<const C*>(pool) + sm.key_off[k & 1][r] + c * 4;
+          if constexpr (kAsync) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                             smem_u32(&to[r][c * 4])), "l"(src), "r"(ok ? 16 : 0) : "memory");
+          } else {
+            float f[4] = {0.f, 0.f, 0.f, 0.f};
+            if (ok) load_row_piece<C, D>(src, f);
+            *reinterpret_cast<float4*>(&to[r][c * 4]) = make_float4(f[0], f[1], f[2], f[3]);
           }
-          *reinterpret_cast<float4*>(&sm.k[0][r][c * 4]) = make_float4(fk[0], fk[1], fk[2], fk[3]);
-          *reinterpret_cast<float4*>(&sm.v[0][r][c * 4]) = make_float4(fv[0], fv[1], fv[2], fv[3]);
         }
       }
       if constexpr (kAsync) cp_async_commit();
     };
-    if constexpr (kAsync) {  // records of two tiles, the first on its way
-      if (it.k0 < it.k1) locate(it.k0);
-      if (it.k0 + 1 < it.k1) locate(it.k0 + 1);
-      __syncthreads();
-      if (it.k0 < it.k1) copy(it.k0);
-    }
+    if (it.k0 < it.k1) locate(it.k0);
+    __syncthreads();
+    copy(it.k0, a.kv.k, sm.k);
+    copy(it.k0, a.kv.v, sm.v);
     for (int k = it.k0; k < it.k1; ++k) {
-      const int base = (it.tile0 + k) * kKeys;
-      const int rec = k & 1, buf = kAsync ? k & 1 : 0;
-      if constexpr (kAsync) {
-        cp_async_wait_dyn(0);
-        __syncthreads();  // this tile is there, and the tile before is done with
-        if (k + 1 < it.k1) copy(k + 1);
-      } else {
-        __syncthreads();  // the previous tile's reads are done
-        locate(k);
-        __syncthreads();
-        copy(k);
-        __syncthreads();
-      }
-      float s[4][4];
+      const int base = (it.tile0 + k) * kKeys, rec = k & 1;
+      if (k + 1 < it.k1) locate(k + 1);
+      if constexpr (kAsync) cp_async_wait_dyn(1);  // K; V may be on its way
+      __syncthreads();
+      float s[kX][4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
+      for (int x = 0; x < kX; ++x)
 #pragma unroll
         for (int y = 0; y < 4; ++y) s[x][y] = 0.f;
-#pragma unroll 4
-      for (int d = 0; d < D; d += 4) {
-        float4 qa[4], kb[4];
+#pragma unroll 2
+      for (int d = busy ? 0 : D; d < D; d += 4) {
+        float4 qa[kX], kb[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) qa[x] = *reinterpret_cast<float4*>(&sm.q[ty * 4 + x][d]);
+        for (int x = 0; x < kX; ++x) qa[x] = *reinterpret_cast<float4*>(&sm.q[ty * kX + x][d]);
 #pragma unroll
-        for (int y = 0; y < 4; ++y) kb[y] = *reinterpret_cast<float4*>(&sm.k[buf][tx + 16 * y][d]);
+        for (int y = 0; y < 4; ++y) kb[y] = *reinterpret_cast<float4*>(&sm.k[tx + 16 * y][d]);
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < kX; ++x)
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             s[x][y] = fmaf(qa[x].x, kb[y].x, s[x][y]);
@@ -203,9 +192,11 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
             s[x][y] = fmaf(qa[x].w, kb[y].w, s[x][y]);
           }
       }
+      __syncthreads();  // K is done with
+      copy(k + 1, a.kv.k, sm.k);
       bool cut = false;  // some row of the block does not see every key of the tile
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
+      for (int x = 0; x < kX; ++x) {
         float mx = m[x];
         bool see[4];
 #pragma unroll
@@ -226,7 +217,7 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
           const float p = see[y] ? exp2f(s[x][y] - ref) : 0.f;
           sum += p;
           // an unseen key is marked by a negative weight
-          sm.p[ty * 4 + x][tx + 16 * y] = see[y] ? p : -1.f;
+          sm.p[ty * kX + x][tx + 16 * y] = see[y] ? p : -1.f;
         }
 #pragma unroll
         for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
@@ -235,29 +226,29 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) o[x][d] *= fix;
       }
+      if constexpr (kAsync) cp_async_wait_dyn(1);  // V; the next K may be on its way
       cut = __syncthreads_or(cut);
-      if (kAsync && k + 2 < it.k1) locate(k + 2);  // this tile's record was read before
 #pragma unroll 1
-      for (int c = 0; c < kKeys; c += 4) {
-        float p[4][4];  // four keys at a time: one wide load a row
+      for (int c = busy ? 0 : kKeys; c < kKeys; c += 4) {
+        float p[kX][4];  // four keys at a time: one wide load a row
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          *reinterpret_cast<float4*>(p[x]) = *reinterpret_cast<float4*>(&sm.p[ty * 4 + x][c]);
+        for (int x = 0; x < kX; ++x)
+          *reinterpret_cast<float4*>(p[x]) = *reinterpret_cast<float4*>(&sm.p[ty * kX + x][c]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float v[D / 16];
 #pragma unroll
           for (int y = 0; y < D / 64; ++y)
             *reinterpret_cast<float4*>(v + 4 * y) =
-                *reinterpret_cast<float4*>(&sm.v[buf][c + i][tx * 4 + 64 * y]);
+                *reinterpret_cast<float4*>(&sm.v[c + i][tx * 4 + 64 * y]);
           if (!cut) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
+            for (int x = 0; x < kX; ++x)
 #pragma unroll
               for (int d = 0; d < D / 16; ++d) o[x][d] = fmaf(p[x][i], v[d], o[x][d]);
           } else {
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
+            for (int x = 0; x < kX; ++x)
 #pragma unroll
               for (int d = 0; d < D / 16; ++d)
                 o[x][d] = p[x][i] >= 0.f || p[x][i] != p[x][i] ? fmaf(p[x][i], v[d], o[x][d])
@@ -265,12 +256,14 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
           }
         }
       }
+      __syncthreads();  // V and the weights are done with
+      copy(k + 1, a.kv.v, sm.v);
     }
     // whole items are finished here, pieces go to a partial slot
     if (it.whole) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int r = ty * 4 + x;
+      for (int x = 0; x < kX; ++x) {
+        const int r = ty * kX + x;
         if (r >= rows) continue;
         const int64_t tok = it.q.tok0 + it.t0 + r / G;
         const int head = it.h * G + r % G;
@@ -286,8 +279,8 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
     } else {
       float* part = a.parts + (size_t)(2 * cta + it.slot) * chunk_slot_floats(kRows, D);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int r = ty * 4 + x;
+      for (int x = 0; x < kX; ++x) {
+        const int r = ty * kX + x;
         if (r >= rows) continue;
         if (tx == 0) {
           part[r] = m[x];
@@ -313,7 +306,7 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
 }
 
 template <typename T, typename C>
-cudaError_t launch_general_d(const GenArgs& a, int ctas, cudaStream_t s) {
+cudaError_t launch_general_d(const GenArgs& a, int rows, int ctas, cudaStream_t s) {
   auto go = [&](auto kernel, size_t smem) -> cudaError_t {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
@@ -322,19 +315,21 @@ cudaError_t launch_general_d(const GenArgs& a, int ctas, cudaStream_t s) {
     return cudaGetLastError();
   };
   switch (a.kv.d) {
-    case 64: return go(chunk_general_kernel<T, C, 64>, sizeof(GenSmem<C, 64>));
-    case 128: return go(chunk_general_kernel<T, C, 128>, sizeof(GenSmem<C, 128>));
-    case 256: return go(chunk_general_kernel<T, C, 256>, sizeof(GenSmem<C, 256>));
+    case 64: return go(chunk_general_kernel<T, C, 64, 64>, sizeof(GenSmem<64, 64>));
+    case 128:
+      if (rows == 64) return go(chunk_general_kernel<T, C, 128, 64>, sizeof(GenSmem<128, 64>));
+      return go(chunk_general_kernel<T, C, 128, 128>, sizeof(GenSmem<128, 128>));
+    case 256: return go(chunk_general_kernel<T, C, 256, 64>, sizeof(GenSmem<256, 64>));
     default: return cudaErrorInvalidValue;
   }
 }
 
 template <typename T>
-cudaError_t launch_general_c(const GenArgs& a, int ctas, cudaStream_t s) {
+cudaError_t launch_general_c(const GenArgs& a, int rows, int ctas, cudaStream_t s) {
   switch (a.kv.dtype) {
-    case CVSA_DTYPE_BF16: return launch_general_d<T, __nv_bfloat16>(a, ctas, s);
-    case CVSA_DTYPE_F16: return launch_general_d<T, __half>(a, ctas, s);
-    default: return launch_general_d<T, float>(a, ctas, s);
+    case CVSA_DTYPE_BF16: return launch_general_d<T, __nv_bfloat16>(a, rows, ctas, s);
+    case CVSA_DTYPE_F16: return launch_general_d<T, __half>(a, rows, ctas, s);
+    default: return launch_general_d<T, float>(a, rows, ctas, s);
   }
 }
 
@@ -451,7 +446,7 @@ ChunkGeo general_geo(const KvView& kv, const RaggedView& rg, const ChunkView& c)
   g.bs = kv.bs;
   g.hkv = kv.hkv;
   g.G = c.hq / kv.hkv;
-  g.P = kRows / g.G;
+  g.P = gen_rows(rg, kv, g.G) / g.G;
   g.KT = kKeys;
   g.causal = c.causal;
   g.window = c.window;
@@ -463,13 +458,13 @@ ChunkGeo general_geo(const KvView& kv, const RaggedView& rg, const ChunkView& c)
 }  // namespace
 
 bool chunk_attend_supported(const KvView& kv, const RaggedView& rg, const ChunkView& c) {
-  return (kv.d == 64 || kv.d == 128 || kv.d == 256) && c.hq / kv.hkv <= kRows &&
+  return (kv.d == 64 || kv.d == 128 || kv.d == 256) && c.hq / kv.hkv <= 64 &&
          chunk_fits(rg, chunk_tc_eligible(kv, c) ? chunk_tc_geo(kv, rg, c)
                                                  : general_geo(kv, rg, c));
 }
 
 size_t chunk_attend_workspace_bytes(const KvView& kv, const RaggedView& rg, const ChunkView& c) {
-  const int rows = chunk_tc_eligible(kv, c) ? chunk_tc_rows() : kRows;
+  const int rows = chunk_tc_eligible(kv, c) ? chunk_tc_rows() : gen_max_rows(kv.d);
   return kDescBytes + 2 * (size_t)chunk_ctas(kv, chunk_tc_eligible(kv, c)) * chunk_slot_floats(rows, kv.d) * 4;
 }
 
@@ -477,6 +472,7 @@ cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const Ch
                                 void* ws, int32_t* dev_err, cudaStream_t s) {
   const bool tc = chunk_tc_eligible(kv, c);
   const int ctas = chunk_ctas(kv, tc);
+  const int rows = tc ? chunk_tc_rows() : gen_rows(rg, kv, c.hq / kv.hkv);  // of an item
   ChunkMergeDesc* desc = reinterpret_cast<ChunkMergeDesc*>(ws);
   float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kDescBytes);
   const bool split = tc ? chunk_tc_geo(kv, rg, c).split : general_geo(kv, rg, c).split;
@@ -495,9 +491,9 @@ cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const Ch
     a.parts = parts;
     a.dev_err = dev_err;
     switch (c.dtype) {
-      case CVSA_DTYPE_BF16: e = launch_general_c<__nv_bfloat16>(a, ctas, s); break;
-      case CVSA_DTYPE_F16: e = launch_general_c<__half>(a, ctas, s); break;
-      default: e = launch_general_c<float>(a, ctas, s); break;
+      case CVSA_DTYPE_BF16: e = launch_general_c<__nv_bfloat16>(a, rows, ctas, s); break;
+      case CVSA_DTYPE_F16: e = launch_general_c<__half>(a, rows, ctas, s); break;
+      default: e = launch_general_c<float>(a, rows, ctas, s); break;
     }
   }
   if (e != cudaSuccess || !split) return e;
@@ -505,11 +501,11 @@ cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const Ch
   m.parts = parts;
   m.desc = desc;
   m.c = c;
-  m.rows = tc ? chunk_tc_rows() : kRows;
+  m.rows = rows;
   m.G = c.hq / kv.hkv;
   m.d = kv.d;
-  const int64_t rows = (int64_t)rg.T * m.G;  // of an item, at most
-  const dim3 grid(((rows < m.rows ? (int)rows : m.rows) + 31) / 32, ctas);
+  const int64_t all = (int64_t)rg.T * m.G;
+  const dim3 grid(((all < rows ? (int)all : rows) + 31) / 32, ctas);
   switch (c.dtype) {
     case CVSA_DTYPE_BF16:
       return launch_k(chunk_merge_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, true, m);

@@ -57,7 +57,7 @@ def test_page_sizes(cuda, dtype, page):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
-@pytest.mark.parametrize("window", [1, 2, 17, 128, 130, 5000])
+@pytest.mark.parametrize("window", [1, 2, 17, 128, 130, 5000, 2 ** 31 - 1])
 def test_window(cuda, dtype, window):
     check(Problem([150, 1, 20], [700, 400, 20], 8, 2, 128, dtype=dtype, seed=window),
           window=window)
