@@ -450,7 +450,8 @@ ChunkGeo general_geo(const KvView& kv, const RaggedView& rg, const ChunkView& c)
   g.KT = kKeys;
   g.causal = c.causal;
   g.window = c.window;
-  g.fixed = 1;
+  g.fixed = g.fixed_few = 1;
+  g.few = 0;
   g.split = chunk_may_split(rg, kv.bs, kKeys);
   return g;
 }

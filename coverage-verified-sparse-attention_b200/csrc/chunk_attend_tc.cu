@@ -962,6 +962,8 @@ ChunkGeo chunk_tc_geo(const KvView& kv, const RaggedView& rg, const ChunkView& c
   g.causal = c.causal;
   g.window = c.window;
   g.fixed = 2;
+  g.few = kPairRows;
+  g.fixed_few = 4;
   g.split = chunk_may_split(rg, kv.bs, kKT);
   return g;
 }

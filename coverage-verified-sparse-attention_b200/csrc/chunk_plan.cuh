@@ -32,6 +32,7 @@ struct ChunkGeo {
   int KT;       // keys a tile
   int causal, window;
   int fixed;    // units an item counts beside its tiles
+  int few, fixed_few;  // the same for items of at most `few` rows
   int split;    // items may cross ranges
 };
 
@@ -81,10 +82,14 @@ __device__ __forceinline__ int chunk_tiles(int lo, int hi, int KT) {
   return hi > lo ? (hi + KT - 1) / KT - lo / KT : 0;
 }
 
+__device__ __forceinline__ int chunk_fixed(const ChunkGeo& g, int tokens) {
+  return tokens * g.G <= g.few ? g.fixed_few : g.fixed;
+}
+
 __device__ __forceinline__ int chunk_units(const SeqInfo& q, const ChunkGeo& g, int i) {
   int lo, hi;
   chunk_keys(q, g, i * g.P, min(q.n, (i + 1) * g.P), lo, hi);
-  return chunk_tiles(lo, hi, g.KT) + g.fixed;
+  return chunk_tiles(lo, hi, g.KT) + chunk_fixed(g, min(q.n - i * g.P, g.P));
 }
 
 // What a CTA does: units [u0, u1) of the stream, starting at unit `skip` of
@@ -221,7 +226,7 @@ struct ChunkWalk {
       it.t0 = i * g.P;
       it.t1 = min(q.n, it.t0 + g.P);
       chunk_keys(q, g, it.t0, it.t1, it.lo, it.hi);
-      const int tiles = chunk_tiles(it.lo, it.hi, g.KT), units = tiles + g.fixed;
+      const int tiles = chunk_tiles(it.lo, it.hi, g.KT), units = tiles + chunk_fixed(g, it.t1 - it.t0);
       const int k0 = skip, k1 = g.split ? min(units, skip + (r.u1 - u)) : units;
       const int first = u - skip;
       u += k1 - k0;
@@ -257,7 +262,7 @@ __host__ __device__ constexpr size_t chunk_slot_floats(int rows, int d) {
 // Whether a call's units fit 31 bits, and whether its items may be split.
 inline bool chunk_fits(const RaggedView& rg, const ChunkGeo& g) {
   const int64_t tiles = ((int64_t)rg.W * g.bs + g.KT - 1) / g.KT + 1;
-  return ((int64_t)rg.T / g.P + rg.B + 1) * g.hkv * (tiles + g.fixed) < (int64_t(1) << 31);
+  return ((int64_t)rg.T / g.P + rg.B + 1) * g.hkv * (tiles + g.fixed + g.fixed_few) < (int64_t(1) << 31);
 }
 inline int chunk_may_split(const RaggedView& rg, int bs, int KT) {
   // up to four tiles: less than the merge's launch and the partials' way
