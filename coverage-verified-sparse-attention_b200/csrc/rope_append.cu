@@ -141,6 +141,7 @@ struct RopeArgs {
   RopeView r;
   int rows_per_token;
   uint32_t rows;  // T * rows_per_token, below 2^31
+  int bs_shift;   // log2 of the page size, or -1
   int32_t* dev_err;
 };
 
@@ -190,7 +191,7 @@ __device__ __forceinline__ int warp_find_seq(const int32_t* cu, int B, int t) {
 }
 
 template <typename T, typename C, int U>  // input type, cache type, lanes a row (head_dim / 16)
-__global__ void __launch_bounds__(256) rope_append_kernel(RopeArgs a) {
+__global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int D = U * 16, RPW = 32 / U;
   const int lane = threadIdx.x & 31, u = lane % U;
   const uint32_t row0 = ((blockIdx.x * 256 + threadIdx.x) >> 5) * RPW;
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(256) rope_append_kernel(RopeArgs a) {
     if (t == tok) b = f;
   }
   const bool rotate = a.r.cos_sin != nullptr && kind != 2;
-  int pos = -1, slot = -1;
+  int pos = -1, slot = -1, page = 0;
   bool good = live && b >= 0;
   if (good) {
     slot = a.rg.seq_ids ? a.rg.seq_ids[b] : b;
@@ -241,14 +242,15 @@ __global__ void __launch_bounds__(256) rope_append_kernel(RopeArgs a) {
     } else {
       pos = a.rg.lens[slot] - (a.rg.cu[b + 1] - tok);
     }
-    if (good && (pos < 0 || pos / a.kv.bs >= a.rg.W ||
+    page = a.bs_shift >= 0 ? pos >> a.bs_shift : pos / a.kv.bs;
+    if (good && (pos < 0 || page >= a.rg.W ||
                  (a.r.cos_sin && pos >= a.r.max_positions))) {
       good = false;
       if (u == 0) set_dev_error(a.dev_err, CVSA_DEV_ERR_RAGGED);
     }
   }
   int blk = 0;
-  if (good && kind != 0) blk = a.rg.tables[(int64_t)slot * a.rg.W + pos / a.kv.bs];
+  if (good && kind != 0) blk = a.rg.tables[(int64_t)slot * a.rg.W + page];
   float cs[16];
   if (good && rotate && in_rot) {
     const float* c = a.r.cos_sin + (int64_t)pos * a.r.rot + u * 8;
@@ -259,10 +261,12 @@ __global__ void __launch_bounds__(256) rope_append_kernel(RopeArgs a) {
   }
   const void* wn = kind == 0 ? a.r.q_norm : kind == 1 ? a.r.k_norm : nullptr;
   float ss = 0.f;
+  if (a.r.q_norm || a.r.k_norm) {  // every lane, for the shuffles
 #pragma unroll
-  for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
+    for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
-  for (int o = U / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    for (int o = U / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  }
   if (wn) {
     float w[16];
     if (a.r.norm_f32) {
@@ -310,7 +314,7 @@ __global__ void __launch_bounds__(256) rope_append_kernel(RopeArgs a) {
     return;
   }
   void* pool = const_cast<void*>(kind == 1 ? a.kv.k : a.kv.v);
-  const int64_t at = blk * a.kv.sb + (pos % a.kv.bs) * a.kv.st + h * a.kv.sh;
+  const int64_t at = blk * a.kv.sb + (pos - page * a.kv.bs) * a.kv.st + h * a.kv.sh;
   store8<C>(pool, at + e0, x);
   store8<C>(pool, at + e1, x + 8);
 }
@@ -363,6 +367,9 @@ cudaError_t launch_rope_append(const RaggedView& rg, const KvView& kv, const Rop
   a.rows_per_token = r.hq + 2 * kv.hkv;
   a.rows = (uint32_t)rg.T * (uint32_t)a.rows_per_token;
   a.dev_err = dev_err;
+  a.bs_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (kv.bs == 1 << i) a.bs_shift = i;
   switch (r.dtype) {
     case CVSA_DTYPE_BF16: return launch_rc<__nv_bfloat16>(a, s);
     case CVSA_DTYPE_F16: return launch_rc<__half>(a, s);
