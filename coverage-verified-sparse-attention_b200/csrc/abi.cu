@@ -1112,6 +1112,12 @@ int cvsa_rope_append(const cvsa_kv_desc_t* kvd, const cvsa_ragged_desc_t* rgd,
     return fail(CVSA_ERR_INVALID, "q/k/v/q_out rows, cos_sin and weights must be 16-byte aligned");
   if ((int64_t)rg.T * (hq + 2 * (int64_t)kv.hkv) >= (int64_t(1) << 31))
     return fail(CVSA_ERR_UNSUPPORTED, "num_tokens * heads above 2^31");
+  for (int64_t st : {args->k_stride_token, args->k_stride_head, args->v_stride_token,
+                     args->v_stride_head, kv.st, kv.sh, hq ? args->q_stride_token : 0,
+                     hq ? args->q_stride_head : 0, hq ? args->q_out_stride_token : 0,
+                     hq ? args->q_out_stride_head : 0})
+    if (st >= (int64_t(1) << 31) || st < -(int64_t(1) << 31))
+      return fail(CVSA_ERR_UNSUPPORTED, "token and head strides must fit 32 bits");
   if (rg.B == 0 || rg.T == 0) return CVSA_OK;
   RopeView r;
   r.q = args->q;

@@ -17,8 +17,10 @@
 // latency for a few tokens. A row is held by D/16 neighbouring lanes, 16
 // elements (8 pairs) a lane, so a rotation never leaves its lane and a norm is
 // a few shuffles; rows are independent, so there is no shared memory and no
-// block-wide barrier. The row's data loads are issued before the lookup of
-// its token (sequence, position, block id), whose dependent loads they hide.
+// block-wide barrier. A block holds rows of one token, so that the lookup
+// (sequence, position, block id) is uniform; the row's data loads are issued before it. It is bound by
+// instruction issue and occupancy together: several rows a lane, or a lookup a
+// token shared through shared memory, cost more in registers than they saved.
 #include "cvsa_common.cuh"
 #include "cvsa_internal.h"
 
@@ -140,7 +142,7 @@ struct RopeArgs {
   KvView kv;
   RopeView r;
   int rows_per_token;
-  uint32_t rows;  // T * rows_per_token, below 2^31
+  int q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh, c_st, c_sh;  // strides (31 bits)
   int bs_shift;   // log2 of the page size, or -1
   int32_t* dev_err;
 };
@@ -191,16 +193,15 @@ __device__ __forceinline__ int warp_find_seq(const int32_t* cu, int B, int t) {
 }
 
 template <typename T, typename C, int U>  // input type, cache type, lanes a row (head_dim / 16)
-__global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant__ RopeArgs a) {
-  constexpr int D = U * 16, RPW = 32 / U;
+__global__ void __launch_bounds__(64) rope_append_kernel(const __grid_constant__ RopeArgs a) {
+  constexpr int D = U * 16;
   const int lane = threadIdx.x & 31, u = lane % U;
-  const uint32_t row0 = ((blockIdx.x * 256 + threadIdx.x) >> 5) * RPW;
-  if (row0 >= a.rows) return;
-  const uint32_t row = min(row0 + lane / U, a.rows - 1);
-  const bool live = row0 + lane / U < a.rows;
-  const int hq = a.r.hq, hkv = a.kv.hkv;
-  const int tok = row / (uint32_t)a.rows_per_token;
-  const int r = row - (uint32_t)tok * a.rows_per_token;
+  // blockIdx.x is the token, so what is looked up is the same for the block
+  const int tok = blockIdx.x, hq = a.r.hq, hkv = a.kv.hkv;
+  const int row = (blockIdx.y * blockDim.x + threadIdx.x) / U;
+  const bool live = row < a.rows_per_token;
+  if (!__any_sync(0xffffffffu, live)) return;
+  const int r = live ? row : 0;
   // kind 0: query head r, 1: key head, 2: value head
   const int kind = r < hq ? 0 : r < hq + hkv ? 1 : 2;
   const int h = kind == 0 ? r : kind == 1 ? r - hq : r - hq - hkv;
@@ -213,20 +214,13 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
   float x[16];
   {
     const void* base = kind == 0 ? a.r.q : kind == 1 ? a.r.k : a.r.v;
-    const int64_t st = kind == 0 ? a.r.q_st : kind == 1 ? a.r.k_st : a.r.v_st;
-    const int64_t sh = kind == 0 ? a.r.q_sh : kind == 1 ? a.r.k_sh : a.r.v_sh;
-    const int64_t at = tok * st + h * sh;
+    const int st = kind == 0 ? a.q_st : kind == 1 ? a.k_st : a.v_st;
+    const int sh = kind == 0 ? a.q_sh : kind == 1 ? a.k_sh : a.v_sh;
+    const int64_t at = (int64_t)tok * st + (int64_t)h * sh;
     load8<T>(base, at + e0, x);
     load8<T>(base, at + e1, x + 8);
   }
-  // token -> sequence: a warp holds the rows of one token, or a few neighbours
-  int b = -1;
-  const int t_first = __shfl_sync(0xffffffffu, tok, 0);
-  const int t_last = __shfl_sync(0xffffffffu, tok, 31);
-  for (int t = t_first; t <= t_last; ++t) {
-    const int f = warp_find_seq(a.rg.cu, a.rg.B, t);
-    if (t == tok) b = f;
-  }
+  const int b = warp_find_seq(a.rg.cu, a.rg.B, tok);
   const bool rotate = a.r.cos_sin != nullptr && kind != 2;
   int pos = -1, slot = -1, page = 0;
   bool good = live && b >= 0;
@@ -303,7 +297,7 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = 0.f;
     }
-    const int64_t at = tok * a.r.qo_st + h * a.r.qo_sh;
+    const int64_t at = (int64_t)tok * a.qo_st + (int64_t)h * a.qo_sh;
     store8<T>(a.r.q_out, at + e0, x);
     store8<T>(a.r.q_out, at + e1, x + 8);
     return;
@@ -314,19 +308,21 @@ __global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant_
     return;
   }
   void* pool = const_cast<void*>(kind == 1 ? a.kv.k : a.kv.v);
-  const int64_t at = blk * a.kv.sb + (pos - page * a.kv.bs) * a.kv.st + h * a.kv.sh;
+  const int64_t at = blk * a.kv.sb + (int64_t)(pos - page * a.kv.bs) * a.c_st + (int64_t)h * a.c_sh;
   store8<C>(pool, at + e0, x);
   store8<C>(pool, at + e1, x + 8);
 }
 
 template <typename T, typename C>
 cudaError_t launch_ru(const RopeArgs& a, cudaStream_t s) {
-  const int rpw = 32 / (a.kv.d / 16);
-  const int grid = (int)((a.rows + 8 * rpw - 1) / (8 * rpw));
+  const int lanes = a.rows_per_token * (a.kv.d / 16);
+  // two warps a block: 8192 tokens of 48 heads 46 us, 49 with four, 63 with twelve
+  const int parts = (lanes + 63) / 64;
+  const dim3 grid(a.rg.T, parts), block(((lanes + parts - 1) / parts + 31) / 32 * 32);
   switch (a.kv.d) {
-    case 64: rope_append_kernel<T, C, 4><<<grid, 256, 0, s>>>(a); break;
-    case 128: rope_append_kernel<T, C, 8><<<grid, 256, 0, s>>>(a); break;
-    case 256: rope_append_kernel<T, C, 16><<<grid, 256, 0, s>>>(a); break;
+    case 64: rope_append_kernel<T, C, 4><<<grid, block, 0, s>>>(a); break;
+    case 128: rope_append_kernel<T, C, 8><<<grid, block, 0, s>>>(a); break;
+    case 256: rope_append_kernel<T, C, 16><<<grid, block, 0, s>>>(a); break;
     default: return cudaErrorInvalidValue;
   }
   return cudaGetLastError();
@@ -365,7 +361,16 @@ cudaError_t launch_rope_append(const RaggedView& rg, const KvView& kv, const Rop
   a.kv = kv;
   a.r = r;
   a.rows_per_token = r.hq + 2 * kv.hkv;
-  a.rows = (uint32_t)rg.T * (uint32_t)a.rows_per_token;
+  a.q_st = (int)r.q_st;
+  a.q_sh = (int)r.q_sh;
+  a.k_st = (int)r.k_st;
+  a.k_sh = (int)r.k_sh;
+  a.v_st = (int)r.v_st;
+  a.v_sh = (int)r.v_sh;
+  a.qo_st = (int)r.qo_st;
+  a.qo_sh = (int)r.qo_sh;
+  a.c_st = (int)kv.st;
+  a.c_sh = (int)kv.sh;
   a.dev_err = dev_err;
   a.bs_shift = -1;
   for (int i = 0; i < 31; ++i)
