@@ -407,12 +407,13 @@ class Workspace:
         return buf[off:]
 
     def address(self, nbytes: int, device: torch.device, stream: int, tag: str) -> int:
-        """Aligned address of at least nbytes, for calls that pass no tensor on."""
-        key = (device.index, stream, tag)
+        """Aligned address of nbytes, for calls that pass no tensor on. A buffer for each
+        size, kept: a captured graph may hold its address."""
+        key = (device.index, stream, tag, nbytes)
         got = self._bufs.get(key)
-        if got is None or got[2] < nbytes:
+        if got is None:
             buf = torch.zeros(nbytes + 256, dtype=torch.uint8, device=device)
-            got = (buf, buf.data_ptr() + (-buf.data_ptr()) % 256, nbytes)
+            got = (buf, buf.data_ptr() + (-buf.data_ptr()) % 256)
             self._bufs[key] = got
         return got[1]
 

@@ -339,3 +339,26 @@ def test_wait_limit_runs_out_and_recovers(cuda, d):
     P.dev_error.zero_()
     again, _ = run(P)
     assert torch.equal(again, first) and int(P.dev_error.item()) == 0
+
+
+def test_graph_survives_a_larger_call(cuda):
+    """A captured call's workspace stays its own when a later call on the same
+    stream needs a larger one."""
+    P = Problem([40, 1], [900, 7000], 8, 2, 64, seed=24)
+    Q = Problem([40, 1], [900, 7000], 8, 2, 128, seed=25)
+    s, out = torch.cuda.Stream(), torch.empty_like(P.q)
+    with torch.cuda.stream(s):
+        chunk_attention(P.q, P.k_cache, P.v_cache, P.tables, P.lens, P.cu, out=out)
+        s.synchronize()
+        want = out.clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            chunk_attention(P.q, P.k_cache, P.v_cache, P.tables, P.lens, P.cu, out=out)
+        big, _ = run(Q)
+        junk = [torch.full((1 << 22,), float("nan"), device=cuda) for _ in range(16)]
+        out.zero_()
+        g.replay()
+        s.synchronize()
+        assert torch.equal(out, want)
+        assert all(bool(torch.isnan(j).all()) for j in junk)
+        assert torch.equal(run(Q)[0], big)
