@@ -199,9 +199,7 @@ constexpr int kReaders = 14;  // warps that read the records
 // ---------------------------------------------------------------------------
 // items (one warp finds the range, one lane walks it)
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void item_role(const TcArgs& a, TcMeta* m) {
-  const ChunkRange rng =
-      chunk_range(a.rg, a.g, blockIdx.x, gridDim.x, a.min_units, a.dev_err);
+__device__ __forceinline__ void item_role(const TcArgs& a, TcMeta* m, const ChunkRange& rng) {
   if ((threadIdx.x & 31) != 0) return;
   ChunkWalk walk(rng);
   ChunkItem it;
@@ -934,6 +932,9 @@ chunk_tc_kernel(const __grid_constant__ TcArgs a) {
   }
   pdl_launch_dependents();  // the merge's blocks wait for this grid's end on the SMs it leaves
   if (warp == 12) tmem_alloc(smem_u32(&m->tmem), 512);
+  ChunkRange rng = {};
+  if (warp == 13)  // beside the set-up
+    rng = chunk_range(a.rg, a.g, blockIdx.x, gridDim.x, a.min_units, a.dev_err);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -947,7 +948,7 @@ chunk_tc_kernel(const __grid_constant__ TcArgs a) {
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 12 || warp == 14) mma_role<T, D>(a, m, base, tmem, (warp - 12) / 2);
-    if (warp == 13) item_role(a, m);
+    if (warp == 13) item_role(a, m, rng);
     __syncwarp();
   }
   tc_fence_before();
