@@ -352,6 +352,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) chunk_merge_kernel(MergeArgs a) {
   __shared__ float w[kMaxCtas][32];  // weight of each part, then of the output
   __shared__ float red[8][32];
+  pdl_launch_dependents();
   pdl_wait();
   const int cta = blockIdx.y;
   const ChunkMergeDesc ds = a.desc[cta];

@@ -53,6 +53,7 @@
 #include "chunk_plan.cuh"
 #include "cvsa_common.cuh"
 #include "cvsa_internal.h"
+#include "cvsa_launch.cuh"
 #include "tcgen05.cuh"
 
 namespace cvsa {
@@ -928,10 +929,12 @@ chunk_tc_kernel(const __grid_constant__ TcArgs a) {
     for (int i = 0; i < 2; ++i) mbar_init(&m->drain[i], 1);
     m->abort = 0;
     fence_mbar_init();
-    a.desc[blockIdx.x].parts = 0;
   }
   pdl_launch_dependents();  // the merge's blocks wait for this grid's end on the SMs it leaves
   if (warp == 12) tmem_alloc(smem_u32(&m->tmem), 512);
+  // launched early too: nothing global is touched before the work ahead is complete
+  pdl_wait();
+  if (threadIdx.x == 0) a.desc[blockIdx.x].parts = 0;
   ChunkRange rng = {};
   if (warp == 13)  // beside the set-up
     rng = chunk_range(a.rg, a.g, blockIdx.x, gridDim.x, a.min_units, a.dev_err);
@@ -967,8 +970,7 @@ cudaError_t launch_tc(const TcArgs& a, int ctas, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(chunk_tc_kernel<T, D>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  chunk_tc_kernel<T, D><<<ctas, kThreads, kSmem, s>>>(a);
-  return cudaGetLastError();
+  return launch_k(chunk_tc_kernel<T, D>, dim3(ctas), dim3(kThreads), kSmem, s, true, a);
 }
 
 }  // namespace
