@@ -29,7 +29,7 @@
 // registers by unrolled code. The first 64 weights of a row are handed over
 // before the rest is computed, so the second product starts earlier, and the
 // next tile's last 64 scores are formed as soon as this tile's were read for
-// the last time (1024 tokens at 32K keys, 64 heads: 1.44 -> 1.34 ms, 800
+// the last time (1024 tokens at 32K keys, 64 heads: 1.44 -> 1.34 ms in short runs, 800
 // TFLOP/s).
 //
 // Loads: a page holds 16 tokens of one head 2 KB or 4 KB apart, so a tensor
