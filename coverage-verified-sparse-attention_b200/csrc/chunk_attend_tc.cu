@@ -37,12 +37,18 @@
 // straight into the 128-byte-swizzled layout, take any page size and stride.
 // Keys outside the item's range and bad blocks are zero-filled.
 //
-// The running maximum is only raised when it grows by more than 2^8 in the
-// weights' domain (weights up to 256 are exact enough in fp32 sums and in
-// 16 bits), so O is rarely rescaled. Weights are rounded to the 16-bit type for
-// the second product (the tensor core's operand type); their sum is taken
-// before the rounding, in fp32, and the error this adds is of the size of the
-// output's own rounding.
+// The reference maximum is only raised when the row's maximum passes it by more
+// than 2^kRaise in the weights' domain, so O is rarely rescaled. Weights are
+// rounded to the 16-bit type for the second product (the tensor core's operand
+// type); their sum is taken before the rounding, in fp32, so what the rounding
+// loses is missing from the output. In bf16 that is at most 2^-8 of a weight,
+// whatever its size. In f16 a weight below 2^-25 would vanish, and many small weights
+// behind one large one (an early key that takes most of the weight) are most of
+// the output when that key's value is small: 65536 of them at 2^-27 of the largest
+// were lost whole. So f16 weights carry 2^11: at most 2^15 of the type's 65504,
+// 11 bits each down to 2^-25 of the reference and none lost above 2^-36 of it
+// (2^7 with a raise of 2^8 would lose 0.5 % of weights at 2^-25.1). The factor is
+// exact and leaves again in the log-sum-exp and in the partials' maxima.
 //
 // A masked weight is exactly 0, but 0 times a non-finite V is NaN: the loading
 // warps check the V rows of tiles some row sees only in part, and a tile with
@@ -66,7 +72,9 @@ constexpr int kThreads = 512, kTile = 128, kKT = 128;
 // tiles before at most: j or a later one.
 constexpr int kSlots = 16;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kRaise = 8.f;  // log2 growth of the maximum that triggers a rescale
+// log2: growth of the maximum that triggers a rescale, and the weights' factor
+template <typename T> struct Weight { static constexpr float kRaise = 8.f, kUp = 0.f; };
+template <> struct Weight<__half> { static constexpr float kRaise = 4.f, kUp = 11.f; };
 
 template <int D>
 struct Cfg {
@@ -579,6 +587,7 @@ template <typename T, int D>
 __device__ __forceinline__ void softmax_role(const TcArgs& a, TcMeta* m, uint32_t base,
                                              uint32_t tmem, const int g) {
   using C = Cfg<D>;
+  constexpr float kRaise = Weight<T>::kRaise, kUp = Weight<T>::kUp;
   const int r = threadIdx.x & 127, warp = r >> 5;
   const uint32_t lanes = (uint32_t)(warp * 32) << 16;
   const uint32_t ts = tmem + g * kKT + lanes, to = tmem + 2 * kKT + g * D + lanes;
@@ -664,7 +673,7 @@ __device__ __forceinline__ void softmax_role(const TcArgs& a, TcMeta* m, uint32_
           }
         }
         l *= fix;
-        const float ref = mx == neg_inf() ? 0.f : -mx * scale2;
+        const float ref = mx == neg_inf() ? 0.f : fmaf(-mx, scale2, kUp);
         if (odd) {
           // a value of V is not finite and some row does not see it: plain FMAs.
           // The weights go over S in fp32, -1 for an unseen key.
@@ -876,9 +885,10 @@ __device__ __forceinline__ void softmax_role(const TcArgs& a, TcMeta* m, uint32_
         const float m2 = mx * scale2;
         if (whole) {
           if (a.c.lse)
-            a.c.lse[tok * a.c.hq + head] = l == 0.f ? neg_inf() : (m2 + log2f(l)) * kLn2;
+            a.c.lse[tok * a.c.hq + head] =
+                l == 0.f ? neg_inf() : (m2 + log2f(l * exp2f(-kUp))) * kLn2;
         } else {
-          part[rr] = l == 0.f ? neg_inf() : m2;
+          part[rr] = l == 0.f ? neg_inf() : m2 - kUp;
           part[R + rr] = l;
         }
       }

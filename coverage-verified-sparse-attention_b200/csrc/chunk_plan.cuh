@@ -249,7 +249,7 @@ struct ChunkWalk {
 
 // Partial slots. A slot holds m [ROWS], l [ROWS] and o as [D / 4][ROWS]
 // float4 columns (lanes of a warp own neighbouring rows, so both sides are
-// whole lines); m is a maximum in the base-2 domain.
+// whole lines); l and o count in units of 2^m.
 struct ChunkMergeDesc {
   int32_t parts;       // CTAs that share the item (0: none)
   int32_t tok, rows;   // its first packed token; query rows

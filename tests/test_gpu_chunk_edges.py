@@ -1,0 +1,100 @@
+"""chunk_attention and its layer where a call can go wrong without being refused:
+weights far below the largest, rows of refused sequences, calls that are refused
+after a reservation, captured and concurrent calls."""
+
+import pytest
+import torch
+
+from cvsa.kernels.chunk_attend import chunk_attention
+from ragged_ref import E32, U
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+# ---------------------------------------------------------------------------
+# weights far below the largest
+# ---------------------------------------------------------------------------
+
+def sink_call(cuda, dtype, n, gap, new=1, d=64, sink=0, steps=None, seqs=1):
+    """`new` tokens over n keys of page 16 whose scores are 0, but `gap` bits (log2 of the
+    weight) at key `sink`, or as `steps` [n] says. Values: 0 at the sink, else 0.75 to 1.25.
+    All is exact in 16 bits up to the gap's own rounding. `seqs` sequences hold the same
+    pages. Returns (out, lse, want, want_lse) of the last one, which all others have to equal,
+    the definition in 64 bits, and the largest score."""
+    bits = torch.zeros(n, dtype=torch.float64)
+    bits[sink] = gap
+    if steps is not None:
+        bits = steps.double()
+    q = torch.zeros((seqs * new, 1, d), dtype=dtype, device=cuda)
+    q[:, 0, 0] = 1.0
+    k = torch.zeros((n, 1, d), dtype=dtype)
+    k[:, 0, 0] = bits.to(dtype)               # score = k0 * scale, scale = ln 2
+    scale = 0.6931471805599453
+    v = 1.0 + (((torch.arange(n)[:, None] * 7 + torch.arange(d) * 3) % 33) - 16) / 64.0
+    if steps is None:
+        v[sink] = 0.0
+    v = v.to(dtype)
+    page, blocks = 16, -(-n // 16)
+    kc = torch.zeros((blocks * page, 1, d), dtype=dtype)
+    vc = torch.zeros((blocks * page, 1, d), dtype=dtype)
+    kc[:n], vc[:n, 0] = k, v
+    table = torch.arange(blocks, dtype=torch.int32, device=cuda).repeat(seqs, 1)
+    lens = torch.full((seqs,), n, dtype=torch.int32, device=cuda)
+    cu = torch.arange(seqs + 1, dtype=torch.int32, device=cuda) * new
+    lse = torch.empty((seqs * new, 1), device=cuda)
+    out = chunk_attention(q, kc.view(blocks, page, 1, d).to(cuda),
+                          vc.view(blocks, page, 1, d).to(cuda), table, lens, cu, scale=scale,
+                          lse=lse)
+    out, lse = out[:, 0].double().view(seqs, new, d), lse[:, 0].double().view(seqs, new)
+    s = (k[:, 0, 0].double() * scale).to(cuda)
+    v64 = v.double().to(cuda)
+    want = torch.stack([torch.softmax(s[:n - new + i + 1], 0) @ v64[:n - new + i + 1]
+                        for i in range(new)])
+    wl = torch.stack([torch.logsumexp(s[:n - new + i + 1], 0) for i in range(new)])
+    return out, lse, want, wl, float(s.abs().max())
+
+
+def bounds(dtype, want, wl, n, smax, vmax=1.25):
+    """A weight is rounded to the 16-bit type: u relative, and in f16, where the row's largest
+    weight is held at 2^11 or more and the smallest step is 2^-24, at most 2^-36 of the
+    largest a key. The rest as in ragged_ref.attend64 (scores here are one exact product,
+    so the exponential's 2^-21 (1 + |s|) and the sums' (n + 16) 2^-24 are left)."""
+    u = U[dtype]
+    rel = 2 * 2.0 ** -21 * (1 + smax) + (n + 16) * E32 + (u if dtype != F32 else 0.0)
+    low = n * 2.0 ** -36 * vmax if dtype == F16 else 0.0
+    otol = 1.01 * (rel * want.abs() + low) + u * want.abs() * (1 + rel) + 6e-8
+    ltol = 2.0 ** -21 * (1 + smax) + (n + 16) * E32 + 4 * E32 * wl.abs()
+    return otol, ltol
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("gap", [17.5, 24.0, 25.125, 27.0])
+@pytest.mark.parametrize("n,new,seqs", [(131072, 1, 1), (70001, 150, 1), (65536, 1, 300),
+                                        (65536, 150, 150)])
+def test_sink_over_a_long_context(cuda, dtype, gap, n, new, seqs):
+    """One early key takes nearly all of the weight and has value 0: what is left of the
+    output is the many keys whose weights are 2^-gap of the largest. With one sequence the
+    keys are shared by many CTAs, with more than there are CTAs one walks them all."""
+    if dtype == F32 and seqs > 1:
+        n = 8192
+    out, lse, want, wl, smax = sink_call(cuda, dtype, n, gap, new=new, seqs=seqs)
+    otol, ltol = bounds(dtype, want, wl, n, smax)
+    assert bool(((out - want).abs() <= otol).all()), float(((out - want).abs() / otol).max())
+    assert bool(((lse - wl).abs() <= ltol).all()), float(((lse - wl).abs() / ltol).max())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d,new", [(64, 1), (128, 40), (128, 150)])
+@pytest.mark.parametrize("rise", [0.5, 2.0, 3.75, 4.0, 4.25, 7.75, 8.0, 8.25, 11.0, 20.0])
+def test_maximum_rises_by_steps(cuda, dtype, d, new, rise):
+    """Every 128 keys the scores rise by `rise` bits: the largest weight before the reference
+    maximum follows stays finite in f16, and the earlier keys keep their share."""
+    n = 1500
+    steps = torch.arange(n) // 128 * rise
+    out, lse, want, wl, smax = sink_call(cuda, dtype, n, 0.0, new=new, d=d, steps=steps)
+    otol, ltol = bounds(dtype, want, wl, n, smax)
+    assert bool(torch.isfinite(out).all())
+    assert bool(((out - want).abs() <= otol).all()), float(((out - want).abs() / otol).max())
+    assert bool(((lse - wl).abs() <= ltol).all()), float(((lse - wl).abs() / ltol).max())
