@@ -396,6 +396,7 @@ class Workspace:
 
     def __init__(self):
         self._bufs = {}
+        self.lock = threading.Lock()
 
     def get(self, nbytes: int, device: torch.device, tag: str = "") -> torch.Tensor:
         key = (device, torch.cuda.current_stream(device).cuda_stream, tag)
@@ -407,8 +408,10 @@ class Workspace:
         return buf[off:]
 
     def address(self, nbytes: int, device: torch.device, stream: int, tag: str) -> int:
-        """Aligned address of nbytes, for calls that pass no tensor on. A buffer for each
-        size, kept: a captured graph may hold its address."""
+        """Aligned address of nbytes, for calls that pass no tensor on; a buffer for each size,
+        kept. Under `lock`, until the call has enqueued all its kernels: threads share a stream
+        (the default one), and what one call's kernels leave for one another is lost if another
+        call's come between. A captured graph may hold the address."""
         key = (device.index, stream, tag, nbytes)
         got = self._bufs.get(key)
         if got is None:

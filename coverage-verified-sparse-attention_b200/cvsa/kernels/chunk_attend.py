@@ -33,6 +33,8 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     otherwise all of it. lse, if given, is a float32 [T, H_q] tensor to fill
     with the log-sum-exp of each row's scaled scores (for a merge with
     attention over other keys). A row that sees no key gives 0 and -inf.
+
+    Threads may call on one stream.
     """
     dev = _lib.same_device(q, k_cache, v_cache, block_tables, context_lens, cu_tokens, seq_ids,
                            start_positions, out, lse, dev_error)
@@ -62,8 +64,10 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         nbytes = lib.cvsa_chunk_attend_workspace_size(mem.kv, mem.rg, mem.chunk)
         if nbytes:
             _ws_bytes[key] = nbytes
-    ws = _lib.WORKSPACE.address(nbytes, q.device, stream, "chunk") if nbytes else None
-    st = lib.cvsa_chunk_attend(mem.kv, mem.rg, mem.chunk, _lib.ptr(dev_error), ws, nbytes, stream)
+    with _lib.WORKSPACE.lock:
+        ws = _lib.WORKSPACE.address(nbytes, q.device, stream, "chunk") if nbytes else None
+        st = lib.cvsa_chunk_attend(mem.kv, mem.rg, mem.chunk, _lib.ptr(dev_error), ws, nbytes,
+                                   stream)
     if st:
         _lib.check(st, "cvsa_chunk_attend")
     return out

@@ -605,7 +605,10 @@ size_t cvsa_chunk_attend_workspace_size(const cvsa_kv_desc_t* kv, const cvsa_rag
  * and accumulation; with a 16-bit pool of q's dtype and head_dim 64 or 128
  * the products run on the tensor cores with the weights rounded to that
  * dtype. head_dim 64, 128 or 256, up to 64 query heads a KV head, any
- * block_size. The workspace is not read before it is written. */
+ * block_size. The workspace is not read before it is written; one call's
+ * kernels hand partial results over in it, so until they have run no other
+ * call may use it, except one enqueued on the same stream after this one has
+ * returned. */
 int cvsa_chunk_attend(const cvsa_kv_desc_t* kv, const cvsa_ragged_desc_t* rg,
                       const cvsa_chunk_attend_t* args, int32_t* dev_error, void* workspace,
                       size_t workspace_bytes, void* stream);

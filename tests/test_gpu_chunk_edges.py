@@ -2,11 +2,13 @@
 weights far below the largest, rows of refused sequences, calls that are refused
 after a reservation, captured and concurrent calls."""
 
+import threading
+
 import pytest
 import torch
 
 from cvsa.kernels.chunk_attend import chunk_attention
-from ragged_ref import E32, U
+from ragged_ref import E32, U, Problem
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +100,38 @@ def test_maximum_rises_by_steps(cuda, dtype, d, new, rise):
     assert bool(torch.isfinite(out).all())
     assert bool(((out - want).abs() <= otol).all()), float(((out - want).abs() / otol).max())
     assert bool(((lse - wl).abs() <= ltol).all()), float(((lse - wl).abs() / ltol).max())
+
+
+# ---------------------------------------------------------------------------
+# captured and concurrent calls
+# ---------------------------------------------------------------------------
+
+def split_problems(n):
+    """Calls of different batches whose items are all split over CTAs and merged."""
+    return [Problem([1 + 5 * i, 40], [9000 + 700 * i, 3000], 8, 2, 128, seed=40 + i)
+            for i in range(n)]
+
+
+def attend(P, **kw):
+    return chunk_attention(P.q, P.k_cache, P.v_cache, P.tables, P.lens, P.cu,
+                           dev_error=P.dev_error, **kw)
+
+
+def test_threads_on_the_default_stream(cuda):
+    problems = split_problems(3)
+    want = [attend(P) for P in problems]
+    wrong, errors = [], []
+
+    def work(P, w):
+        try:
+            got = [attend(P) for _ in range(40)]
+            wrong.extend(not torch.equal(x, w) for x in got)
+        except Exception as e:  # noqa: BLE001 - shown by the assertion below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(problems, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and len(wrong) == 120 and not any(wrong)

@@ -1,0 +1,110 @@
+"""How the ragged-batch calls reach the library, without a GPU: the library and the device
+queries are stand-ins, the tensors are on the host."""
+
+import threading
+import time
+
+import pytest
+import torch
+
+from cvsa import _lib
+from cvsa.kernels import chunk_attend, rope_append
+
+BYTES = 1000
+
+
+class Library:
+    """Records (call, current device, workspace) and what overlaps."""
+
+    def __init__(self, pause=0.0):
+        self.calls, self.inside, self.overlaps, self.pause = [], {}, 0, pause
+        self.device, self.status = 0, _lib.OK
+        self.guard = threading.Lock()
+
+    def cvsa_chunk_attend_workspace_size(self, kv, rg, args):
+        return BYTES
+
+    def cvsa_chunk_attend(self, kv, rg, args, err, ws, nbytes, stream):
+        with self.guard:
+            self.calls.append(("chunk_attend", self.device, ws))
+            self.overlaps += self.inside.get(ws, 0) > 0
+            self.inside[ws] = self.inside.get(ws, 0) + 1
+        time.sleep(self.pause)
+        with self.guard:
+            self.inside[ws] -= 1
+        return self.status
+
+    def cvsa_rope_append(self, kv, rg, args, err, stream):
+        self.calls.append(("rope_append", self.device, None))
+        return self.status
+
+    def cvsa_paged_reserve(self, *args):
+        self.calls.append(("reserve", self.device, None))
+        return self.status
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    """A library and a CUDA runtime with two devices, of which 0 is current; every tensor
+    passes for one of device `lib.tensors`."""
+    lib = Library()
+    lib.tensors, lib.capturing = 0, False
+
+    class OnDevice:
+        def __init__(self, index):
+            self.index = getattr(index, "index", index)
+
+        def __enter__(self):
+            self.before, lib.device = lib.device, self.index
+
+        def __exit__(self, *exc):
+            lib.device = self.before
+
+    monkeypatch.setattr(_lib, "load", lambda path=None: lib)
+    monkeypatch.setattr(_lib, "same_device", lambda *t: lib.tensors)
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(_lib, "raw_stream", lambda index: 0)
+    monkeypatch.setattr(_lib, "stream_ptr", lambda device: 0)
+    monkeypatch.setattr(_lib, "WORKSPACE", _lib.Workspace())
+    monkeypatch.setattr(chunk_attend, "_ws_bytes", {})
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: lib.device)
+    monkeypatch.setattr(torch.cuda, "device", OnDevice)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: lib.capturing)
+    return lib
+
+
+def tensors():
+    q, k = torch.zeros(3, 4, 64), torch.zeros(3, 2, 64)
+    pool = torch.zeros(4, 16, 2, 64)
+    i = torch.zeros(2, dtype=torch.int32)
+    return q, k, pool, i
+
+
+def attend():
+    q, _, pool, i = tensors()
+    return chunk_attend.chunk_attention(q, pool, pool, i.view(1, 2), i[:1], i)
+
+
+def test_threads_on_one_stream_share_a_workspace_one_call_at_a_time(fake, monkeypatch):
+    """A call's kernels hand partials over in its workspace; first calls of several threads
+    find one buffer, which stays."""
+    fake.pause = 0.01
+    made, real = [], torch.zeros
+
+    def slow_zeros(*a, **kw):
+        t = real(*a, **kw)
+        if kw.get("dtype") is torch.uint8:
+            made.append(t)
+            time.sleep(0.02)
+        return t
+
+    monkeypatch.setattr(_lib.torch, "zeros", slow_zeros)
+    threads = [threading.Thread(target=attend) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(fake.calls) == 4 and len(made) == 1
+    assert len({ws for _, _, ws in fake.calls}) == 1
+    assert fake.overlaps == 0
+    assert all(ws % 256 == 0 for _, _, ws in fake.calls)
