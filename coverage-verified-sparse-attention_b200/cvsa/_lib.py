@@ -411,7 +411,8 @@ class Workspace:
         """Aligned address of nbytes, for calls that pass no tensor on; a buffer for each size,
         kept. Under `lock`, until the call has enqueued all its kernels: threads share a stream
         (the default one), and what one call's kernels leave for one another is lost if another
-        call's come between. A captured graph may hold the address."""
+        call's come between. Not for a call that is captured: every graph would hold the same
+        buffer, and graphs may run at the same time."""
         key = (device.index, stream, tag, nbytes)
         got = self._bufs.get(key)
         if got is None:

@@ -34,7 +34,8 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     with the log-sum-exp of each row's scaled scores (for a merge with
     attention over other keys). A row that sees no key gives 0 and -inf.
 
-    Threads may call on one stream.
+    Threads may call on one stream. A captured call's workspace is memory of its
+    graph's pool: graphs of different pools may be replayed at the same time.
     """
     dev = _lib.same_device(q, k_cache, v_cache, block_tables, context_lens, cu_tokens, seq_ids,
                            start_positions, out, lse, dev_error)
@@ -64,10 +65,16 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         nbytes = lib.cvsa_chunk_attend_workspace_size(mem.kv, mem.rg, mem.chunk)
         if nbytes:
             _ws_bytes[key] = nbytes
-    with _lib.WORKSPACE.lock:
-        ws = _lib.WORKSPACE.address(nbytes, q.device, stream, "chunk") if nbytes else None
-        st = lib.cvsa_chunk_attend(mem.kv, mem.rg, mem.chunk, _lib.ptr(dev_error), ws, nbytes,
-                                   stream)
+    if nbytes and torch.cuda.is_current_stream_capturing():
+        # memory of the graph, like its other tensors
+        buf = torch.empty(nbytes + 256, dtype=torch.uint8, device=q.device)
+        st = lib.cvsa_chunk_attend(mem.kv, mem.rg, mem.chunk, _lib.ptr(dev_error),
+                                   buf.data_ptr() + (-buf.data_ptr()) % 256, nbytes, stream)
+    else:
+        with _lib.WORKSPACE.lock:
+            ws = _lib.WORKSPACE.address(nbytes, q.device, stream, "chunk") if nbytes else None
+            st = lib.cvsa_chunk_attend(mem.kv, mem.rg, mem.chunk, _lib.ptr(dev_error), ws, nbytes,
+                                       stream)
     if st:
         _lib.check(st, "cvsa_chunk_attend")
     return out

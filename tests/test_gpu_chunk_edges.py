@@ -117,6 +117,31 @@ def attend(P, **kw):
                            dev_error=P.dev_error, **kw)
 
 
+def test_graphs_of_one_capture_stream_run_at_the_same_time(cuda):
+    """torch captures every graph on one stream if told of none: their workspaces differ."""
+    problems = split_problems(2)
+    want = [attend(P) for P in problems]
+    outs = [torch.empty_like(P.q) for P in problems]
+    graphs = [torch.cuda.CUDAGraph() for _ in problems]
+    for g, P, out in zip(graphs, problems, outs):
+        with torch.cuda.graph(g):
+            attend(P, out=out)
+    streams = [torch.cuda.Stream() for _ in problems]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                for _ in range(5):
+                    g.replay()
+        torch.cuda.synchronize()
+        for out, w in zip(outs, want):
+            assert torch.equal(out, w)
+    assert all(int(P.dev_error.item()) == 0 for P in problems)
+
+
 def test_threads_on_the_default_stream(cuda):
     problems = split_problems(3)
     want = [attend(P) for P in problems]

@@ -108,3 +108,23 @@ def test_threads_on_one_stream_share_a_workspace_one_call_at_a_time(fake, monkey
     assert len({ws for _, _, ws in fake.calls}) == 1
     assert fake.overlaps == 0
     assert all(ws % 256 == 0 for _, _, ws in fake.calls)
+
+
+def test_a_captured_call_has_a_workspace_of_its_own(fake, monkeypatch):
+    """Not the stream's: graphs captured on one stream may run at the same time."""
+    attend()
+    kept = fake.calls[-1][2]
+    fake.capturing = True
+    bufs, real = [], torch.empty
+
+    def empty(*a, **kw):
+        bufs.append(real(*a, **kw))
+        return bufs[-1]
+
+    monkeypatch.setattr(chunk_attend.torch, "empty", empty)
+    attend()
+    attend()
+    own = [ws for _, _, ws in fake.calls[1:]]
+    assert kept not in own and len(set(own)) == 2
+    for ws, b in zip(own, bufs):
+        assert ws % 256 == 0 and b.data_ptr() <= ws and ws + BYTES <= b.data_ptr() + b.numel()
