@@ -39,6 +39,11 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """
     dev = _lib.same_device(q, k_cache, v_cache, block_tables, context_lens, cu_tokens, seq_ids,
                            start_positions, out, lse, dev_error)
+    if dev != torch.cuda.current_device():  # a launch goes to the current device
+        with torch.cuda.device(dev):
+            return chunk_attention(q, k_cache, v_cache, block_tables, context_lens, cu_tokens,
+                                   causal, window, scale, seq_ids, start_positions, out, lse,
+                                   dev_error)
     q = _lib.token_rows(q, "q")
     T, Hq, D = shape = q.shape
     if k_cache.dim() != 4 or k_cache.shape[3] != D:

@@ -59,6 +59,11 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     """
     dev = _lib.same_device(k, q, v, k_cache, v_cache, block_tables, context_lens, cu_tokens,
                            cos_sin, q_norm, k_norm, seq_ids, start_positions, out, dev_error)
+    if dev != torch.cuda.current_device():  # a launch goes to the current device
+        with torch.cuda.device(dev):
+            return rope_append(q, k, v, k_cache, v_cache, block_tables, context_lens, cu_tokens,
+                               cos_sin, q_norm, k_norm, eps, interleaved, seq_ids,
+                               start_positions, out, dev_error)
     T, Hkv, D = k.shape
     if v.shape != k.shape or k_cache.dim() != 4 or tuple(k_cache.shape[2:]) != (Hkv, D):
         raise ValueError("k and v must be [T, H_kv, D] with the cache's H_kv and D")

@@ -9,6 +9,7 @@ import torch
 
 from cvsa import _lib
 from cvsa.kernels import chunk_attend, rope_append
+from cvsa.runtime.kv_cache import PagedKVCache, SequenceKVManager
 
 BYTES = 1000
 
@@ -62,7 +63,9 @@ def fake(monkeypatch):
 
     monkeypatch.setattr(_lib, "load", lambda path=None: lib)
     monkeypatch.setattr(_lib, "same_device", lambda *t: lib.tensors)
-    monkeypatch.setattr(_lib, "require_cuda", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: torch.device("cuda", lib.tensors))
+    real_empty = torch.empty  # the tensors stay on the host
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: real_empty(*a, **{**kw, "device": "cpu"}))
     monkeypatch.setattr(_lib, "raw_stream", lambda index: 0)
     monkeypatch.setattr(_lib, "stream_ptr", lambda device: 0)
     monkeypatch.setattr(_lib, "WORKSPACE", _lib.Workspace())
@@ -128,3 +131,25 @@ def test_a_captured_call_has_a_workspace_of_its_own(fake, monkeypatch):
     assert kept not in own and len(set(own)) == 2
     for ws, b in zip(own, bufs):
         assert ws % 256 == 0 and b.data_ptr() <= ws and ws + BYTES <= b.data_ptr() + b.numel()
+
+
+def append():
+    q, k, pool, i = tensors()
+    return rope_append.rope_append(q, k, k, pool, pool, i.view(1, 2), i[:1], i)
+
+
+def reserve():
+    manager = SequenceKVManager(PagedKVCache(4, 16, 2, 64, device="cpu"), 1, 64)
+    return manager.reserve(torch.tensor([0, 3]))
+
+
+@pytest.mark.parametrize("call,name", [(attend, "chunk_attend"), (append, "rope_append"),
+                                       (reserve, "reserve")])
+def test_launches_go_to_the_tensors_device(fake, call, name):
+    """The default stream's handle is the same on every device, so the tensors' device has to
+    be current for the launch, and the caller's is current again afterwards."""
+    for device in (0, 1):
+        fake.tensors = device
+        call()
+        assert fake.calls[-1][:2] == (name, device)
+        assert fake.device == 0
