@@ -56,9 +56,14 @@ __device__ __forceinline__ SeqInfo chunk_seq(const RaggedView& rg, int bs, int b
   const int start = rg.starts ? rg.starts[b] : 0;
   q.n = end - q.tok0;
   q.start = rg.starts ? start : q.ctx - q.n;
-  if (q.tok0 < 0 || end > rg.T || end < q.tok0 || !row_ok) {
+  if (q.tok0 < 0 || end > rg.T || end < q.tok0) {  // whose tokens these are is not known
     set_dev_error(dev_err, CVSA_DEV_ERR_RAGGED);
     q.n = q.slot = q.start = q.ctx = 0;
+    return q;
+  }
+  if (!row_ok) {  // its rows see no key
+    set_dev_error(dev_err, CVSA_DEV_ERR_RAGGED);
+    q.slot = q.start = q.ctx = 0;
     return q;
   }
   if (q.ctx < 0 || q.ctx > (int64_t)rg.W * bs) {

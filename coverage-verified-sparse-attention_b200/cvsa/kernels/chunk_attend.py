@@ -32,7 +32,9 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     sequence up to itself, of which the last `window` keys if window > 0;
     otherwise all of it. lse, if given, is a float32 [T, H_q] tensor to fill
     with the log-sum-exp of each row's scaled scores (for a merge with
-    attention over other keys). A row that sees no key gives 0 and -inf.
+    attention over other keys). A row that sees no key gives 0 and -inf, as
+    does a sequence that was refused or whose table row is out of range. Rows no sequence
+    owns (padding, offsets out of range) are not written.
 
     Threads may call on one stream. A captured call's workspace is memory of its
     graph's pool: graphs of different pools may be replayed at the same time.

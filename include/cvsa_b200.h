@@ -523,7 +523,9 @@ int cvsa_paged_gather(const cvsa_kv_desc_t* kv, const int32_t* block_table_row,
  *   cvsa_paged_reserve -> cvsa_rope_append -> cvsa_chunk_attend.
  * Entries out of range never trap: they set CVSA_DEV_ERR_RAGGED or
  * CVSA_DEV_ERR_BLOCK_RANGE in *dev_error (nullable) and the token, row or key
- * is skipped. */
+ * is skipped. Output rows of a sequence whose table row is out of range are 0;
+ * output rows of one whose offsets are (negative, decreasing, past num_tokens)
+ * are not written. */
 typedef struct cvsa_ragged_desc {
   const int32_t* cu_tokens;       /* [batch + 1], non-decreasing, from 0 */
   const int32_t* seq_ids;         /* [batch] rows of the tables, or NULL: row b */

@@ -7,6 +7,7 @@ import threading
 import pytest
 import torch
 
+from cvsa import _lib
 from cvsa.kernels.chunk_attend import chunk_attention
 from ragged_ref import E32, U, Problem
 
@@ -160,3 +161,33 @@ def test_threads_on_the_default_stream(cuda):
     for t in threads:
         t.join()
     assert not errors and len(wrong) == 120 and not any(wrong)
+
+
+# ---------------------------------------------------------------------------
+# refused sequences
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (F16, 128), (BF16, 256), (F32, 64), (F32, 128)])
+@pytest.mark.parametrize("bad", [-1, 5, 1 << 30])
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_of_a_bad_table_row_are_zero(cuda, dtype, d, bad, causal):
+    """The rows of a sequence whose table row is out of range belong to the caller's output:
+    0 and -inf, not what the memory held. The other sequences are as if alone."""
+    P = Problem([4, 150, 5, 1], [60, 190, 33, 700], 4, 2, d, dtype=dtype, seed=19)
+    good = attend(P, causal=causal)
+    for b in range(4):
+        ids = torch.arange(4, dtype=torch.int32, device=cuda)
+        ids[b] = bad
+        out = torch.full_like(P.q, float("nan"))
+        lse = torch.full((P.T, P.hq), float("nan"), device=cuda)
+        attend(P, causal=causal, seq_ids=ids, out=out, lse=lse)
+        lo, hi = P.cu[b].item(), P.cu[b + 1].item()
+        assert bool((out[lo:hi] == 0).all()) and bool((lse[lo:hi] == float("-inf")).all())
+        rest = torch.cat([torch.arange(lo), torch.arange(hi, P.T)]).to(cuda)
+        # a refused sequence moves the cut of the work: equal up to the order of the sums
+        far = 2 * U[dtype] if dtype != F32 else 1e-5
+        assert float((out[rest].float() - good[rest].float()).abs().max()) <= far * float(
+            good.float().abs().max())
+        assert bool(torch.isfinite(lse[rest]).all())
+        assert int(P.dev_error.item()) == _lib.DEV_ERR_RAGGED
+        P.dev_error.zero_()
