@@ -174,6 +174,89 @@ int check_chunk(const cvsa_chunk_attend_t* a, const KvView& kv, const RaggedView
   return CVSA_OK;
 }
 
+int check_rope(const cvsa_rope_append_t* args, const KvView& kv, const RaggedView& rg,
+               RopeView* out) {
+  if (!args) return fail(CVSA_ERR_INVALID, "arguments are NULL");
+  if (!valid_dtype(args->dtype)) return fail(CVSA_ERR_INVALID, "dtype %d unknown", args->dtype);
+  const int hq = args->num_q_heads;
+  if (hq < 0 || (args->q && hq == 0) || (!args->q && hq != 0 && rg.T > 0))
+    return fail(CVSA_ERR_INVALID, "num_q_heads=%d does not fit q", args->num_q_heads);
+  if (rg.T > 0 && (!args->k || !args->v || (hq && !args->q_out)))
+    return fail(CVSA_ERR_INVALID, "k/v/q_out is NULL");
+  if ((args->q_norm || args->k_norm) && args->norm_dtype != args->dtype &&
+      args->norm_dtype != CVSA_DTYPE_F32)
+    return fail(CVSA_ERR_INVALID, "norm weights must have the tokens' dtype or float32");
+  if ((args->q_norm || args->k_norm) && !(args->eps >= 0.f))
+    return fail(CVSA_ERR_INVALID, "eps must be >= 0");
+  if (!rope_append_supported(kv))
+    return fail(CVSA_ERR_UNSUPPORTED, "rope_append built for head_dim 64/128/256");
+  if (args->cos_sin && (args->rot_dim <= 0 || args->rot_dim > kv.d || args->rot_dim % 32 ||
+                        args->max_positions <= 0))
+    return fail(CVSA_ERR_INVALID,
+                "rot_dim=%d must be a multiple of 32 up to head_dim, max_positions=%d positive",
+                args->rot_dim, args->max_positions);
+  const int eb = dtype_bytes(args->dtype);
+  auto aligned = [&](const void* p, int64_t st_tok, int64_t st_head) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (st_tok * eb) % 16 == 0 &&
+           (st_head * eb) % 16 == 0;
+  };
+  if (!aligned(args->k, args->k_stride_token, args->k_stride_head) ||
+      !aligned(args->v, args->v_stride_token, args->v_stride_head) ||
+      (hq && (!aligned(args->q, args->q_stride_token, args->q_stride_head) ||
+              !aligned(args->q_out, args->q_out_stride_token, args->q_out_stride_head))) ||
+      (reinterpret_cast<uintptr_t>(args->cos_sin) | reinterpret_cast<uintptr_t>(args->q_norm) |
+       reinterpret_cast<uintptr_t>(args->k_norm)) % 16)
+    return fail(CVSA_ERR_INVALID, "q/k/v/q_out rows, cos_sin and weights must be 16-byte aligned");
+  if ((int64_t)rg.T * (hq + 2 * (int64_t)kv.hkv) >= (int64_t(1) << 31))
+    return fail(CVSA_ERR_UNSUPPORTED, "num_tokens * heads above 2^31");
+  for (int64_t st : {args->k_stride_token, args->k_stride_head, args->v_stride_token,
+                     args->v_stride_head, kv.st, kv.sh, hq ? args->q_stride_token : 0,
+                     hq ? args->q_stride_head : 0, hq ? args->q_out_stride_token : 0,
+                     hq ? args->q_out_stride_head : 0})
+    if (st >= (int64_t(1) << 31) || st < -(int64_t(1) << 31))
+      return fail(CVSA_ERR_UNSUPPORTED, "token and head strides must fit 32 bits");
+  out->q = args->q;
+  out->k = args->k;
+  out->v = args->v;
+  out->q_out = args->q_out;
+  out->dtype = args->dtype;
+  out->hq = hq;
+  out->q_st = args->q_stride_token;
+  out->q_sh = args->q_stride_head;
+  out->k_st = args->k_stride_token;
+  out->k_sh = args->k_stride_head;
+  out->v_st = args->v_stride_token;
+  out->v_sh = args->v_stride_head;
+  out->qo_st = args->q_out_stride_token;
+  out->qo_sh = args->q_out_stride_head;
+  out->cos_sin = args->cos_sin;
+  out->max_positions = args->max_positions;
+  out->rot = args->cos_sin ? args->rot_dim : 0;
+  out->interleaved = args->interleaved;
+  out->q_norm = args->q_norm;
+  out->k_norm = args->k_norm;
+  out->norm_f32 = args->norm_dtype == CVSA_DTYPE_F32;
+  out->eps = args->eps;
+  return CVSA_OK;
+}
+
+// Descriptors and arguments of a ragged-batch call.
+int check_rope_call(const cvsa_kv_desc_t* kvd, const cvsa_ragged_desc_t* rgd,
+                    const cvsa_rope_append_t* args, KvView* kv, RaggedView* rg, RopeView* r) {
+  int st = check_kv(kvd, kv);
+  if (st) return st;
+  st = check_ragged(rgd, rg);
+  return st ? st : check_rope(args, *kv, *rg, r);
+}
+
+int check_chunk_call(const cvsa_kv_desc_t* kvd, const cvsa_ragged_desc_t* rgd,
+                     const cvsa_chunk_attend_t* args, KvView* kv, RaggedView* rg, ChunkView* c) {
+  int st = check_kv(kvd, kv);
+  if (st) return st;
+  st = check_ragged(rgd, rg);
+  return st ? st : check_chunk(args, *kv, *rg, c);
+}
+
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // Largest page count the select kernel can hold in shared memory.
@@ -1071,79 +1154,32 @@ int cvsa_paged_reserve(int32_t block_size, const int32_t* cu_tokens, const int32
                      "reserve launch");
 }
 
+int cvsa_rope_append_check(const cvsa_kv_desc_t* kvd, const cvsa_ragged_desc_t* rgd,
+                           const cvsa_rope_append_t* args) {
+  KvView kv;
+  RaggedView rg;
+  RopeView r;
+  return check_rope_call(kvd, rgd, args, &kv, &rg, &r);
+}
+
 int cvsa_rope_append(const cvsa_kv_desc_t* kvd, const cvsa_ragged_desc_t* rgd,
                      const cvsa_rope_append_t* args, int32_t* dev_error, void* stream) {
   KvView kv;
   RaggedView rg;
-  int st = check_kv(kvd, &kv);
-  if (st) return st;
-  st = check_ragged(rgd, &rg);
-  if (st) return st;
-  if (!args) return fail(CVSA_ERR_INVALID, "arguments are NULL");
-  if (!valid_dtype(args->dtype)) return fail(CVSA_ERR_INVALID, "dtype %d unknown", args->dtype);
-  const int hq = args->num_q_heads;
-  if (hq < 0 || (args->q && hq == 0) || (!args->q && hq != 0 && rg.T > 0))
-    return fail(CVSA_ERR_INVALID, "num_q_heads=%d does not fit q", args->num_q_heads);
-  if (rg.T > 0 && (!args->k || !args->v || (hq && !args->q_out)))
-    return fail(CVSA_ERR_INVALID, "k/v/q_out is NULL");
-  if ((args->q_norm || args->k_norm) && args->norm_dtype != args->dtype &&
-      args->norm_dtype != CVSA_DTYPE_F32)
-    return fail(CVSA_ERR_INVALID, "norm weights must have the tokens' dtype or float32");
-  if ((args->q_norm || args->k_norm) && !(args->eps >= 0.f))
-    return fail(CVSA_ERR_INVALID, "eps must be >= 0");
-  if (!rope_append_supported(kv))
-    return fail(CVSA_ERR_UNSUPPORTED, "rope_append built for head_dim 64/128/256");
-  if (args->cos_sin && (args->rot_dim <= 0 || args->rot_dim > kv.d || args->rot_dim % 32 ||
-                        args->max_positions <= 0))
-    return fail(CVSA_ERR_INVALID,
-                "rot_dim=%d must be a multiple of 32 up to head_dim, max_positions=%d positive",
-                args->rot_dim, args->max_positions);
-  const int eb = dtype_bytes(args->dtype);
-  auto aligned = [&](const void* p, int64_t st_tok, int64_t st_head) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (st_tok * eb) % 16 == 0 &&
-           (st_head * eb) % 16 == 0;
-  };
-  if (!aligned(args->k, args->k_stride_token, args->k_stride_head) ||
-      !aligned(args->v, args->v_stride_token, args->v_stride_head) ||
-      (hq && (!aligned(args->q, args->q_stride_token, args->q_stride_head) ||
-              !aligned(args->q_out, args->q_out_stride_token, args->q_out_stride_head))) ||
-      (reinterpret_cast<uintptr_t>(args->cos_sin) | reinterpret_cast<uintptr_t>(args->q_norm) |
-       reinterpret_cast<uintptr_t>(args->k_norm)) % 16)
-    return fail(CVSA_ERR_INVALID, "q/k/v/q_out rows, cos_sin and weights must be 16-byte aligned");
-  if ((int64_t)rg.T * (hq + 2 * (int64_t)kv.hkv) >= (int64_t(1) << 31))
-    return fail(CVSA_ERR_UNSUPPORTED, "num_tokens * heads above 2^31");
-  for (int64_t st : {args->k_stride_token, args->k_stride_head, args->v_stride_token,
-                     args->v_stride_head, kv.st, kv.sh, hq ? args->q_stride_token : 0,
-                     hq ? args->q_stride_head : 0, hq ? args->q_out_stride_token : 0,
-                     hq ? args->q_out_stride_head : 0})
-    if (st >= (int64_t(1) << 31) || st < -(int64_t(1) << 31))
-      return fail(CVSA_ERR_UNSUPPORTED, "token and head strides must fit 32 bits");
-  if (rg.B == 0 || rg.T == 0) return CVSA_OK;
   RopeView r;
-  r.q = args->q;
-  r.k = args->k;
-  r.v = args->v;
-  r.q_out = args->q_out;
-  r.dtype = args->dtype;
-  r.hq = hq;
-  r.q_st = args->q_stride_token;
-  r.q_sh = args->q_stride_head;
-  r.k_st = args->k_stride_token;
-  r.k_sh = args->k_stride_head;
-  r.v_st = args->v_stride_token;
-  r.v_sh = args->v_stride_head;
-  r.qo_st = args->q_out_stride_token;
-  r.qo_sh = args->q_out_stride_head;
-  r.cos_sin = args->cos_sin;
-  r.max_positions = args->max_positions;
-  r.rot = args->cos_sin ? args->rot_dim : 0;
-  r.interleaved = args->interleaved;
-  r.q_norm = args->q_norm;
-  r.k_norm = args->k_norm;
-  r.norm_f32 = args->norm_dtype == CVSA_DTYPE_F32;
-  r.eps = args->eps;
+  const int st = check_rope_call(kvd, rgd, args, &kv, &rg, &r);
+  if (st) return st;
+  if (rg.B == 0 || rg.T == 0) return CVSA_OK;
   return cuda_status(launch_rope_append(rg, kv, r, dev_error, (cudaStream_t)stream),
                      "rope_append launch");
+}
+
+int cvsa_chunk_attend_check(const cvsa_kv_desc_t* kvd, const cvsa_ragged_desc_t* rgd,
+                            const cvsa_chunk_attend_t* args) {
+  KvView kv;
+  RaggedView rg;
+  ChunkView c;
+  return check_chunk_call(kvd, rgd, args, &kv, &rg, &c);
 }
 
 size_t cvsa_chunk_attend_workspace_size(const cvsa_kv_desc_t* kvd, const cvsa_ragged_desc_t* rgd,
@@ -1151,7 +1187,7 @@ size_t cvsa_chunk_attend_workspace_size(const cvsa_kv_desc_t* kvd, const cvsa_ra
   KvView kv;
   RaggedView rg;
   ChunkView c;
-  if (check_kv(kvd, &kv) || check_ragged(rgd, &rg) || check_chunk(args, kv, rg, &c)) return 0;
+  if (check_chunk_call(kvd, rgd, args, &kv, &rg, &c)) return 0;
   return chunk_attend_workspace_bytes(kv, rg, c);
 }
 
@@ -1161,11 +1197,7 @@ int cvsa_chunk_attend(const cvsa_kv_desc_t* kvd, const cvsa_ragged_desc_t* rgd,
   KvView kv;
   RaggedView rg;
   ChunkView c;
-  int st = check_kv(kvd, &kv);
-  if (st) return st;
-  st = check_ragged(rgd, &rg);
-  if (st) return st;
-  st = check_chunk(args, kv, rg, &c);
+  const int st = check_chunk_call(kvd, rgd, args, &kv, &rg, &c);
   if (st) return st;
   if (rg.B == 0 || rg.T == 0) return CVSA_OK;
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 ||

@@ -183,6 +183,10 @@ _SIGS = {
                            ctypes.c_int),
     "cvsa_rope_append": ([ctypes.POINTER(KvDesc), ctypes.POINTER(RaggedDesc),
                           ctypes.POINTER(RopeAppend), _P, _P], ctypes.c_int),
+    "cvsa_rope_append_check": ([ctypes.POINTER(KvDesc), ctypes.POINTER(RaggedDesc),
+                                ctypes.POINTER(RopeAppend)], ctypes.c_int),
+    "cvsa_chunk_attend_check": ([ctypes.POINTER(KvDesc), ctypes.POINTER(RaggedDesc),
+                                 ctypes.POINTER(ChunkAttend)], ctypes.c_int),
     "cvsa_chunk_attend_workspace_size": ([ctypes.POINTER(KvDesc), ctypes.POINTER(RaggedDesc),
                                           ctypes.POINTER(ChunkAttend)], ctypes.c_size_t),
     "cvsa_chunk_attend": ([ctypes.POINTER(KvDesc), ctypes.POINTER(RaggedDesc),

@@ -23,7 +23,8 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     scale: Optional[float] = None, seq_ids: Optional[torch.Tensor] = None,
                     start_positions: Optional[torch.Tensor] = None,
                     out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
-                    dev_error: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    dev_error: Optional[torch.Tensor] = None, *,
+                    check_only: bool = False) -> torch.Tensor:
     """softmax(scale q K^T) V per new token and query head, [T, H_q, D] in q's dtype.
 
     q [T, H_q, D]; the pools, tables [num_seqs, max_pages] and lengths
@@ -35,6 +36,8 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     attention over other keys). A row that sees no key gives 0 and -inf, as
     does a sequence that was refused or whose table row is out of range. Rows no sequence
     owns (padding, offsets out of range) are not written.
+    check_only raises what the call would be refused with and returns the output
+    unfilled, without a launch.
 
     Threads may call on one stream. A captured call's workspace is memory of its
     graph's pool: graphs of different pools may be replayed at the same time.
@@ -45,7 +48,7 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         with torch.cuda.device(dev):
             return chunk_attention(q, k_cache, v_cache, block_tables, context_lens, cu_tokens,
                                    causal, window, scale, seq_ids, start_positions, out, lse,
-                                   dev_error)
+                                   dev_error, check_only=check_only)
     q = _lib.token_rows(q, "q")
     T, Hq, D = shape = q.shape
     if k_cache.dim() != 4 or k_cache.shape[3] != D:
@@ -65,6 +68,9 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                    _lib.dtype_code(q.dtype), Hq, qs[0], qs[1], os_[0], os_[1],
                    D ** -0.5 if scale is None else scale, causal, window)
     lib, stream = _lib.load(), _lib.raw_stream(dev)
+    if check_only:
+        _lib.check(lib.cvsa_chunk_attend_check(mem.kv, mem.rg, mem.chunk), "cvsa_chunk_attend")
+        return out
     # the size depends on the head layout alone; 0 for what the call will refuse
     key = (dev, D, q.dtype, k_cache.dtype)
     nbytes = _ws_bytes.get(key)

@@ -10,7 +10,7 @@ norms and rotation to the model library and appends token by token
 (cvsa/runtime/kv_cache.py:133-150).
 """
 
-from typing import Optional
+from typing import Callable, Optional
 
 import torch
 
@@ -47,7 +47,8 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
                 interleaved: bool = False, seq_ids: Optional[torch.Tensor] = None,
                 start_positions: Optional[torch.Tensor] = None,
                 out: Optional[torch.Tensor] = None,
-                dev_error: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+                dev_error: Optional[torch.Tensor] = None, *,
+                _reserve: Optional[Callable[[], None]] = None) -> Optional[torch.Tensor]:
     """Normed and rotated queries [T, H_q, D] (None without q); keys and values are appended.
 
     q [T, H_q, D], k and v [T, H_kv, D] in one dtype (the pool may have
@@ -57,13 +58,15 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     instead of the halves of the rotated part. start_positions and seq_ids as
     returned by / given to `reserve`. `out` may be q itself.
     """
+    # _reserve, if given, makes the reservation when nothing can refuse the call any more
+    # (it may not call an operator that packs its arguments into this thread's memory)
     dev = _lib.same_device(k, q, v, k_cache, v_cache, block_tables, context_lens, cu_tokens,
                            cos_sin, q_norm, k_norm, seq_ids, start_positions, out, dev_error)
     if dev != torch.cuda.current_device():  # a launch goes to the current device
         with torch.cuda.device(dev):
             return rope_append(q, k, v, k_cache, v_cache, block_tables, context_lens, cu_tokens,
                                cos_sin, q_norm, k_norm, eps, interleaved, seq_ids,
-                               start_positions, out, dev_error)
+                               start_positions, out, dev_error, _reserve=_reserve)
     T, Hkv, D = k.shape
     if v.shape != k.shape or k_cache.dim() != 4 or tuple(k_cache.shape[2:]) != (Hkv, D):
         raise ValueError("k and v must be [T, H_kv, D] with the cache's H_kv and D")
@@ -105,8 +108,12 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
                   0 if cos_sin is None else cos_sin.data_ptr(), pos, rot, interleaved,
                   _lib.dtype_code(ndt), 0 if q_norm is None else q_norm.data_ptr(),
                   0 if k_norm is None else k_norm.data_ptr(), eps)
-    st = _lib.load().cvsa_rope_append(mem.kv, mem.rg, mem.rope, _lib.ptr(dev_error),
-                                      _lib.raw_stream(dev))
+    lib = _lib.load()
+    if _reserve is not None:
+        _lib.check(lib.cvsa_rope_append_check(mem.kv, mem.rg, mem.rope), "cvsa_rope_append")
+        _reserve()
+    st = lib.cvsa_rope_append(mem.kv, mem.rg, mem.rope, _lib.ptr(dev_error),
+                              _lib.raw_stream(dev))
     if st:
         _lib.check(st, "cvsa_rope_append")
     return out

@@ -34,29 +34,40 @@ class ChunkedAttention:
         self.window = window
         self.scale = scale
 
-    def append(self, manager, q, k, v, cu_tokens, seq_ids=None):
+    def append(self, manager, q, k, v, cu_tokens, seq_ids=None, out=None):
         """Reserve pages, write the keys and values, return (rotated queries, start positions).
 
-        For a decode step: the queries go to the sparse backend."""
+        For a decode step: the queries go to the sparse backend. A call that is
+        refused (ValueError, RuntimeError) has reserved nothing."""
         c = manager.cache
-        starts = manager.reserve(cu_tokens, seq_ids)
+        cu, ids = _int32(cu_tokens), _int32(seq_ids)
+        starts = torch.empty((max(cu.numel() - 1, 0),), dtype=torch.int32, device=cu.device)
         q = rope_append(q, k, v, c.k_cache, c.v_cache, manager.block_tables,
-                        manager.context_lens, cu_tokens, cos_sin=self.cos_sin,
+                        manager.context_lens, cu, cos_sin=self.cos_sin,
                         q_norm=self.q_norm, k_norm=self.k_norm, eps=self.eps,
-                        interleaved=self.interleaved, seq_ids=seq_ids, start_positions=starts,
-                        dev_error=c.dev_error)
+                        interleaved=self.interleaved, seq_ids=ids, start_positions=starts,
+                        out=out, dev_error=c.dev_error,
+                        _reserve=lambda: manager._reserve(cu, ids, starts))
         return q, starts
 
     def __call__(self, manager, q, k, v, cu_tokens, seq_ids=None):
         """q [T, H_q, D], k and v [T, H_kv, D] of the packed new tokens -> [T, H_q, D].
 
         manager is the layer's `SequenceKVManager`; sequence seq_ids[b] (default
-        b) owns tokens cu_tokens[b]..cu_tokens[b + 1] (int32, on the device).
-        Nothing synchronises: a sequence that does not fit yields zeros and
-        `manager.cache.check()` raises."""
+        b) owns tokens cu_tokens[b]..cu_tokens[b + 1] (on the device). Nothing
+        synchronises: a sequence that does not fit yields zeros and
+        `manager.cache.check()` raises. A call that is refused (ValueError,
+        RuntimeError) has appended nothing."""
         c = manager.cache
-        q, starts = self.append(manager, q, k, v, cu_tokens, seq_ids)
-        return chunk_attention(q, c.k_cache, c.v_cache, manager.block_tables,
-                               manager.context_lens, cu_tokens, window=self.window,
-                               scale=self.scale, seq_ids=seq_ids, start_positions=starts,
-                               dev_error=c.dev_error)
+        cu, ids = _int32(cu_tokens), _int32(seq_ids)
+        rotated = q.new_empty(q.shape)
+        form = dict(window=self.window, scale=self.scale, seq_ids=ids, dev_error=c.dev_error)
+        out = chunk_attention(rotated, c.k_cache, c.v_cache, manager.block_tables,
+                              manager.context_lens, cu, check_only=True, **form)
+        _, starts = self.append(manager, q, k, v, cu, ids, out=rotated)
+        return chunk_attention(rotated, c.k_cache, c.v_cache, manager.block_tables,
+                               manager.context_lens, cu, start_positions=starts, out=out, **form)
+
+
+def _int32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if t is None else t.to(torch.int32).contiguous()

@@ -178,14 +178,21 @@ class SequenceKVManager:
         elif n > self.batch_size:
             raise ValueError(f"{n} sequences but {self.batch_size} table rows")
         starts = torch.empty((n,), dtype=torch.int32, device=dev)
+        self._reserve(cu, seq_ids, starts)
+        return starts
+
+    def _reserve(self, cu, seq_ids, starts):
+        """`reserve` of checked int32 arrays."""
+        c = self.cache
+        dev = _lib.require_cuda(cu, c.k_cache)
         with torch.cuda.device(dev):  # a launch goes to the current device
             _lib.check(_lib.load().cvsa_paged_reserve(
-                self.block_size, cu.data_ptr(), _lib.ptr(seq_ids), n, self.batch_size,
-                self.block_tables.data_ptr(), self.max_pages, self.context_lens.data_ptr(),
-                self.pages_allocated.data_ptr(), c.free_list.data_ptr(), c.free_list.numel(),
-                c.free_head.data_ptr(), starts.data_ptr(), c.dev_error.data_ptr(),
-                _lib.stream_ptr(dev)), "cvsa_paged_reserve")
-        return starts
+                self.block_size, cu.data_ptr(), _lib.ptr(seq_ids), starts.numel(),
+                self.batch_size, self.block_tables.data_ptr(), self.max_pages,
+                self.context_lens.data_ptr(), self.pages_allocated.data_ptr(),
+                c.free_list.data_ptr(), c.free_list.numel(), c.free_head.data_ptr(),
+                starts.data_ptr(), c.dev_error.data_ptr(), _lib.stream_ptr(dev)),
+                "cvsa_paged_reserve")
 
     def _append(self, k, v, ids):
         c = self.cache

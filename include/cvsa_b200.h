@@ -584,6 +584,11 @@ typedef struct cvsa_rope_append {
 int cvsa_rope_append(const cvsa_kv_desc_t* kv, const cvsa_ragged_desc_t* rg,
                      const cvsa_rope_append_t* args, int32_t* dev_error, void* stream);
 
+/* The status cvsa_rope_append would refuse these arguments with (or CVSA_OK);
+ * nothing is launched. For a caller that reserves pages first. */
+int cvsa_rope_append_check(const cvsa_kv_desc_t* kv, const cvsa_ragged_desc_t* rg,
+                           const cvsa_rope_append_t* args);
+
 typedef struct cvsa_chunk_attend {
   const void* q;          /* [num_tokens, num_q_heads, head_dim] */
   void* out;              /* the same shape and dtype */
@@ -596,6 +601,10 @@ typedef struct cvsa_chunk_attend {
   int32_t causal;         /* 1: a token sees its sequence up to itself; 0: all of it */
   int32_t window;         /* causal only: keys a token sees, itself included; 0: no limit */
 } cvsa_chunk_attend_t;
+
+/* As cvsa_rope_append_check; the workspace is not part of it. */
+int cvsa_chunk_attend_check(const cvsa_kv_desc_t* kv, const cvsa_ragged_desc_t* rg,
+                            const cvsa_chunk_attend_t* args);
 
 size_t cvsa_chunk_attend_workspace_size(const cvsa_kv_desc_t* kv, const cvsa_ragged_desc_t* rg,
                                         const cvsa_chunk_attend_t* args);

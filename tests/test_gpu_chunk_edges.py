@@ -9,6 +9,9 @@ import torch
 
 from cvsa import _lib
 from cvsa.kernels.chunk_attend import chunk_attention
+from cvsa.kernels.rope_append import rope_table
+from cvsa.runtime.chunked import ChunkedAttention
+from cvsa.runtime.kv_cache import PagedKVCache, SequenceKVManager
 from ragged_ref import E32, U, Problem
 
 pytestmark = pytest.mark.gpu
@@ -191,3 +194,97 @@ def test_rows_of_a_bad_table_row_are_zero(cuda, dtype, d, bad, causal):
         assert bool(torch.isfinite(lse[rest]).all())
         assert int(P.dev_error.item()) == _lib.DEV_ERR_RAGGED
         P.dev_error.zero_()
+
+
+# ---------------------------------------------------------------------------
+# refused calls of a layer
+# ---------------------------------------------------------------------------
+
+def layer_state(manager):
+    c = manager.cache
+    return [t.clone() for t in (manager.context_lens, manager.pages_allocated,
+                                manager.block_tables, c.free_head, c.k_cache, c.v_cache)]
+
+
+def layer_call(cuda, T=21, hq=8, hkv=2, d=128, dtype=BF16):
+    q = torch.randn((T, hq, d), device=cuda).to(dtype)
+    k, v = (torch.randn((T, hkv, d), device=cuda).to(dtype) for _ in range(2))
+    return q, k, v
+
+
+REFUSED = {  # what is wrong: (layer's settings, changes of the call)
+    "dtype of k": ({}, dict(k=lambda q, k, v: k.float())),
+    "no such dtype": ({}, dict(q=lambda q, k, v: q.double(), k=lambda q, k, v: k.double(),
+                               v=lambda q, k, v: v.double())),
+    "tokens of q": ({}, dict(q=lambda q, k, v: q[:-1])),
+    "heads of k": ({}, dict(k=lambda q, k, v: k[:, :1], v=lambda q, k, v: v[:, :1])),
+    "shape of v": ({}, dict(v=lambda q, k, v: v[:, :, :64])),
+    "dimensions": ({}, dict(q=lambda q, k, v: q.flatten(1))),
+    "offsets' shape": ({}, dict(cu=lambda cu: cu[None])),
+    "table rows' shape": ({}, dict(ids=[0])),
+    "more sequences than rows": ({}, dict(cu=lambda cu: torch.cat([cu, cu[-1:].expand(3)]))),
+    "norm's width": (dict(q_norm=64, k_norm=64), {}),
+    "norm's dtype": (dict(k_norm=F16), {}),
+    "eps": (dict(k_norm=BF16, eps=-1.0), {}),
+    "rotated width": (dict(table=48), {}),
+    "table's dtype": (dict(table=F16), {}),
+}
+REFUSED_ATTENTION = {  # by the attention that follows the append
+    "scale": (dict(scale=-1.0), {}),
+    "window": (dict(window=-3), {}),
+    "query heads": ({}, dict(q=lambda q, k, v: q[:, :7])),
+    "query heads a KV head": ({}, dict(q=lambda q, k, v: q.repeat(1, 17, 1))),
+}
+
+
+@pytest.mark.parametrize("what", list(REFUSED) + list(REFUSED_ATTENTION))
+def test_a_refused_layer_call_reserves_nothing(cuda, what):
+    """Lengths, tables, pool and cache are as before, so the call can be made again."""
+    settings, change = {**REFUSED, **REFUSED_ATTENTION}[what]
+    settings = dict(settings)
+    table = settings.pop("table", None)
+    if table is not None:
+        table = rope_table(64, 48, device=cuda) if table == 48 else \
+            rope_table(64, 128, device=cuda).to(table)
+    for name in ("q_norm", "k_norm"):
+        if name in settings:
+            w = settings[name]
+            settings[name] = torch.ones(64, dtype=BF16, device=cuda) if w == 64 else \
+                torch.ones(128, dtype=w, device=cuda)
+    layer = ChunkedAttention(cos_sin=table, **settings)
+    manager = SequenceKVManager(PagedKVCache(16, 16, 2, 128, device="cuda"), 2, 64)
+    q, k, v = layer_call(cuda)
+    cu = torch.tensor([0, 18, 21], dtype=torch.int32, device=cuda)
+    new = {name: change[name](q, k, v) if name in change else x
+           for name, x in (("q", q), ("k", k), ("v", v))}
+    cu_bad = change["cu"](cu) if "cu" in change else cu
+    ids = torch.tensor(change["ids"], dtype=torch.int32, device=cuda) if "ids" in change else None
+    ChunkedAttention()(manager, q, k, v, cu)          # the sequences hold something
+    before = layer_state(manager)
+    calls = [layer] if what in REFUSED_ATTENTION else [layer, layer.append]
+    for call in calls:
+        with pytest.raises((ValueError, RuntimeError)):
+            call(manager, new["q"], new["k"], new["v"], cu_bad, ids)
+        torch.cuda.synchronize()
+        for a, b in zip(before, layer_state(manager)):
+            assert torch.equal(a, b)
+    manager.cache.check()
+
+
+def test_a_layer_takes_64_bit_offsets_and_rows(cuda):
+    """torch's default integers: converted once, for the reservation and for the calls."""
+    q, k, v = layer_call(cuda)
+    outs, states = [], []
+    for dtype in (torch.int32, torch.int64):
+        manager = SequenceKVManager(PagedKVCache(16, 16, 2, 128, device="cuda"), 3, 64)
+        cu = torch.tensor([0, 18, 21], dtype=dtype, device=cuda)
+        ids = torch.tensor([2, 0], dtype=dtype, device=cuda)
+        layer = ChunkedAttention(cos_sin=rope_table(64, 128, device=cuda))
+        outs.append(layer(manager, q, k, v, cu, ids))
+        rotated, starts = layer.append(manager, q, k, v, cu, ids)
+        outs.append(rotated)
+        assert starts.tolist() == [18, 3]
+        states.append(layer_state(manager))
+        manager.cache.check()
+    assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
+    assert all(torch.equal(a, b) for a, b in zip(*states))

@@ -153,3 +153,29 @@ def test_launches_go_to_the_tensors_device(fake, call, name):
         call()
         assert fake.calls[-1][:2] == (name, device)
         assert fake.device == 0
+
+
+def test_checks_refuse_what_the_calls_refuse():
+    """The check entry points answer as the calls do, whatever else the call would need."""
+    lib = _lib.load()
+    kv = _lib.KvDesc(256, 256, _lib.DTYPE_BF16, 10, 16, 2, 128, 0, 4096, 256, 128)
+    rg = _lib.RaggedDesc(256, None, None, 256, 256, 2, 9, 2, 4)
+
+    def rope(rot=128, hq=8, eps=1e-6):
+        return _lib.RopeAppend(256, 256, 256, 256, _lib.DTYPE_BF16, hq, *[1024, 128] * 4, 256, 99,
+                               rot, 0, _lib.DTYPE_BF16, None, 256, eps)
+
+    def chunk(hq=8, scale=0.1, window=0):
+        return _lib.ChunkAttend(256, 256, None, _lib.DTYPE_BF16, hq, 1024, 128, 1024, 128, scale,
+                                1, window)
+
+    assert lib.cvsa_rope_append_check(kv, rg, rope()) == _lib.OK
+    assert lib.cvsa_chunk_attend_check(kv, rg, chunk()) == _lib.OK
+    for bad in (rope(rot=48), rope(hq=0), rope(eps=-1.0), None):
+        st = lib.cvsa_rope_append(kv, rg, bad, None, None)
+        assert st != _lib.OK and lib.cvsa_rope_append_check(kv, rg, bad) == st
+    for bad in (chunk(hq=7), chunk(hq=130), chunk(scale=-1.0), chunk(window=-1), None):
+        st = lib.cvsa_chunk_attend(kv, rg, bad, None, 256, 1 << 40, None)
+        assert st != _lib.OK and lib.cvsa_chunk_attend_check(kv, rg, bad) == st
+    assert lib.cvsa_rope_append_check(None, rg, rope()) == _lib.ERR_INVALID
+    assert lib.cvsa_chunk_attend_check(kv, None, chunk()) == _lib.ERR_INVALID
