@@ -98,7 +98,8 @@ __device__ __forceinline__ int chunk_units(const SeqInfo& q, const ChunkGeo& g, 
 }
 
 // What a CTA does: units [u0, u1) of the stream, starting at unit `skip` of
-// item (b, i, h). (The host has checked that the units fit 31 bits.)
+// item (b, i, h). The host has checked that the units of sequences that share
+// no token fit 31 bits.
 struct ChunkRange {
   int u0, u1, per_cta;
   int b, i, h, skip;
@@ -145,12 +146,19 @@ __device__ __forceinline__ ChunkRange chunk_range(const RaggedView& rg, const Ch
   const int lane = threadIdx.x & 31;
   SeqInfo q = {};
   ChunkRange r = {};
-  int total = 0, units = 0;
+  int units = 0;
+  int64_t sum = 0;
 #pragma unroll 1
   for (int b0 = 0; b0 < rg.B; b0 += 32) {
     units = chunk_seq_units(rg, g, b0, q, cta == 0 ? dev_err : nullptr);
-    total += warp_sum_i(units);
+    sum += __reduce_add_sync(0xffffffffu, (unsigned)units & 0xffff) +
+           ((int64_t)__reduce_add_sync(0xffffffffu, (unsigned)units >> 16) << 16);
   }
+  if (sum > 0x7fffffff) {  // offsets that name tokens again and again: nothing is done
+    if (cta == 0) set_dev_error(dev_err, CVSA_DEV_ERR_RAGGED);
+    return r;
+  }
+  const int total = (int)sum;
   r.per_cta = max(min_units, (total + ctas - 1) / ctas);
   r.u0 = (int)min((int64_t)total, (int64_t)cta * r.per_cta);
   r.u1 = min(total, r.u0 + r.per_cta);

@@ -525,7 +525,8 @@ int cvsa_paged_gather(const cvsa_kv_desc_t* kv, const int32_t* block_table_row,
  * CVSA_DEV_ERR_BLOCK_RANGE in *dev_error (nullable) and the token, row or key
  * is skipped. Output rows of a sequence whose table row is out of range are 0;
  * output rows of one whose offsets are (negative, decreasing, past num_tokens)
- * are not written. */
+ * are not written, nor are any where decreasing offsets name so many tokens
+ * twice that the work passes 2^31 tiles. */
 typedef struct cvsa_ragged_desc {
   const int32_t* cu_tokens;       /* [batch + 1], non-decreasing, from 0 */
   const int32_t* seq_ids;         /* [batch] rows of the tables, or NULL: row b */

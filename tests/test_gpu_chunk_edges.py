@@ -288,3 +288,26 @@ def test_a_layer_takes_64_bit_offsets_and_rows(cuda):
         manager.cache.check()
     assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
     assert all(torch.equal(a, b) for a, b in zip(*states))
+
+
+@pytest.mark.parametrize("dtype,pairs", [(BF16, 550), (BF16, 1100), (F32, 600)])
+def test_offsets_that_name_all_tokens_again_and_again(cuda, dtype, pairs):
+    """Offsets 0, T, 0, T, ...: every second sequence is out of order, the others own all
+    tokens, and the work of all of them does not fit the plan's 31 bits. Flagged, nothing
+    written; the next call is as ever."""
+    T, ctx, hkv, d, page = 8192, 131072, 2, 64, 16
+    pool = torch.zeros((ctx // page, page, hkv, d), dtype=dtype, device=cuda)
+    q = torch.zeros((1, 64 * hkv, d), dtype=dtype, device=cuda).expand(T, -1, -1)
+    tables = torch.arange(ctx // page, dtype=torch.int32, device=cuda)[None]
+    lens = torch.tensor([ctx], dtype=torch.int32, device=cuda)
+    cu = torch.tensor([0, T] * pairs + [0], dtype=torch.int32, device=cuda)
+    ids = torch.zeros(2 * pairs, dtype=torch.int32, device=cuda)
+    out = torch.full(q.shape, 3.0, dtype=dtype, device=cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    chunk_attention(q, pool, pool, tables, lens, cu, causal=False, seq_ids=ids, out=out,
+                    dev_error=err)
+    assert int(err.item()) == _lib.DEV_ERR_RAGGED
+    assert bool((out == 3).all())
+    P = Problem([3, 140], [700, 300], 8, 2, d, dtype=dtype, seed=50)
+    got = attend(P)
+    assert int(P.dev_error.item()) == 0 and bool(torch.isfinite(got).all())
