@@ -33,20 +33,21 @@ namespace {
 constexpr int kReserveThreads = 1024;
 
 // Inclusive sum over the block; `warp_sums` holds one value a warp.
-__device__ __forceinline__ int block_scan_incl(int v, int* warp_sums) {
+template <typename T>
+__device__ __forceinline__ T block_scan_incl(T v, T* warp_sums) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int t = __shfl_up_sync(0xffffffffu, v, o);
+    const T t = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += t;
   }
   if (lane == 31) warp_sums[wid] = v;
   __syncthreads();
   if (wid == 0) {
-    int w = warp_sums[lane];
+    T w = warp_sums[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, w, o);
+      const T t = __shfl_up_sync(0xffffffffu, w, o);
       if (lane >= o) w += t;
     }
     warp_sums[lane] = w;
@@ -62,6 +63,7 @@ reserve_kernel(const int32_t* cu, const int32_t* seq_ids, int B, int num_seqs, i
                int32_t* tables, int W, int32_t* lens, int32_t* pages_alloc,
                const int32_t* free_list, int free_len, int32_t* free_head, int32_t* starts,
                int32_t* dev_err) {
+  __shared__ int64_t wanted_sums[32];
   __shared__ int warp_sums[32];
   __shared__ int s_incl[kReserveThreads];   // inclusive sum of the pages granted
   __shared__ int s_slot[kReserveThreads];   // table row and first new page of a granted sequence
@@ -93,15 +95,16 @@ reserve_kernel(const int32_t* cu, const int32_t* seq_ids, int B, int num_seqs, i
         }
       }
     }
-    const int incl = block_scan_incl(need, warp_sums);
+    // 64 bits: offsets out of order can ask for the same pages again and again
+    const int64_t incl = block_scan_incl((int64_t)need, wanted_sums);
     if (ok && need > 0 && (head0 < 0 || head0 + wanted + incl > free_len)) {
       set_dev_error(dev_err, CVSA_DEV_ERR_POOL);
       ok = false;
       need = 0;
     }
-    if (tid == kReserveThreads - 1) warp_sums[0] = incl;
+    if (tid == kReserveThreads - 1) wanted_sums[0] = incl;
     __syncthreads();
-    wanted += warp_sums[0];
+    wanted += wanted_sums[0];
     __syncthreads();
     if (b < B) {
       if (starts) starts[b] = ok ? start : -1;

@@ -311,3 +311,17 @@ def test_offsets_that_name_all_tokens_again_and_again(cuda, dtype, pairs):
     P = Problem([3, 140], [700, 300], 8, 2, d, dtype=dtype, seed=50)
     got = attend(P)
     assert int(P.dev_error.item()) == 0 and bool(torch.isfinite(got).all())
+
+
+def test_reservations_that_ask_for_more_than_31_bits_of_pages(cuda):
+    """Offsets 0, n, 0, n, ... over one row: 512 times 2^22 pages, the sum of which passes 31
+    bits. Every one is refused; the pool and the row keep their state."""
+    cache = PagedKVCache(64, 1, 1, 64, device="cuda")
+    manager = SequenceKVManager(cache, 1, 1 << 22)
+    cu = torch.tensor([0, 1 << 22] * 512 + [0], dtype=torch.int32, device=cuda)
+    ids = torch.zeros(1024, dtype=torch.int32, device=cuda)
+    starts = manager.reserve(cu, ids)
+    assert starts.tolist() == [-1] * 1024
+    assert int(cache.dev_error.item()) == _lib.DEV_ERR_RAGGED | _lib.DEV_ERR_POOL
+    assert cache._next_free == 0 and manager.context_lens.tolist() == [0]
+    assert manager.pages_allocated.tolist() == [0] and int(manager.block_tables.abs().max()) == 0
