@@ -8,12 +8,14 @@ csrc/chunk_attend.cu). The reference computes prompts in the model library
 (eval/latency_benchmark.py:376-420) and has no counterpart.
 """
 
+import struct
 from typing import Optional
 
 import torch
 
 from cvsa import _lib
 
+_ALL = 2 ** 31 - 1  # keys: more than a sequence can hold
 _ws_bytes = {}  # workspace bytes by (device, head_dim, dtypes)
 
 
@@ -61,12 +63,16 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                             or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous float32 [T, H_q]")
     qs, os_, mem = q.stride(), out.stride(), _lib.ARGS
-    mem.pack_chunk(mem.buf, 0, *_lib.kv_fields(k_cache, v_cache),
-                   *_lib.ragged_fields(T, cu_tokens, block_tables, context_lens, seq_ids,
-                                       start_positions),
-                   q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-                   _lib.dtype_code(q.dtype), Hq, qs[0], qs[1], os_[0], os_[1],
-                   D ** -0.5 if scale is None else scale, causal, window)
+    try:
+        mem.pack_chunk(mem.buf, 0, *_lib.kv_fields(k_cache, v_cache),
+                       *_lib.ragged_fields(T, cu_tokens, block_tables, context_lens, seq_ids,
+                                           start_positions),
+                       q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                       _lib.dtype_code(q.dtype), Hq, qs[0], qs[1], os_[0], os_[1],
+                       D ** -0.5 if scale is None else scale, causal,
+                       window if window < _ALL else _ALL)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"chunk_attention: an argument is out of range ({e})") from None
     lib, stream = _lib.load(), _lib.raw_stream(dev)
     if check_only:
         _lib.check(lib.cvsa_chunk_attend_check(mem.kv, mem.rg, mem.chunk), "cvsa_chunk_attend")

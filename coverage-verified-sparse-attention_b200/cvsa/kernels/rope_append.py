@@ -10,6 +10,7 @@ norms and rotation to the model library and appends token by token
 (cvsa/runtime/kv_cache.py:133-150).
 """
 
+import struct
 from typing import Callable, Optional
 
 import torch
@@ -100,14 +101,17 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
             raise ValueError("cos_sin must be a contiguous float32 [max_positions, rot_dim]")
         pos, rot = cos_sin.shape
     ks, vs, mem = k.stride(), v.stride(), _lib.ARGS
-    mem.pack_rope(mem.buf, 0, *_lib.kv_fields(k_cache, v_cache),
-                  *_lib.ragged_fields(T, cu_tokens, block_tables, context_lens, seq_ids,
-                                      start_positions),
-                  qp, k.data_ptr(), v.data_ptr(), op, _lib.dtype_code(k.dtype), Hq,
-                  qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1],
-                  0 if cos_sin is None else cos_sin.data_ptr(), pos, rot, interleaved,
-                  _lib.dtype_code(ndt), 0 if q_norm is None else q_norm.data_ptr(),
-                  0 if k_norm is None else k_norm.data_ptr(), eps)
+    try:
+        mem.pack_rope(mem.buf, 0, *_lib.kv_fields(k_cache, v_cache),
+                      *_lib.ragged_fields(T, cu_tokens, block_tables, context_lens, seq_ids,
+                                          start_positions),
+                      qp, k.data_ptr(), v.data_ptr(), op, _lib.dtype_code(k.dtype), Hq,
+                      qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os_[0], os_[1],
+                      0 if cos_sin is None else cos_sin.data_ptr(), pos, rot, interleaved,
+                      _lib.dtype_code(ndt), 0 if q_norm is None else q_norm.data_ptr(),
+                      0 if k_norm is None else k_norm.data_ptr(), eps)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"rope_append: an argument is out of range ({e})") from None
     lib = _lib.load()
     if _reserve is not None:
         _lib.check(lib.cvsa_rope_append_check(mem.kv, mem.rg, mem.rope), "cvsa_rope_append")

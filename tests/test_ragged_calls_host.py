@@ -179,3 +179,18 @@ def test_checks_refuse_what_the_calls_refuse():
         assert st != _lib.OK and lib.cvsa_chunk_attend_check(kv, rg, bad) == st
     assert lib.cvsa_rope_append_check(None, rg, rope()) == _lib.ERR_INVALID
     assert lib.cvsa_chunk_attend_check(kv, None, chunk()) == _lib.ERR_INVALID
+
+
+def test_arguments_past_their_type(fake):
+    """A window of any size is a window; other numbers the library's structs cannot hold are
+    a ValueError like every refused argument."""
+    q, k, pool, i = tensors()
+    where = (i.view(1, 2), i[:1], i)
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 63):
+        chunk_attend.chunk_attention(q, pool, pool, *where, window=window)
+        assert _lib.ARGS.chunk.window == 2 ** 31 - 1
+    for bad in (dict(scale=1e39), dict(scale=-1e39), dict(window=-2 ** 31 - 1)):
+        with pytest.raises(ValueError, match="out of range"):
+            chunk_attend.chunk_attention(q, pool, pool, *where, **bad)
+    with pytest.raises(ValueError, match="out of range"):
+        rope_append.rope_append(q, k, k, pool, pool, *where, k_norm=torch.ones(64), eps=1e39)
