@@ -194,7 +194,9 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
       }
       __syncthreads();  // K is done with
       copy(k + 1, a.kv.k, sm.k);
-      bool cut = false;  // some row of the block does not see every key of the tile
+      // some row of the block does not see every key of the tile; rows past the item's
+      // end see none, so items that do not fill the block take the selecting loop
+      bool cut = false;
 #pragma unroll
       for (int x = 0; x < kX; ++x) {
         float mx = m[x];

@@ -29,8 +29,9 @@
 // registers by unrolled code. The first 64 weights of a row are handed over
 // before the rest is computed, so the second product starts earlier, and the
 // next tile's last 64 scores are formed as soon as this tile's were read for
-// the last time (1024 tokens at 32K keys, 64 heads: 1.44 -> 1.34 ms in short runs, 800
-// TFLOP/s).
+// the last time (1024 tokens at 32K keys, 64 heads: 1.44 -> 1.34 ms when it was
+// made). That case takes 1.28 ms now in ten calls after a pause, 845 TFLOP/s, and
+// 1.45 ms, 749 TFLOP/s, in a second of calls, whose power lowers the clock.
 //
 // Loads: a page holds 16 tokens of one head 2 KB or 4 KB apart, so a tensor
 // copy would be many small boxes; 16-byte asynchronous copies per lane,
