@@ -21,6 +21,7 @@ int dtype_bytes(int dtype) {
     case CVSA_DTYPE_F32: return 4;
     case CVSA_DTYPE_F16: return 2;
     case CVSA_DTYPE_BF16: return 2;
+    case CVSA_DTYPE_E4M3: return 1;
     default: return 0;
   }
 }
@@ -65,10 +66,11 @@ int cuda_status(cudaError_t e, const char* what) {
 
 bool valid_dtype(int dt) { return dt == CVSA_DTYPE_F32 || dt == CVSA_DTYPE_F16 || dt == CVSA_DTYPE_BF16; }
 
-int check_kv(const cvsa_kv_desc_t* kv, KvView* out) {
+// `f8`: the call takes 8-bit pools too.
+int check_kv(const cvsa_kv_desc_t* kv, KvView* out, bool f8 = false) {
   if (!kv) return fail(CVSA_ERR_INVALID, "kv descriptor is NULL");
   if (!kv->k_cache || !kv->v_cache) return fail(CVSA_ERR_INVALID, "k_cache/v_cache is NULL");
-  if (!valid_dtype(kv->dtype)) return fail(CVSA_ERR_INVALID, "kv dtype %d unknown", kv->dtype);
+  if (!valid_dtype(kv->dtype) && !(f8 && kv->dtype == CVSA_DTYPE_E4M3)) return fail(CVSA_ERR_INVALID, "kv dtype %d unknown", kv->dtype);
   if (kv->num_blocks <= 0 || kv->block_size <= 0 || kv->num_kv_heads <= 0 || kv->head_dim <= 0)
     return fail(CVSA_ERR_INVALID, "kv shape must be positive (blocks=%d bs=%d hkv=%d d=%d)",
                 kv->num_blocks, kv->block_size, kv->num_kv_heads, kv->head_dim);
@@ -89,6 +91,20 @@ int check_kv(const cvsa_kv_desc_t* kv, KvView* out) {
   out->sb = kv->stride_block;
   out->st = kv->stride_token;
   out->sh = kv->stride_head;
+  return CVSA_OK;
+}
+
+// Pools that may be of 8 bits, with their pages' scales (NULL for other pools). A call
+// that reads keys only passes need_v false.
+int check_kv8(const cvsa_kv_desc_t* kv, const float* k_scale, const float* v_scale, KvView* out,
+              bool need_v = true) {
+  const int st = check_kv(kv, out, true);
+  if (st) return st;
+  const bool f8 = kv->dtype == CVSA_DTYPE_E4M3;
+  if (f8 != (k_scale != nullptr) || (need_v && f8 != (v_scale != nullptr)))
+    return fail(CVSA_ERR_INVALID, "scales go with 8-bit pools, and with those only");
+  out->ks = k_scale;
+  out->vs = v_scale;
   return CVSA_OK;
 }
 
@@ -255,6 +271,84 @@ int check_chunk_call(const cvsa_kv_desc_t* kvd, const cvsa_ragged_desc_t* rgd,
   if (st) return st;
   st = check_ragged(rgd, rg);
   return st ? st : check_chunk(args, *kv, *rg, c);
+}
+
+int check_append_to(const cvsa_kv_desc_t* kvd, const float* k_scale, const float* v_scale,
+                    const cvsa_ragged_desc_t* rgd, const cvsa_rope_append_t* args,
+                    const int32_t* position_shift, KvView* kv, RaggedView* rg, RopeView* r) {
+  int st = check_kv8(kvd, k_scale, v_scale, kv);
+  if (st) return st;
+  if ((st = check_ragged(rgd, rg))) return st;
+  if ((st = check_rope(args, *kv, *rg, r))) return st;
+  r->shift = position_shift;
+  if (kv->dtype == CVSA_DTYPE_E4M3 && !append8_fits(*rg, *kv, *r))
+    return fail(CVSA_ERR_UNSUPPORTED, "pages and query rows of the batch above 2^31 blocks");
+  return CVSA_OK;
+}
+
+int check_chunk_q8(const cvsa_kv_desc_t* kvd, const float* k_scale, const float* v_scale,
+                   const cvsa_ragged_desc_t* rgd, const cvsa_chunk_attend_t* args, KvView* kv,
+                   RaggedView* rg, ChunkView* c) {
+  int st = check_kv8(kvd, k_scale, v_scale, kv);
+  if (st) return st;
+  if (kv->dtype != CVSA_DTYPE_E4M3) return fail(CVSA_ERR_INVALID, "kv dtype is not of 8 bits");
+  st = check_ragged(rgd, rg);
+  return st ? st : check_chunk(args, *kv, *rg, c);
+}
+
+int check_key_weights(const cvsa_kv_desc_t* kvd, const float* k_scale,
+                      const cvsa_ragged_desc_t* rgd, const cvsa_key_weights_t* a, KvView* kv,
+                      RaggedView* rg, KeyWeightsView* w) {
+  int st = check_kv8(kvd, k_scale, nullptr, kv, false);
+  if (st) return st;
+  if ((st = check_ragged(rgd, rg))) return st;
+  if (!a) return fail(CVSA_ERR_INVALID, "arguments are NULL");
+  if (!valid_dtype(a->dtype)) return fail(CVSA_ERR_INVALID, "q dtype %d unknown", a->dtype);
+  if (a->num_q_heads <= 0 || a->num_q_heads % kv->hkv != 0)
+    return fail(CVSA_ERR_INVALID, "num_q_heads=%d is not a positive multiple of num_kv_heads=%d",
+                a->num_q_heads, kv->hkv);
+  if (rg->T > 0 && (!a->q || !a->lse)) return fail(CVSA_ERR_INVALID, "q/lse is NULL");
+  if (rg->B > 0 && (!a->prior || !a->out)) return fail(CVSA_ERR_INVALID, "prior/out is NULL");
+  if (!(a->scale > 0.f) || a->scale > 3.0e38f)
+    return fail(CVSA_ERR_INVALID, "scale must be positive and finite");
+  if (!(a->decay >= 0.f) || a->decay > 3.0e38f)
+    return fail(CVSA_ERR_INVALID, "decay must be >= 0 and finite");
+  if (a->window < 0 || (a->window > 0 && !a->causal))
+    return fail(CVSA_ERR_INVALID, "window must be >= 0, and 0 without causal");
+  if (a->weights_stride < (int64_t)rg->W * kv->bs)
+    return fail(CVSA_ERR_INVALID, "weights rows must hold max_pages * block_size keys");
+  const int eb = dtype_bytes(a->dtype);
+  if (reinterpret_cast<uintptr_t>(a->q) % 16 || (a->q_stride_token * eb) % 16 ||
+      (a->q_stride_head * eb) % 16)
+    return fail(CVSA_ERR_INVALID, "q rows must be 16-byte aligned");
+  w->q = a->q;
+  w->lse = a->lse;
+  w->dtype = a->dtype;
+  w->hq = a->num_q_heads;
+  w->q_st = a->q_stride_token;
+  w->q_sh = a->q_stride_head;
+  w->scale = a->scale;
+  w->decay = a->decay;
+  w->causal = a->causal != 0;
+  w->window = a->window < (1 << 30) ? a->window : 1 << 30;  // positions less a window fit
+  w->prior = a->prior;
+  w->out = a->out;
+  w->stride = a->weights_stride;
+  if (!key_weights_supported(*kv, *rg, *w))
+    return fail(CVSA_ERR_UNSUPPORTED,
+                "key_weights built for head_dim 64/128/256, G<=64, and fewer than 2^31 tiles of "
+                "64 keys over the tables and heads");
+  return CVSA_OK;
+}
+
+// pages that `keep` tokens of a page size take
+int64_t pages_of(int64_t keep, int bs) { return (keep + bs - 1) / bs; }
+
+int check_keep(int keep, int sink, int recent) {
+  if (keep <= 0 || sink < 0 || recent < 0 || (int64_t)sink + recent > keep)
+    return fail(CVSA_ERR_INVALID, "keep=%d must be positive, sink=%d + recent=%d at most that",
+                keep, sink, recent);
+  return CVSA_OK;
 }
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -1206,6 +1300,174 @@ int cvsa_chunk_attend(const cvsa_kv_desc_t* kvd, const cvsa_ragged_desc_t* rgd,
                 chunk_attend_workspace_bytes(kv, rg, c));
   return cuda_status(launch_chunk_attend(kv, rg, c, workspace, dev_error, (cudaStream_t)stream),
                      "chunk_attend launch");
+}
+
+int cvsa_rope_append_to_check(const cvsa_kv_desc_t* kvd, const float* k_scale,
+                              const float* v_scale, const cvsa_ragged_desc_t* rgd,
+                              const cvsa_rope_append_t* args, const int32_t* position_shift) {
+  KvView kv;
+  RaggedView rg;
+  RopeView r;
+  return check_append_to(kvd, k_scale, v_scale, rgd, args, position_shift, &kv, &rg, &r);
+}
+
+int cvsa_rope_append_to(const cvsa_kv_desc_t* kvd, float* k_scale, float* v_scale,
+                        const cvsa_ragged_desc_t* rgd, const cvsa_rope_append_t* args,
+                        const int32_t* position_shift, int32_t* dev_error, void* stream) {
+  KvView kv;
+  RaggedView rg;
+  RopeView r;
+  const int st = check_append_to(kvd, k_scale, v_scale, rgd, args, position_shift, &kv, &rg, &r);
+  if (st) return st;
+  if (rg.B == 0 || rg.T == 0) return CVSA_OK;
+  const cudaStream_t s = (cudaStream_t)stream;
+  return cuda_status(kv.dtype == CVSA_DTYPE_E4M3 ? launch_append8(rg, kv, r, dev_error, s)
+                                                 : launch_rope_append(rg, kv, r, dev_error, s),
+                     "rope_append launch");
+}
+
+int cvsa_chunk_attend_q8_check(const cvsa_kv_desc_t* kvd, const float* k_scale,
+                               const float* v_scale, const cvsa_ragged_desc_t* rgd,
+                               const cvsa_chunk_attend_t* args) {
+  KvView kv;
+  RaggedView rg;
+  ChunkView c;
+  return check_chunk_q8(kvd, k_scale, v_scale, rgd, args, &kv, &rg, &c);
+}
+
+size_t cvsa_chunk_attend_q8_workspace_size(const cvsa_kv_desc_t* kvd, const float* k_scale,
+                                           const float* v_scale, const cvsa_ragged_desc_t* rgd,
+                                           const cvsa_chunk_attend_t* args) {
+  KvView kv;
+  RaggedView rg;
+  ChunkView c;
+  if (check_chunk_q8(kvd, k_scale, v_scale, rgd, args, &kv, &rg, &c)) return 0;
+  return chunk_attend_workspace_bytes(kv, rg, c);
+}
+
+int cvsa_chunk_attend_q8(const cvsa_kv_desc_t* kvd, const float* k_scale, const float* v_scale,
+                         const cvsa_ragged_desc_t* rgd, const cvsa_chunk_attend_t* args,
+                         int32_t* dev_error, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  KvView kv;
+  RaggedView rg;
+  ChunkView c;
+  const int st = check_chunk_q8(kvd, k_scale, v_scale, rgd, args, &kv, &rg, &c);
+  if (st) return st;
+  if (rg.B == 0 || rg.T == 0) return CVSA_OK;
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 ||
+      workspace_bytes < chunk_attend_workspace_bytes(kv, rg, c))
+    return fail(CVSA_ERR_WORKSPACE, "workspace NULL, misaligned or below %zu bytes",
+                chunk_attend_workspace_bytes(kv, rg, c));
+  return cuda_status(launch_chunk_attend(kv, rg, c, workspace, dev_error, (cudaStream_t)stream),
+                     "chunk_attend launch");
+}
+
+int cvsa_key_weights_check(const cvsa_kv_desc_t* kvd, const float* k_scale,
+                           const cvsa_ragged_desc_t* rgd, const cvsa_key_weights_t* args) {
+  KvView kv;
+  RaggedView rg;
+  KeyWeightsView w;
+  return check_key_weights(kvd, k_scale, rgd, args, &kv, &rg, &w);
+}
+
+int cvsa_key_weights(const cvsa_kv_desc_t* kvd, const float* k_scale,
+                     const cvsa_ragged_desc_t* rgd, const cvsa_key_weights_t* args,
+                     int32_t* dev_error, void* stream) {
+  KvView kv;
+  RaggedView rg;
+  KeyWeightsView w;
+  const int st = check_key_weights(kvd, k_scale, rgd, args, &kv, &rg, &w);
+  if (st) return st;
+  if (rg.B == 0) return CVSA_OK;
+  return cuda_status(launch_key_weights(kv, rg, w, dev_error, (cudaStream_t)stream),
+                     "key_weights launch");
+}
+
+int cvsa_evict(const cvsa_kv_desc_t* kvd, float* k_scale, float* v_scale,
+               const int32_t* block_tables, const int32_t* context_lens, int32_t num_seqs,
+               int32_t max_pages, const cvsa_evict_t* a, int32_t* dev_error, void* stream) {
+  KvView kv;
+  int st = check_kv8(kvd, k_scale, v_scale, &kv);
+  if (st) return st;
+  if (!a) return fail(CVSA_ERR_INVALID, "arguments are NULL");
+  if (num_seqs < 0 || max_pages <= 0) return fail(CVSA_ERR_INVALID, "bad shape");
+  if ((st = check_keep(a->keep, a->sink, a->recent))) return st;
+  if (a->new_pages != pages_of(a->keep, kv.bs))
+    return fail(CVSA_ERR_INVALID, "new_pages=%d, but %d tokens take %lld", a->new_pages, a->keep,
+                (long long)pages_of(a->keep, kv.bs));
+  if (a->weights_stride < (int64_t)max_pages * kv.bs || a->out_stride < a->keep ||
+      (a->out_weights == a->weights && a->out_stride != a->weights_stride))
+    return fail(CVSA_ERR_INVALID, "rows of weights must hold max_pages * block_size keys, of "
+                                  "out_weights `keep`; in place both are the same");
+  if (num_seqs == 0) return CVSA_OK;
+  if (!block_tables || !context_lens || !a->weights || !a->out_weights || !a->new_tables ||
+      !a->kept)
+    return fail(CVSA_ERR_INVALID, "NULL pointer");
+  EvictView e;
+  e.tables = block_tables;
+  e.lens = context_lens;
+  e.S = num_seqs;
+  e.W = max_pages;
+  e.weights = a->weights;
+  e.w_stride = a->weights_stride;
+  e.out_weights = a->out_weights;
+  e.o_stride = a->out_stride;
+  e.new_tables = a->new_tables;
+  e.new_pages = a->new_pages;
+  e.kept = a->kept;
+  e.keep = a->keep;
+  e.sink = a->sink;
+  e.recent = a->recent;
+  if (!evict_supported(kv, e))
+    return fail(CVSA_ERR_UNSUPPORTED, "evict built for tables of fewer than 2^30 keys");
+  return cuda_status(launch_evict(kv, e, dev_error, (cudaStream_t)stream), "evict launch");
+}
+
+static int check_evict_pages(const cvsa_evict_pages_t* a, EvictPages* p) {
+  if (!a) return fail(CVSA_ERR_INVALID, "arguments are NULL");
+  if (a->num_seqs < 0 || a->max_pages <= 0 || a->block_size <= 0 || a->keep <= 0 ||
+      a->free_list_len < 0)
+    return fail(CVSA_ERR_INVALID, "bad shape");
+  if (pages_of(a->keep, a->block_size) > a->max_pages)
+    return fail(CVSA_ERR_INVALID, "keep=%d exceeds the block table", a->keep);
+  if (a->num_seqs > 0 && (!a->block_tables || !a->context_lens || !a->pages_allocated ||
+                          !a->evicted || !a->free_list || !a->free_head || !a->new_tables ||
+                          !a->plan_lens))
+    return fail(CVSA_ERR_INVALID, "NULL pointer");
+  p->S = a->num_seqs;
+  p->W = a->max_pages;
+  p->bs = a->block_size;
+  p->keep = a->keep;
+  p->new_pages = (int)pages_of(a->keep, a->block_size);
+  p->tables = a->block_tables;
+  p->lens = a->context_lens;
+  p->pages_alloc = a->pages_allocated;
+  p->evicted = a->evicted;
+  p->free_list = a->free_list;
+  p->free_head = a->free_head;
+  p->free_len = a->free_list_len;
+  p->new_tables = a->new_tables;
+  p->plan_lens = a->plan_lens;
+  return CVSA_OK;
+}
+
+int cvsa_evict_reserve(const cvsa_evict_pages_t* args, int32_t* dev_error, void* stream) {
+  EvictPages p;
+  const int st = check_evict_pages(args, &p);
+  if (st) return st;
+  if (p.S == 0) return CVSA_OK;
+  return cuda_status(launch_evict_reserve(p, dev_error, (cudaStream_t)stream),
+                     "evict reserve launch");
+}
+
+int cvsa_evict_commit(const cvsa_evict_pages_t* args, int32_t* dev_error, void* stream) {
+  EvictPages p;
+  const int st = check_evict_pages(args, &p);
+  if (st) return st;
+  if (p.S == 0) return CVSA_OK;
+  return cuda_status(launch_evict_commit(p, dev_error, (cudaStream_t)stream),
+                     "evict commit launch");
 }
 
 }  // extern "C"

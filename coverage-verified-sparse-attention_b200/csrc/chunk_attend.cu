@@ -1,5 +1,5 @@
 // Attention of a ragged batch of new tokens over the paged cache: the general
-// kernel (any mix of fp32, bf16, f16) and the merge of split items.
+// kernel (any mix of fp32, bf16, f16, and 8-bit pools) and the merge of split items.
 //
 // Row (token t, query head h) at position p sees keys [lo, hi): hi = p + 1
 // (causal) or the context length, lo = max(0, p - window + 1) or 0.
@@ -21,6 +21,7 @@
 #include "cvsa_common.cuh"
 #include "cvsa_internal.h"
 #include "cvsa_launch.cuh"
+#include "fp8.cuh"
 
 namespace cvsa {
 namespace {
@@ -52,6 +53,8 @@ template <typename T, int D>
 __device__ __forceinline__ void load_row_piece(const T* src, float* dst) {  // 4 elements
   if constexpr (sizeof(T) == 4) {
     *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(src);
+  } else if constexpr (sizeof(T) == 1) {
+    e4m3x4_to_f4(*reinterpret_cast<const uint32_t*>(src), dst);
   } else {
     const uint2 w = *reinterpret_cast<const uint2*>(src);
     float f[4];
@@ -79,13 +82,20 @@ struct GenSmem {
   int8_t key_ok[2][kKeys];
   ChunkRange range;
 };
+template <int D, int ROWS>
+struct GenSmem8 : GenSmem<D, ROWS> {  // of an 8-bit pool: scales of a key's page
+  float k_scale[2][kKeys], v_scale[2][kKeys];
+};
+template <typename C, int D, int ROWS>
+using GenSmemOf = typename std::conditional<sizeof(C) == 1, GenSmem8<D, ROWS>, GenSmem<D, ROWS>>::type;
 
 template <typename T, typename C, int D, int kRows>
 __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
 chunk_general_kernel(const __grid_constant__ GenArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   constexpr int kX = kRows / 16;  // rows of a thread
-  GenSmem<D, kRows>& sm = *reinterpret_cast<GenSmem<D, kRows>*>(smem_raw);
+  using Smem = GenSmemOf<C, D, kRows>;
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
   const int cta = blockIdx.x;
   if (tid < 32) {
@@ -139,6 +149,11 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
         ok = blk >= 0 && blk < a.kv.num_blocks;
         if (!ok) set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);
         off = ok ? blk * a.kv.sb + (key % a.kv.bs) * a.kv.st + it.h * a.kv.sh : 0;
+        if constexpr (sizeof(C) == 1) {
+          const int64_t at = (int64_t)blk * a.kv.hkv + it.h;
+          sm.k_scale[k & 1][tid] = ok ? a.kv.ks[at] : 0.f;
+          sm.v_scale[k & 1][tid] = ok ? a.kv.vs[at] : 0.f;
+        }
       }
       sm.key_off[k & 1][tid] = off;
       sm.key_ok[k & 1][tid] = ok;
@@ -155,6 +170,10 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
           } else {
             float f[4] = {0.f, 0.f, 0.f, 0.f};
             if (ok) load_row_piece<C, D>(src, f);
+            if constexpr (sizeof(C) == 1) {
+              const float x = to == sm.k ? sm.k_scale[k & 1][r] : sm.v_scale[k & 1][r];
+              if (ok) f[0] *= x, f[1] *= x, f[2] *= x, f[3] *= x;
+            }
             *reinterpret_cast<float4*>(&to[r][c * 4]) = make_float4(f[0], f[1], f[2], f[3]);
           }
         }
@@ -317,11 +336,11 @@ cudaError_t launch_general_d(const GenArgs& a, int rows, int ctas, cudaStream_t 
     return cudaGetLastError();
   };
   switch (a.kv.d) {
-    case 64: return go(chunk_general_kernel<T, C, 64, 64>, sizeof(GenSmem<64, 64>));
+    case 64: return go(chunk_general_kernel<T, C, 64, 64>, sizeof(GenSmemOf<C, 64, 64>));
     case 128:
-      if (rows == 64) return go(chunk_general_kernel<T, C, 128, 64>, sizeof(GenSmem<128, 64>));
-      return go(chunk_general_kernel<T, C, 128, 128>, sizeof(GenSmem<128, 128>));
-    case 256: return go(chunk_general_kernel<T, C, 256, 64>, sizeof(GenSmem<256, 64>));
+      if (rows == 64) return go(chunk_general_kernel<T, C, 128, 64>, sizeof(GenSmemOf<C, 128, 64>));
+      return go(chunk_general_kernel<T, C, 128, 128>, sizeof(GenSmemOf<C, 128, 128>));
+    case 256: return go(chunk_general_kernel<T, C, 256, 64>, sizeof(GenSmemOf<C, 256, 64>));
     default: return cudaErrorInvalidValue;
   }
 }
@@ -331,6 +350,7 @@ cudaError_t launch_general_c(const GenArgs& a, int rows, int ctas, cudaStream_t 
   switch (a.kv.dtype) {
     case CVSA_DTYPE_BF16: return launch_general_d<T, __nv_bfloat16>(a, rows, ctas, s);
     case CVSA_DTYPE_F16: return launch_general_d<T, __half>(a, rows, ctas, s);
+    case CVSA_DTYPE_E4M3: return launch_general_d<T, uint8_t>(a, rows, ctas, s);
     default: return launch_general_d<T, float>(a, rows, ctas, s);
   }
 }

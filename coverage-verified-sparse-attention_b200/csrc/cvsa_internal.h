@@ -20,6 +20,9 @@ struct KvView {
   int hkv;  // KV heads
   int d;    // head_dim
   int64_t sb, st, sh;  // strides (elements): block, token, head
+  // 8-bit pools (CVSA_DTYPE_E4M3): scales [num_blocks, hkv] of keys and values
+  const float* ks = nullptr;
+  const float* vs = nullptr;
 };
 
 struct QView {
@@ -268,6 +271,7 @@ struct RopeView {
   const void* q_norm; const void* k_norm;  // [head_dim] or null
   int norm_f32;            // weights are float32 (else dtype)
   float eps;
+  const int32_t* shift = nullptr;  // [num_seqs] added to positions for the rotation
 };
 cudaError_t launch_paged_reserve(const int32_t* cu, const int32_t* seq_ids, int B, int num_seqs,
                                  int bs, int32_t* tables, int W, int32_t* lens,
@@ -277,6 +281,11 @@ cudaError_t launch_paged_reserve(const int32_t* cu, const int32_t* seq_ids, int 
 bool rope_append_supported(const KvView& kv);
 cudaError_t launch_rope_append(const RaggedView& rg, const KvView& kv, const RopeView& r,
                                int32_t* dev_err, cudaStream_t s);
+
+// ---- append8.cu (8-bit pools) ----
+bool append8_fits(const RaggedView& rg, const KvView& kv, const RopeView& r);
+cudaError_t launch_append8(const RaggedView& rg, const KvView& kv, const RopeView& r,
+                           int32_t* dev_err, cudaStream_t s);
 
 // ---- chunk_attend.cu (any supported type), chunk_attend_tc.cu (16-bit, tensor cores) ----
 struct ChunkView {
@@ -290,5 +299,41 @@ size_t chunk_attend_workspace_bytes(const KvView& kv, const RaggedView& rg, cons
 bool chunk_attend_supported(const KvView& kv, const RaggedView& rg, const ChunkView& c);
 cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const ChunkView& c,
                                 void* ws, int32_t* dev_err, cudaStream_t s);
+
+// ---- key_weights.cu ----
+struct KeyWeightsView {
+  const void* q; const float* lse;        // lse [T, hq]
+  int dtype, hq;
+  int64_t q_st, q_sh;                     // element strides: token, head
+  float scale, decay;
+  int causal, window;                     // window 0: none
+  const float* prior; float* out;         // [num_seqs, hkv, stride]
+  int64_t stride;
+};
+bool key_weights_supported(const KvView& kv, const RaggedView& rg, const KeyWeightsView& w);
+cudaError_t launch_key_weights(const KvView& kv, const RaggedView& rg, const KeyWeightsView& w,
+                               int32_t* dev_err, cudaStream_t s);
+
+// ---- evict.cu ----
+struct EvictView {
+  const int32_t* tables; const int32_t* lens;  // [S, W], [S]
+  int S, W;
+  const float* weights; int64_t w_stride;      // [S, hkv, w_stride]
+  float* out_weights; int64_t o_stride;        // [S, hkv, o_stride]; may be weights
+  const int32_t* new_tables; int new_pages;    // [S, new_pages]
+  int32_t* kept;                               // [S, hkv, keep]
+  int keep, sink, recent;
+};
+bool evict_supported(const KvView& kv, const EvictView& e);
+cudaError_t launch_evict(const KvView& kv, const EvictView& e, int32_t* dev_err, cudaStream_t s);
+struct EvictPages {
+  int S, W, bs, keep, new_pages;
+  int32_t* tables; int32_t* lens; int32_t* pages_alloc; int32_t* evicted;
+  int32_t* free_list; int32_t* free_head;
+  int free_len;
+  int32_t* new_tables; int32_t* plan_lens;     // [S, new_pages], [S]
+};
+cudaError_t launch_evict_reserve(const EvictPages& p, int32_t* dev_err, cudaStream_t s);
+cudaError_t launch_evict_commit(const EvictPages& p, int32_t* dev_err, cudaStream_t s);
 
 }  // namespace cvsa

@@ -1,0 +1,404 @@
+// Eviction from the paged cache by accumulated attention weight.
+//
+// A sequence longer than `keep` keeps, for each KV head, its first `sink` keys, its
+// last `recent` ones and those of largest weight between (equal weights: the earlier
+// key; NaN below everything), `keep` in all, in their order. Their keys, values and
+// weights move to the front: rows to new pages, so that no row is written over
+// before it is read and all rows can move at once.
+//
+// select: one block a (sequence, KV head). The cut, the n-th largest weight, is found
+//   by a radix select over the weights' order-preserving keys, 11, 11 and 10 bits a
+//   pass; a pass in order then writes the kept keys, placed by a prefix sum.
+// gather: one warp a new page and KV head; bound by bytes. In an 8-bit cache a new
+//   page gets the largest scale of the rows that go there, so none overflows; rows of
+//   smaller scale move to it (exact but for values that become subnormal).
+// reserve, commit: the page bookkeeping around them, one block each.
+#include "block_scan.cuh"
+#include "cvsa_common.cuh"
+#include "cvsa_internal.h"
+#include "fp8.cuh"
+
+namespace cvsa {
+namespace {
+
+constexpr int kThreads = 1024, kBins = 2048, kEach = 8;
+
+struct SelectArgs {
+  EvictView e;
+  int hkv, bs;
+  int cached;  // keys of a row that shared memory holds
+  int32_t* dev_err;
+};
+
+// The sequence's length where it is evicted from, else 0.
+__device__ __forceinline__ int evict_len(const EvictView& e, int bs, int s, int32_t* dev_err) {
+  const int len = e.lens[s];
+  if (len < 0 || len > (int64_t)e.W * bs) {
+    set_dev_error(dev_err, CVSA_DEV_ERR_RAGGED);
+    return 0;
+  }
+  return len > e.keep ? len : 0;
+}
+
+__global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_constant__ SelectArgs a) {
+  extern __shared__ uint32_t keys[];  // [cached]
+  __shared__ int hist[kBins];
+  __shared__ int sums[32];
+  __shared__ int s_bin, s_left;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int s = blockIdx.x / a.hkv, h = blockIdx.x % a.hkv;
+  const int len = evict_len(a.e, a.bs, s, tid == 0 && h == 0 ? a.dev_err : nullptr);
+  int32_t* const kept = a.e.kept + ((int64_t)s * a.hkv + h) * a.e.keep;
+  if (len == 0) {
+    for (int i = tid; i < a.e.keep; i += kThreads) kept[i] = -1;
+    return;
+  }
+  const float* const w = a.e.weights + ((int64_t)s * a.hkv + h) * a.e.w_stride;
+  float* const out = a.e.out_weights + ((int64_t)s * a.hkv + h) * a.e.o_stride;
+  const int lo = a.e.sink, hi = len - a.e.recent;
+  int left = a.e.keep - a.e.sink - a.e.recent;  // to take of [lo, hi)
+  const int cached = min(a.cached, hi - lo);
+  for (int i = tid; i < cached; i += kThreads) keys[i] = float_key(w[lo + i]);
+  // key of candidate i
+  auto key_at = [&](int i) { return i < cached ? keys[i] : float_key(w[lo + i]); };
+  uint32_t cut = 0xffffffffu;  // keys above are taken
+  int room = 0;                // and this many of those equal to it
+  if (left > 0) {
+    uint32_t prefix = 0, mask = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass < 2 ? 11 : 10;
+      for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
+      __syncthreads();
+      for (int i0 = 0; i0 < hi - lo; i0 += kThreads) {
+        const int i = i0 + tid;
+        const uint32_t k = i < hi - lo ? key_at(i) : 0;
+        const int bin = i < hi - lo && (k & mask) == prefix ? (int)(k >> shift & ((1 << bits) - 1)) : -1;
+        // neighbouring keys share bins: one addition a warp and bin
+        const unsigned same = __match_any_sync(0xffffffffu, bin);
+        if (bin >= 0 && __ffs(same) - 1 == lane) atomicAdd(&hist[bin], __popc(same));
+      }
+      __syncthreads();
+      // bin that holds the left-th key from the top: sums from the highest bin
+      const int top = kBins - 1 - 2 * tid;
+      const int c0 = hist[top], c1 = hist[top - 1];
+      const int incl = block_scan_incl(c0 + c1, sums);
+      const int before = incl - c0 - c1;
+      if (before < left && incl >= left) {
+        const bool first = before + c0 >= left;
+        s_bin = first ? top : top - 1;
+        s_left = left - (first ? before : before + c0);
+      }
+      __syncthreads();
+      prefix |= (uint32_t)s_bin << shift;
+      mask |= (uint32_t)((1 << bits) - 1) << shift;
+      left = s_left;
+      __syncthreads();
+    }
+    cut = prefix;
+    room = left;
+  }
+  // in order, kEach neighbours a thread; a key's place is the number taken before it
+  int taken = 0, equal = 0;  // before this round: taken without those equal to the cut, and these
+  for (int i0 = 0; i0 < len; i0 += kThreads * kEach) {
+    const int base = i0 + tid * kEach;
+    float x[kEach];
+    uint32_t above = 0, same = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int i = base + j;
+      x[j] = i < len ? w[i] : 0.f;
+      const uint32_t k = float_key(x[j]);
+      const bool forced = i < lo || i >= hi;
+      if (i < len && (forced || k > cut)) above |= 1u << j;
+      if (i < len && !forced && k == cut && room > 0) same |= 1u << j;
+    }
+    // both counts in one scan: at most kThreads * kEach = 8192 of each
+    const int mine = __popc(above) | __popc(same) << 16;
+    const int incl = block_scan_incl(mine, sums);
+    int a0 = taken + ((incl - mine) & 0xffff), q0 = equal + ((incl - mine) >> 16);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const bool is_above = above >> j & 1, is_same = same >> j & 1;
+      if (is_above || (is_same && q0 < room)) {
+        const int at = a0 + min(q0, room);
+        kept[at] = base + j;
+        out[at] = x[j];  // at <= base + j: read by this round or an earlier one
+      }
+      a0 += is_above;
+      q0 += is_same;
+    }
+    if (tid == kThreads - 1) sums[0] = incl;
+    __syncthreads();
+    taken += sums[0] & 0xffff;
+    equal += sums[0] >> 16;
+    __syncthreads();
+  }
+}
+
+struct GatherArgs {
+  EvictView e;
+  KvView kv;
+  int eb;        // bytes of an element
+  int chunks;    // 16-byte chunks of a row
+  int32_t* dev_err;
+};
+
+constexpr int kGatherWarps = 4, kBatch = 4;
+
+template <bool F8>
+__global__ void __launch_bounds__(kGatherWarps * 32) evict_gather_kernel(const __grid_constant__ GatherArgs a) {
+  const int lane = threadIdx.x & 31, bs = a.kv.bs, hkv = a.kv.hkv;
+  const int64_t warp = (int64_t)blockIdx.x * kGatherWarps + (threadIdx.x >> 5);
+  const int h = (int)(warp % hkv), page = (int)(warp / hkv % a.e.new_pages);
+  const int64_t s = warp / hkv / a.e.new_pages;
+  if (s >= a.e.S || evict_len(a.e, bs, (int)s, nullptr) == 0) return;
+  const int to = a.e.new_tables[s * a.e.new_pages + page];
+  if (to < 0 || to >= a.kv.num_blocks) {
+    if (lane == 0) set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);
+    return;
+  }
+  const int n = (int)min((int64_t)bs, a.e.keep - (int64_t)page * bs);  // rows of the page
+  const int32_t* const kept = a.e.kept + (s * hkv + h) * a.e.keep + (int64_t)page * bs;
+  const uint8_t* const pk = static_cast<const uint8_t*>(a.kv.k);
+  const uint8_t* const pv = static_cast<const uint8_t*>(a.kv.v);
+  // lane i: byte offset of row r0 + i of the page (-1: none) and its block
+  auto locate = [&](int r0, int& blk) -> int64_t {
+    blk = -1;
+    if (r0 + lane >= n) return -1;
+    const int key = kept[r0 + lane];
+    blk = a.e.tables[s * a.e.W + key / bs];
+    if (blk < 0 || blk >= a.kv.num_blocks) {
+      set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);
+      blk = -1;
+      return -1;
+    }
+    return (blk * a.kv.sb + (key % bs) * a.kv.st + h * a.kv.sh) * a.eb;
+  };
+  int ek = kScaleMin, ev = kScaleMin;  // exponents of the new page
+  if constexpr (F8) {
+    for (int r0 = 0; r0 < n; r0 += 32) {
+      int blk;
+      locate(r0, blk);
+      if (blk >= 0) {
+        ek = max(ek, scale_exponent_of(a.kv.ks[(int64_t)blk * hkv + h]));
+        ev = max(ev, scale_exponent_of(a.kv.vs[(int64_t)blk * hkv + h]));
+      }
+    }
+    ek = __reduce_max_sync(0xffffffffu, ek);
+    ev = __reduce_max_sync(0xffffffffu, ev);
+    if (lane == 0) {
+      const_cast<float*>(a.kv.ks)[(int64_t)to * hkv + h] = pow2(ek);
+      const_cast<float*>(a.kv.vs)[(int64_t)to * hkv + h] = pow2(ev);
+    }
+  }
+  uint8_t* const base_k = const_cast<uint8_t*>(pk) + (to * a.kv.sb + h * a.kv.sh) * a.eb;
+  uint8_t* const base_v = const_cast<uint8_t*>(pv) + (to * a.kv.sb + h * a.kv.sh) * a.eb;
+  const int64_t st = a.kv.st * a.eb;
+  for (int r0 = 0; r0 < n; r0 += 32) {
+    int blk;
+    const int64_t off = locate(r0, blk);
+    float fk = 1.f, fv = 1.f;
+    if constexpr (F8) {
+      if (blk >= 0) {
+        fk = pow2(scale_exponent_of(a.kv.ks[(int64_t)blk * hkv + h]) - ek);
+        fv = pow2(scale_exponent_of(a.kv.vs[(int64_t)blk * hkv + h]) - ev);
+      }
+    }
+    const int pieces = min(32, n - r0) * a.chunks;
+    for (int e0 = 0; e0 < pieces; e0 += 32 * kBatch) {
+      uint4 xk[kBatch], xv[kBatch];
+      int64_t from[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int e = e0 + i * 32 + lane, r = min(e / a.chunks, 31);
+        from[i] = __shfl_sync(0xffffffffu, off, r);
+        if (e >= pieces) from[i] = -1;
+        if (from[i] < 0) continue;
+        const int64_t at = from[i] + e % a.chunks * 16;
+        xk[i] = *reinterpret_cast<const uint4*>(pk + at);
+        xv[i] = *reinterpret_cast<const uint4*>(pv + at);
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int e = e0 + i * 32 + lane, r = min(e / a.chunks, 31);
+        if constexpr (F8) {
+          const float mk = __shfl_sync(0xffffffffu, fk, r), mv = __shfl_sync(0xffffffffu, fv, r);
+          if (from[i] >= 0) {
+            uint32_t* wk = reinterpret_cast<uint32_t*>(&xk[i]);
+            uint32_t* wv = reinterpret_cast<uint32_t*>(&xv[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float f[4];
+              e4m3x4_to_f4(wk[j], f);
+              wk[j] = f4_to_e4m3x4(f[0] * mk, f[1] * mk, f[2] * mk, f[3] * mk);
+              e4m3x4_to_f4(wv[j], f);
+              wv[j] = f4_to_e4m3x4(f[0] * mv, f[1] * mv, f[2] * mv, f[3] * mv);
+            }
+          }
+        }
+        if (from[i] < 0) continue;
+        const int64_t at = (r0 + e / a.chunks) * st + e % a.chunks * 16;
+        *reinterpret_cast<uint4*>(base_k + at) = xk[i];
+        *reinterpret_cast<uint4*>(base_v + at) = xv[i];
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// pages: one block; the sequences' numbers are prefix sums in batch order
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(kThreads) evict_reserve_kernel(const __grid_constant__ EvictPages p,
+                                                                 int32_t* dev_err) {
+  __shared__ int64_t sums[32];
+  __shared__ int64_t s_first[kThreads];  // place of a sequence's first new page in the free list
+  const int tid = threadIdx.x;
+  const int64_t head = *p.free_head;
+  // a sequence's pages to give back, or -1: it is not evicted from
+  auto gives = [&](int b) {
+    if (b >= p.S) return -1;
+    const int len = p.lens[b], old = p.pages_alloc[b];
+    if (len < 0 || len > (int64_t)p.W * p.bs || old < 0 || old > p.W) {
+      set_dev_error(dev_err, CVSA_DEV_ERR_RAGGED);
+      return -1;
+    }
+    return len > p.keep ? old : -1;
+  };
+  const int64_t most = head < 0 || head > p.free_len ? 0 : (p.free_len - head) / p.new_pages;
+  // pages that come back from the sequences that get theirs: the first `most`
+  int64_t want = 0, back = 0;
+  for (int b0 = 0; b0 < p.S; b0 += kThreads) {
+    const int g = gives(b0 + tid);
+    const int64_t nth = want + block_scan_incl((int64_t)(g >= 0), sums);
+    const int64_t came = block_scan_incl((int64_t)(g >= 0 && nth <= most ? g : 0), sums);
+    if (tid == kThreads - 1) sums[0] = nth, sums[1] = came;
+    __syncthreads();
+    want = sums[0];
+    back += sums[1];
+    __syncthreads();
+  }
+  const int64_t got = min(want, most);
+  // the list has no room for pages that it did not hand out: nothing is evicted
+  const bool fits = back <= head + got * p.new_pages;
+  if (tid == 0 && (want > most || (want > 0 && !fits))) set_dev_error(dev_err, CVSA_DEV_ERR_POOL);
+  int64_t seen = 0;
+  for (int b0 = 0; b0 < p.S; b0 += kThreads) {
+    const int b = b0 + tid;
+    const int g = gives(b);
+    const int64_t nth = seen + block_scan_incl((int64_t)(g >= 0), sums);
+    const bool ok = g >= 0 && fits && nth <= most;
+    if (b < p.S) p.plan_lens[b] = ok ? p.lens[b] : 0;
+    s_first[tid] = ok ? head + (nth - 1) * p.new_pages : -1;
+    if (tid == kThreads - 1) sums[0] = nth;
+    __syncthreads();
+    seen = sums[0];
+    const int rows = min(kThreads, p.S - b0);
+    for (int64_t e = tid; e < (int64_t)rows * p.new_pages; e += kThreads) {
+      const int64_t first = s_first[e / p.new_pages];
+      p.new_tables[(int64_t)b0 * p.new_pages + e] =
+          first >= 0 ? p.free_list[first + e % p.new_pages] : -1;
+    }
+    __syncthreads();
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) evict_commit_kernel(const __grid_constant__ EvictPages p) {
+  __shared__ int64_t sums[32];
+  __shared__ int64_t s_incl[kThreads];
+  const int tid = threadIdx.x;
+  const int64_t head = *p.free_head;
+  int64_t got = 0, back = 0;
+  for (int b0 = 0; b0 < p.S; b0 += kThreads) {
+    const int b = b0 + tid;
+    const bool ok = b < p.S && p.plan_lens[b] > 0;
+    const int64_t n = block_scan_incl((int64_t)ok, sums);
+    const int64_t g = block_scan_incl((int64_t)(ok ? p.pages_alloc[b] : 0), sums);
+    if (tid == kThreads - 1) sums[0] = n, sums[1] = g;
+    __syncthreads();
+    got += sums[0];
+    back += sums[1];
+    __syncthreads();
+  }
+  int64_t at = head + got * p.new_pages - back;  // the list's new head
+  const int64_t new_head = at;
+  for (int b0 = 0; b0 < p.S; b0 += kThreads) {
+    const int b = b0 + tid;
+    const bool ok = b < p.S && p.plan_lens[b] > 0;
+    s_incl[tid] = block_scan_incl((int64_t)(ok ? p.pages_alloc[b] : 0), sums);
+    __syncthreads();
+    const int64_t total = s_incl[kThreads - 1];
+    for (int64_t e = tid; e < total; e += kThreads) {
+      int lo = 0, hi = kThreads - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s_incl[mid] > e) hi = mid; else lo = mid + 1;
+      }
+      p.free_list[at + e] = p.tables[(int64_t)(b0 + lo) * p.W + (e - (lo ? s_incl[lo - 1] : 0))];
+    }
+    at += total;
+    __syncthreads();
+    const int rows = min(kThreads, p.S - b0);
+    for (int64_t e = tid; e < (int64_t)rows * p.new_pages; e += kThreads) {
+      const int64_t row = b0 + e / p.new_pages;
+      if (p.plan_lens[row] > 0)
+        p.tables[row * p.W + e % p.new_pages] = p.new_tables[row * p.new_pages + e % p.new_pages];
+    }
+    if (ok) {
+      p.evicted[b] += p.plan_lens[b] - p.keep;
+      p.lens[b] = p.keep;
+      p.pages_alloc[b] = p.new_pages;
+    }
+    __syncthreads();
+  }
+  if (tid == 0) *p.free_head = (int)new_head;
+}
+
+}  // namespace
+
+bool evict_supported(const KvView& kv, const EvictView& e) {
+  return (int64_t)e.S * kv.hkv < (int64_t(1) << 31) && (int64_t)e.W * kv.bs < (int64_t(1) << 30) &&
+         (int64_t)e.S * e.new_pages * kv.hkv / kGatherWarps < (int64_t(1) << 31) - 1;
+}
+
+cudaError_t launch_evict(const KvView& kv, const EvictView& e, int32_t* dev_err, cudaStream_t s) {
+  SelectArgs a;
+  a.e = e;
+  a.hkv = kv.hkv;
+  a.bs = kv.bs;
+  a.dev_err = dev_err;
+  const int64_t row = (int64_t)e.W * kv.bs;
+  constexpr int kCached = 48 * 1024;
+  a.cached = row < kCached ? (int)row : kCached;
+  cudaError_t err = cudaFuncSetAttribute(
+      evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCached * 4);
+  if (err != cudaSuccess) return err;
+  evict_select_kernel<<<e.S * kv.hkv, kThreads, a.cached * 4, s>>>(a);
+  err = cudaGetLastError();
+  if (err != cudaSuccess) return err;
+  GatherArgs g;
+  g.e = e;
+  g.kv = kv;
+  g.eb = dtype_bytes(kv.dtype);
+  g.chunks = kv.d * g.eb / 16;
+  g.dev_err = dev_err;
+  const int64_t warps = (int64_t)e.S * e.new_pages * kv.hkv;
+  const unsigned blocks = (unsigned)((warps + kGatherWarps - 1) / kGatherWarps);
+  if (kv.dtype == CVSA_DTYPE_E4M3)
+    evict_gather_kernel<true><<<blocks, kGatherWarps * 32, 0, s>>>(g);
+  else
+    evict_gather_kernel<false><<<blocks, kGatherWarps * 32, 0, s>>>(g);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_evict_reserve(const EvictPages& p, int32_t* dev_err, cudaStream_t s) {
+  evict_reserve_kernel<<<1, kThreads, 0, s>>>(p, dev_err);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_evict_commit(const EvictPages& p, int32_t* dev_err, cudaStream_t s) {
+  evict_commit_kernel<<<1, kThreads, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace cvsa

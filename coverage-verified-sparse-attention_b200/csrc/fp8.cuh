@@ -1,0 +1,51 @@
+// 8-bit floats (e4m3) with power-of-two scales, as the 8-bit cache holds them.
+//
+// A page's scale is 2^e, -15 <= e <= 7, the least that brings the page's largest
+// absolute value under the type's 448. A power of two moves a value without
+// rounding it (but for those that become subnormal), so the mantissa's three bits
+// are all the cache loses, a page can move to a larger scale when larger tokens
+// join it, and the bounds make every stored value an f16 and a bf16 number exactly:
+// 448 * 2^7 = 57344 is below f16's largest, 2^-9 * 2^-15 its smallest.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "cvsa_common.cuh"
+
+namespace cvsa {
+
+constexpr int kScaleMin = -15, kScaleMax = 7;
+
+// Two codes (low byte first) as f16; exact.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
+  return (uint32_t)h.x | (uint32_t)h.y << 16;
+}
+// Four codes as floats; exact.
+__device__ __forceinline__ void e4m3x4_to_f4(uint32_t four, float* f) {
+  f16x2_to_f2(e4m3x2_to_f16x2(four & 0xffffu), f[0], f[1]);
+  f16x2_to_f2(e4m3x2_to_f16x2(four >> 16), f[2], f[3]);
+}
+// Four floats as codes: nearest, halves to even, beyond 448 saturated, NaN kept.
+__device__ __forceinline__ uint32_t f4_to_e4m3x4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
+}
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126..127
+
+// The exponent of a page's scale for largest absolute value `amax` (finite, >= 0):
+// the least e with amax <= 1.75 * 2^(8 + e), in the scale's range.
+__device__ __forceinline__ int scale_exponent(float amax) {
+  const int bits = __float_as_int(amax);
+  const int e = (bits >> 23) - 127 - ((bits & 0x7fffff) > 0x600000 ? 7 : 8);
+  return max(kScaleMin, min(kScaleMax, e));
+}
+// The exponent that a stored scale stands for, in range whatever the word holds.
+__device__ __forceinline__ int scale_exponent_of(float scale) {
+  const int e = ((__float_as_int(scale) >> 23) & 0xff) - 127;
+  return max(kScaleMin, min(kScaleMax, e));
+}
+
+}  // namespace cvsa

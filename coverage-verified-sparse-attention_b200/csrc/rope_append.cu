@@ -21,8 +21,10 @@
 // (sequence, position, block id) is uniform; the row's data loads are issued before it. It is bound by
 // instruction issue and occupancy together: several rows a lane, or a lookup a
 // token shared through shared memory, cost more in registers than they saved.
+#include "block_scan.cuh"
 #include "cvsa_common.cuh"
 #include "cvsa_internal.h"
+#include "rope_rows.cuh"
 
 namespace cvsa {
 namespace {
@@ -31,32 +33,6 @@ namespace {
 // reserve
 // ---------------------------------------------------------------------------
 constexpr int kReserveThreads = 1024;
-
-// Inclusive sum over the block; `warp_sums` holds one value a warp.
-template <typename T>
-__device__ __forceinline__ T block_scan_incl(T v, T* warp_sums) {
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const T t = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += t;
-  }
-  if (lane == 31) warp_sums[wid] = v;
-  __syncthreads();
-  if (wid == 0) {
-    T w = warp_sums[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const T t = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += t;
-    }
-    warp_sums[lane] = w;
-  }
-  __syncthreads();
-  if (wid > 0) v += warp_sums[wid - 1];
-  __syncthreads();
-  return v;
-}
 
 __global__ void __launch_bounds__(kReserveThreads)
 reserve_kernel(const int32_t* cu, const int32_t* seq_ids, int B, int num_seqs, int bs,
@@ -150,54 +126,8 @@ struct RopeArgs {
   int32_t* dev_err;
 };
 
-// 8 consecutive elements as floats, and back.
-template <typename T>
-__device__ __forceinline__ void load8(const void* base, int64_t elem, float* f) {
-  const T* p = reinterpret_cast<const T*>(base) + elem;
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p + i * Vec16<T>::N);
-    Vec16<T>::unpack(w, f + i * Vec16<T>::N);
-  }
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  return Mma<T>::pack(a, b);
-}
-template <typename T>
-__device__ __forceinline__ void store8(void* base, int64_t elem, const float* f) {
-  T* p = reinterpret_cast<T*>(base) + elem;
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
-  } else {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]),
-                                              pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-  }
-}
-
-// The sequence that holds token t, by the whole warp: 32 probes a step of the
-// offsets cu[0..B], so three dependent loads serve any batch up to 32768.
-// -1 when no sequence holds it.
-__device__ __forceinline__ int warp_find_seq(const int32_t* cu, int B, int t) {
-  int lo = 0, n = B;  // the answer, if any, is in [lo, lo + n)
-  const int lane = threadIdx.x & 31;
-  if (t < cu[0] || t >= cu[B]) return -1;
-  while (n > 1) {
-    const int step = (n + 31) / 32;
-    const int at = lo + min(lane * step, n);          // lane 0 probes lo: cu[lo] <= t holds
-    const bool below = lane * step < n && cu[at] <= t;
-    const unsigned m = __ballot_sync(0xffffffffu, below);
-    const int k = 31 - __clz(m | 1u);
-    lo += k * step;
-    n = min(step, n - k * step);
-  }
-  return lo;
-}
-
 template <typename T, typename C, int U>  // input type, cache type, lanes a row (head_dim / 16)
 __global__ void __launch_bounds__(64) rope_append_kernel(const __grid_constant__ RopeArgs a) {
-  constexpr int D = U * 16;
   const int lane = threadIdx.x & 31, u = lane % U;
   // blockIdx.x is the token, so what is looked up is the same for the block
   const int tok = blockIdx.x, hq = a.r.hq, hkv = a.kv.hkv;
@@ -225,7 +155,7 @@ __global__ void __launch_bounds__(64) rope_append_kernel(const __grid_constant__
   }
   const int b = warp_find_seq(a.rg.cu, a.rg.B, tok);
   const bool rotate = a.r.cos_sin != nullptr && kind != 2;
-  int pos = -1, slot = -1, page = 0;
+  int pos = -1, slot = -1, page = 0, turn = 0;
   bool good = live && b >= 0;
   if (good) {
     slot = a.rg.seq_ids ? a.rg.seq_ids[b] : b;
@@ -240,8 +170,10 @@ __global__ void __launch_bounds__(64) rope_append_kernel(const __grid_constant__
       pos = a.rg.lens[slot] - (a.rg.cu[b + 1] - tok);
     }
     page = a.bs_shift >= 0 ? pos >> a.bs_shift : pos / a.kv.bs;
+    turn = pos;
+    if (good && a.r.shift) turn = rope_turn(pos, a.r.shift[slot]);
     if (good && (pos < 0 || page >= a.rg.W ||
-                 (a.r.cos_sin && pos >= a.r.max_positions))) {
+                 (a.r.cos_sin && (turn < 0 || turn >= a.r.max_positions)))) {
       good = false;
       if (u == 0) set_dev_error(a.dev_err, CVSA_DEV_ERR_RAGGED);
     }
@@ -250,50 +182,12 @@ __global__ void __launch_bounds__(64) rope_append_kernel(const __grid_constant__
   if (good && kind != 0) blk = a.rg.tables[(int64_t)slot * a.rg.W + page];
   float cs[16];
   if (good && rotate && in_rot) {
-    const float* c = a.r.cos_sin + (int64_t)pos * a.r.rot + u * 8;
-    *reinterpret_cast<float4*>(cs) = *reinterpret_cast<const float4*>(c);
-    *reinterpret_cast<float4*>(cs + 4) = *reinterpret_cast<const float4*>(c + 4);
-    *reinterpret_cast<float4*>(cs + 8) = *reinterpret_cast<const float4*>(c + half);
-    *reinterpret_cast<float4*>(cs + 12) = *reinterpret_cast<const float4*>(c + half + 4);
+    const float* c = a.r.cos_sin + (int64_t)turn * a.r.rot + u * 8;
+    load_turn(c, half, cs);
   }
   const void* wn = kind == 0 ? a.r.q_norm : kind == 1 ? a.r.k_norm : nullptr;
-  float ss = 0.f;
-  if (a.r.q_norm || a.r.k_norm) {  // every lane, for the shuffles
-#pragma unroll
-    for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-    for (int o = U / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  }
-  if (wn) {
-    float w[16];
-    if (a.r.norm_f32) {
-      load8<float>(wn, e0, w);
-      load8<float>(wn, e1, w + 8);
-    } else {
-      load8<T>(wn, e0, w);
-      load8<T>(wn, e1, w + 8);
-    }
-    const float inv = rsqrtf(ss / D + a.r.eps);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = x[i] * inv * w[i];
-  }
-  if (good && rotate && in_rot) {
-    if (a.r.interleaved) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float p = x[2 * i], q = x[2 * i + 1];
-        x[2 * i] = p * cs[i] - q * cs[8 + i];
-        x[2 * i + 1] = q * cs[i] + p * cs[8 + i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float p = x[i], q = x[8 + i];
-        x[i] = p * cs[i] - q * cs[8 + i];
-        x[8 + i] = q * cs[i] + p * cs[8 + i];
-      }
-    }
-  }
+  if (a.r.q_norm || a.r.k_norm) norm_row<T, U>(x, wn, a.r.norm_f32, a.r.eps, e0, e1);
+  if (good && rotate && in_rot) rotate_row(x, cs, a.r.interleaved);
   if (!live || b < 0) return;
   if (kind == 0) {
     if (!good) {  // a row without a position: a defined value, not the buffer's old one

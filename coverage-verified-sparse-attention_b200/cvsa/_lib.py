@@ -23,7 +23,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcvsa_b200.so")
 
-DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_E4M3 = 0, 1, 2, 3
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_CUDA, ERR_POOL = 0, -1, -2, -3, -4, -5
 MODE_SCORE, MODE_LAZY, MODE_REUSE, MODE_DENSE = 0, 1, 2, 3
 RECOVERY_EXACT, RECOVERY_NONE, RECOVERY_APPROX = 0, 1, 2
@@ -130,6 +130,38 @@ class ChunkAttend(ctypes.Structure):
     ]
 
 
+class KeyWeights(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32), ("q_stride_token", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64), ("scale", ctypes.c_float), ("decay", ctypes.c_float),
+        ("causal", ctypes.c_int32), ("window", ctypes.c_int32), ("prior", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("weights_stride", ctypes.c_int64),
+    ]
+
+
+class Evict(ctypes.Structure):
+    _fields_ = [
+        ("weights", ctypes.c_void_p), ("weights_stride", ctypes.c_int64),
+        ("out_weights", ctypes.c_void_p), ("out_stride", ctypes.c_int64),
+        ("new_tables", ctypes.c_void_p), ("new_pages", ctypes.c_int32),
+        ("kept", ctypes.c_void_p), ("keep", ctypes.c_int32), ("sink", ctypes.c_int32),
+        ("recent", ctypes.c_int32),
+    ]
+
+
+class EvictPages(ctypes.Structure):
+    _fields_ = [
+        ("block_tables", ctypes.c_void_p), ("context_lens", ctypes.c_void_p),
+        ("pages_allocated", ctypes.c_void_p), ("evicted", ctypes.c_void_p),
+        ("free_list", ctypes.c_void_p), ("free_head", ctypes.c_void_p),
+        ("new_tables", ctypes.c_void_p), ("plan_lens", ctypes.c_void_p),
+        ("num_seqs", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+        ("block_size", ctypes.c_int32), ("keep", ctypes.c_int32),
+        ("free_list_len", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
 _SIGS = {
@@ -192,6 +224,26 @@ _SIGS = {
     "cvsa_chunk_attend": ([ctypes.POINTER(KvDesc), ctypes.POINTER(RaggedDesc),
                            ctypes.POINTER(ChunkAttend), _P, _P, ctypes.c_size_t, _P],
                           ctypes.c_int),
+    "cvsa_rope_append_to": ([ctypes.POINTER(KvDesc), _P, _P, ctypes.POINTER(RaggedDesc),
+                             ctypes.POINTER(RopeAppend), _P, _P, _P], ctypes.c_int),
+    "cvsa_rope_append_to_check": ([ctypes.POINTER(KvDesc), _P, _P, ctypes.POINTER(RaggedDesc),
+                                   ctypes.POINTER(RopeAppend), _P], ctypes.c_int),
+    "cvsa_chunk_attend_q8_check": ([ctypes.POINTER(KvDesc), _P, _P, ctypes.POINTER(RaggedDesc),
+                                    ctypes.POINTER(ChunkAttend)], ctypes.c_int),
+    "cvsa_chunk_attend_q8_workspace_size": (
+        [ctypes.POINTER(KvDesc), _P, _P, ctypes.POINTER(RaggedDesc),
+         ctypes.POINTER(ChunkAttend)], ctypes.c_size_t),
+    "cvsa_chunk_attend_q8": ([ctypes.POINTER(KvDesc), _P, _P, ctypes.POINTER(RaggedDesc),
+                              ctypes.POINTER(ChunkAttend), _P, _P, ctypes.c_size_t, _P],
+                             ctypes.c_int),
+    "cvsa_key_weights": ([ctypes.POINTER(KvDesc), _P, ctypes.POINTER(RaggedDesc),
+                          ctypes.POINTER(KeyWeights), _P, _P], ctypes.c_int),
+    "cvsa_key_weights_check": ([ctypes.POINTER(KvDesc), _P, ctypes.POINTER(RaggedDesc),
+                                ctypes.POINTER(KeyWeights)], ctypes.c_int),
+    "cvsa_evict": ([ctypes.POINTER(KvDesc), _P, _P, _P, _P, _I, _I, ctypes.POINTER(Evict), _P,
+                    _P], ctypes.c_int),
+    "cvsa_evict_reserve": ([ctypes.POINTER(EvictPages), _P, _P], ctypes.c_int),
+    "cvsa_evict_commit": ([ctypes.POINTER(EvictPages), _P, _P], ctypes.c_int),
     "cvsa_sparse_decode_noalloc": ([ctypes.POINTER(QueryDesc), ctypes.POINTER(KvDesc), _P, _I, _P,
                                     _P, _P, _P, _P, _I, _P], ctypes.c_int),
 }
@@ -363,22 +415,37 @@ class _ArgMemory(threading.local):
         self.rg = RaggedDesc.from_buffer(self.buf, 64)
         self.chunk = ChunkAttend.from_buffer(self.buf, 120)
         self.rope = RopeAppend.from_buffer(self.buf, 120)
+        self.weights = KeyWeights.from_buffer(self.buf, 120)
         self.pack_chunk = struct.Struct("<" + self._KV + self._RG + "QQQiiqqqqfii").pack_into
         self.pack_rope = struct.Struct("<" + self._KV + self._RG
                                        + "QQQQiiqqqqqqqqQiiiiQQf").pack_into
+        self.pack_weights = struct.Struct("<" + self._KV + self._RG
+                                          + "QQiiqqffiiQQq").pack_into
 
 
 ARGS = _ArgMemory()
 
 
-def kv_fields(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple:
-    """KvDesc's fields (kv_desc's checks)."""
-    shape, stride = k_cache.shape, k_cache.stride()
-    if (len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != k_cache.dtype
+def kv_fields(k_cache: torch.Tensor, v_cache: torch.Tensor, scaled: bool = False) -> tuple:
+    """KvDesc's fields (kv_desc's checks); scaled: the call has scales, for 8-bit pools."""
+    shape, stride, dt = k_cache.shape, k_cache.stride(), k_cache.dtype
+    if (len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != dt
             or v_cache.stride() != stride or stride[3] != 1):
         kv_desc(k_cache, v_cache)  # raises
-    return (k_cache.data_ptr(), v_cache.data_ptr(), dtype_code(k_cache.dtype), *shape, 0,
-            *stride[:3])
+    if scaled != (dt is torch.float8_e4m3fn):
+        raise ValueError("an 8-bit cache (float8_e4m3fn) needs its scales, another has none")
+    return (k_cache.data_ptr(), v_cache.data_ptr(), DTYPE_E4M3 if scaled else dtype_code(dt),
+            *shape, 0, *stride[:3])
+
+
+def scale_ptr(scale: Optional[torch.Tensor], cache: torch.Tensor, name: str) -> Optional[int]:
+    """Address of an 8-bit cache's scales (None without)."""
+    if scale is None:
+        return None
+    if (cache.dim() != 4 or scale.dtype is not torch.float32 or not scale.is_contiguous()
+            or scale.shape != (cache.shape[0], cache.shape[2])):
+        raise ValueError(f"{name} must be a contiguous float32 [num_blocks, H_kv]")
+    return scale.data_ptr()
 
 
 def token_rows(t: torch.Tensor, name: str) -> torch.Tensor:

@@ -26,6 +26,8 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     start_positions: Optional[torch.Tensor] = None,
                     out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
                     dev_error: Optional[torch.Tensor] = None, *,
+                    k_scale: Optional[torch.Tensor] = None,
+                    v_scale: Optional[torch.Tensor] = None,
                     check_only: bool = False) -> torch.Tensor:
     """softmax(scale q K^T) V per new token and query head, [T, H_q, D] in q's dtype.
 
@@ -38,6 +40,8 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     attention over other keys). A row that sees no key gives 0 and -inf, as
     does a sequence that was refused or whose table row is out of range. Rows no sequence
     owns (padding, offsets out of range) are not written.
+    k_scale, v_scale [num_blocks, H_kv]: the scales of an 8-bit cache
+    (float8_e4m3fn pools, any q dtype; a value is its code times its page's scale).
     check_only raises what the call would be refused with and returns the output
     unfilled, without a launch.
 
@@ -45,12 +49,13 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     graph's pool: graphs of different pools may be replayed at the same time.
     """
     dev = _lib.same_device(q, k_cache, v_cache, block_tables, context_lens, cu_tokens, seq_ids,
-                           start_positions, out, lse, dev_error)
+                           start_positions, out, lse, dev_error, k_scale, v_scale)
     if dev != torch.cuda.current_device():  # a launch goes to the current device
         with torch.cuda.device(dev):
             return chunk_attention(q, k_cache, v_cache, block_tables, context_lens, cu_tokens,
                                    causal, window, scale, seq_ids, start_positions, out, lse,
-                                   dev_error, check_only=check_only)
+                                   dev_error, k_scale=k_scale, v_scale=v_scale,
+                                   check_only=check_only)
     q = _lib.token_rows(q, "q")
     T, Hq, D = shape = q.shape
     if k_cache.dim() != 4 or k_cache.shape[3] != D:
@@ -62,9 +67,12 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if lse is not None and (lse.shape != (T, Hq) or lse.dtype != torch.float32
                             or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous float32 [T, H_q]")
+    scaled = k_scale is not None
+    if scaled != (v_scale is not None):
+        raise ValueError("k_scale and v_scale go together")
     qs, os_, mem = q.stride(), out.stride(), _lib.ARGS
     try:
-        mem.pack_chunk(mem.buf, 0, *_lib.kv_fields(k_cache, v_cache),
+        mem.pack_chunk(mem.buf, 0, *_lib.kv_fields(k_cache, v_cache, scaled),
                        *_lib.ragged_fields(T, cu_tokens, block_tables, context_lens, seq_ids,
                                            start_positions),
                        q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
@@ -74,26 +82,31 @@ def chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     except (struct.error, OverflowError) as e:
         raise ValueError(f"chunk_attention: an argument is out of range ({e})") from None
     lib, stream = _lib.load(), _lib.raw_stream(dev)
+    head, call = (mem.kv,), "cvsa_chunk_attend"
+    if scaled:
+        head = (mem.kv, _lib.scale_ptr(k_scale, k_cache, "k_scale"),
+                _lib.scale_ptr(v_scale, k_cache, "v_scale"))
+        call = "cvsa_chunk_attend_q8"
     if check_only:
-        _lib.check(lib.cvsa_chunk_attend_check(mem.kv, mem.rg, mem.chunk), "cvsa_chunk_attend")
+        _lib.check(getattr(lib, call + "_check")(*head, mem.rg, mem.chunk), call)
         return out
+    launch = getattr(lib, call)
     # the size depends on the head layout alone; 0 for what the call will refuse
     key = (dev, D, q.dtype, k_cache.dtype)
     nbytes = _ws_bytes.get(key)
     if nbytes is None:
-        nbytes = lib.cvsa_chunk_attend_workspace_size(mem.kv, mem.rg, mem.chunk)
+        nbytes = getattr(lib, call + "_workspace_size")(*head, mem.rg, mem.chunk)
         if nbytes:
             _ws_bytes[key] = nbytes
     if nbytes and torch.cuda.is_current_stream_capturing():
         # memory of the graph, like its other tensors
         buf = torch.empty(nbytes + 256, dtype=torch.uint8, device=q.device)
-        st = lib.cvsa_chunk_attend(mem.kv, mem.rg, mem.chunk, _lib.ptr(dev_error),
-                                   buf.data_ptr() + (-buf.data_ptr()) % 256, nbytes, stream)
+        st = launch(*head, mem.rg, mem.chunk, _lib.ptr(dev_error),
+                    buf.data_ptr() + (-buf.data_ptr()) % 256, nbytes, stream)
     else:
         with _lib.WORKSPACE.lock:
             ws = _lib.WORKSPACE.address(nbytes, q.device, stream, "chunk") if nbytes else None
-            st = lib.cvsa_chunk_attend(mem.kv, mem.rg, mem.chunk, _lib.ptr(dev_error), ws, nbytes,
-                                       stream)
+            st = launch(*head, mem.rg, mem.chunk, _lib.ptr(dev_error), ws, nbytes, stream)
     if st:
-        _lib.check(st, "cvsa_chunk_attend")
+        _lib.check(st, call)
     return out

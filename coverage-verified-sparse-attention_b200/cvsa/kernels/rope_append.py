@@ -49,6 +49,8 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
                 start_positions: Optional[torch.Tensor] = None,
                 out: Optional[torch.Tensor] = None,
                 dev_error: Optional[torch.Tensor] = None, *,
+                k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                position_shift: Optional[torch.Tensor] = None,
                 _reserve: Optional[Callable[[], None]] = None) -> Optional[torch.Tensor]:
     """Normed and rotated queries [T, H_q, D] (None without q); keys and values are appended.
 
@@ -58,16 +60,25 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     k_norm are RMS-norm weights [D]; interleaved pairs neighbouring elements
     instead of the halves of the rotated part. start_positions and seq_ids as
     returned by / given to `reserve`. `out` may be q itself.
+
+    k_scale, v_scale [num_blocks, H_kv] float32: the scales of an 8-bit cache
+    (float8_e4m3fn pools), which the call keeps (csrc/append8.cu): a page's is the
+    least power of two, from 2^-15 to 2^7, with 448 times it at least the page's largest
+    absolute value. position_shift [num_seqs] int32 is added to a token's
+    position for the rotation: how many keys were evicted before it.
     """
     # _reserve, if given, makes the reservation when nothing can refuse the call any more
     # (it may not call an operator that packs its arguments into this thread's memory)
     dev = _lib.same_device(k, q, v, k_cache, v_cache, block_tables, context_lens, cu_tokens,
-                           cos_sin, q_norm, k_norm, seq_ids, start_positions, out, dev_error)
+                           cos_sin, q_norm, k_norm, seq_ids, start_positions, out, dev_error,
+                           k_scale, v_scale, position_shift)
     if dev != torch.cuda.current_device():  # a launch goes to the current device
         with torch.cuda.device(dev):
             return rope_append(q, k, v, k_cache, v_cache, block_tables, context_lens, cu_tokens,
                                cos_sin, q_norm, k_norm, eps, interleaved, seq_ids,
-                               start_positions, out, dev_error, _reserve=_reserve)
+                               start_positions, out, dev_error, k_scale=k_scale,
+                               v_scale=v_scale, position_shift=position_shift,
+                               _reserve=_reserve)
     T, Hkv, D = k.shape
     if v.shape != k.shape or k_cache.dim() != 4 or tuple(k_cache.shape[2:]) != (Hkv, D):
         raise ValueError("k and v must be [T, H_kv, D] with the cache's H_kv and D")
@@ -100,9 +111,16 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
         if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous():
             raise ValueError("cos_sin must be a contiguous float32 [max_positions, rot_dim]")
         pos, rot = cos_sin.shape
+    scaled = k_scale is not None
+    if scaled != (v_scale is not None):
+        raise ValueError("k_scale and v_scale go together")
+    if position_shift is not None and (
+            position_shift.dtype is not torch.int32 or not position_shift.is_contiguous()
+            or position_shift.shape != context_lens.shape):
+        raise ValueError("position_shift must be a contiguous int32 [num_seqs]")
     ks, vs, mem = k.stride(), v.stride(), _lib.ARGS
     try:
-        mem.pack_rope(mem.buf, 0, *_lib.kv_fields(k_cache, v_cache),
+        mem.pack_rope(mem.buf, 0, *_lib.kv_fields(k_cache, v_cache, scaled),
                       *_lib.ragged_fields(T, cu_tokens, block_tables, context_lens, seq_ids,
                                           start_positions),
                       qp, k.data_ptr(), v.data_ptr(), op, _lib.dtype_code(k.dtype), Hq,
@@ -113,6 +131,16 @@ def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
     except (struct.error, OverflowError) as e:
         raise ValueError(f"rope_append: an argument is out of range ({e})") from None
     lib = _lib.load()
+    if scaled or position_shift is not None:
+        args = (mem.kv, _lib.scale_ptr(k_scale, k_cache, "k_scale"),
+                _lib.scale_ptr(v_scale, k_cache, "v_scale"), mem.rg, mem.rope,
+                _lib.ptr(position_shift))
+        if _reserve is not None:
+            _lib.check(lib.cvsa_rope_append_to_check(*args), "cvsa_rope_append_to")
+            _reserve()
+        _lib.check(lib.cvsa_rope_append_to(*args, _lib.ptr(dev_error), _lib.raw_stream(dev)),
+                   "cvsa_rope_append_to")
+        return out
     if _reserve is not None:
         _lib.check(lib.cvsa_rope_append_check(mem.kv, mem.rg, mem.rope), "cvsa_rope_append")
         _reserve()

@@ -15,6 +15,8 @@ from typing import Optional
 import torch
 
 from cvsa import _lib
+from cvsa.kernels.evict import evict
+from cvsa.kernels.rope_append import rope_append
 
 
 @dataclass
@@ -28,7 +30,13 @@ class CacheConfig:
 
 
 class PagedKVCache:
-    """Paged KV pool with a device free list."""
+    """Paged KV pool with a device free list.
+
+    dtype torch.float8_e4m3fn makes an 8-bit cache: k_scale and v_scale
+    [num_blocks, H_kv] hold a power of two for each page and KV head, a value is
+    its code times its page's scale. It is filled by `rope_append` (a manager's
+    appends, `ChunkedAttention`) and read by `chunk_attention`; the page-sparse
+    decode step reads 16- and 32-bit caches."""
 
     def __init__(self, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
                  dtype: torch.dtype = torch.bfloat16, device: str = "cuda",
@@ -43,6 +51,10 @@ class PagedKVCache:
                                    device=device)
         self.v_cache = torch.zeros(num_blocks, block_size, num_kv_heads, head_dim, dtype=dtype,
                                    device=device)
+        self.k_scale = self.v_scale = None
+        if dtype is torch.float8_e4m3fn:
+            self.k_scale = torch.ones(num_blocks, num_kv_heads, device=device)
+            self.v_scale = torch.ones(num_blocks, num_kv_heads, device=device)
         if free_list is None:
             free_list = torch.arange(num_blocks, dtype=torch.int32)
         if free_list.numel() != num_blocks:
@@ -65,14 +77,20 @@ class PagedKVCache:
         self.free_head += n
         return ids
 
+    def _whole_values(self, what: str):
+        if self.k_scale is not None:
+            raise ValueError(f"{what}: an 8-bit cache is written by rope_append only")
+
     def write_kv(self, block_id: int, token_offset: int, k: torch.Tensor, v: torch.Tensor):
         """k, v: [num_kv_heads, head_dim] (kv_cache.py:64-71)."""
+        self._whole_values("write_kv")
         self.k_cache[block_id, token_offset] = k
         self.v_cache[block_id, token_offset] = v
 
     def write_kv_block(self, block_id: int, k_block: torch.Tensor, v_block: torch.Tensor,
                        n_tokens: int):
         """k_block, v_block: [n_tokens, num_kv_heads, head_dim] (kv_cache.py:73-80)."""
+        self._whole_values("write_kv_block")
         self.k_cache[block_id, :n_tokens] = k_block[:n_tokens]
         self.v_cache[block_id, :n_tokens] = v_block[:n_tokens]
 
@@ -120,6 +138,9 @@ class SequenceKVManager:
         self.context_lens = torch.zeros(batch_size, dtype=torch.int32, device=dev)
         self.pages_allocated = torch.zeros(batch_size, dtype=torch.int32, device=dev)
         self._seq_ids = torch.arange(batch_size, dtype=torch.int32, device=dev)
+        # keys evicted from each sequence so far (None: this manager never evicted)
+        self.evicted = None
+        self._evict_plan = {}
 
     @property
     def _pages_allocated(self):
@@ -127,6 +148,7 @@ class SequenceKVManager:
 
     def prefill_kv(self, seq_idx: int, k_all: torch.Tensor, v_all: torch.Tensor):
         """Store prefill K/V [seq_len, num_kv_heads, head_dim] for one sequence."""
+        self.cache._whole_values("prefill_kv")
         seq_len = k_all.shape[0]
         n_pages = (seq_len + self.block_size - 1) // self.block_size
         if n_pages > self.max_pages:
@@ -146,6 +168,8 @@ class SequenceKVManager:
         self.cache.v_cache.index_copy_(0, idx, vv.view(shp).to(self.cache.v_cache.dtype))
         self.context_lens[seq_idx] = seq_len
         self.pages_allocated[seq_idx] = n_pages
+        if self.evicted is not None:
+            self.evicted[seq_idx] = 0
 
     def append_token_kv(self, seq_idx: int, k: torch.Tensor, v: torch.Tensor):
         """Append one decode token's K/V [num_kv_heads, head_dim] to one sequence."""
@@ -194,8 +218,66 @@ class SequenceKVManager:
                 starts.data_ptr(), c.dev_error.data_ptr(), _lib.stream_ptr(dev)),
                 "cvsa_paged_reserve")
 
+    def track_evictions(self) -> torch.Tensor:
+        """Count evicted keys from now on: `evicted` [batch_size], which `ChunkedAttention`
+        adds to new tokens' positions. The first `evict` does it too; call it before a
+        graph is captured that is to see later evictions."""
+        if self.evicted is None:
+            self.evicted = torch.zeros_like(self.context_lens)
+        return self.evicted
+
+    def evict(self, weights: torch.Tensor, keep: int, sink: int = 0,
+              recent: int = 0) -> torch.Tensor:
+        """Cut every sequence longer than `keep` to its `keep` keys of most weight per KV head.
+
+        weights [batch_size, num_kv_heads, >= max_pages * block_size] float32
+        (`cvsa.kernels.key_weights`) moves along. Of each head the first `sink`
+        and the last `recent` keys stay in any case. Old pages go back to the
+        pool; pages for the kept keys are taken from it first, and a sequence that it
+        has none for stays as it is (`cache.check()` raises). Returns the kept
+        keys [batch_size, num_kv_heads, keep], -1 for sequences that were not
+        cut. Keys keep the rotation of their first position; `evicted` counts
+        what went, for the positions of new tokens. Nothing synchronises."""
+        c = self.cache
+        dev = _lib.require_cuda(weights, c.k_cache)
+        if not 0 < keep <= self.max_pages * self.block_size:
+            raise ValueError("keep must be positive and fit the block table")
+        pages = -(-keep // self.block_size)
+        plan = self._evict_plan.get(pages)
+        if plan is None:
+            i32 = torch.int32
+            plan = (torch.empty((self.batch_size, pages), dtype=i32, device=dev),
+                    torch.empty((self.batch_size,), dtype=i32, device=dev))
+            self._evict_plan[pages] = plan
+        new_tables, lens = plan
+        args = _lib.EvictPages(
+            self.block_tables.data_ptr(), self.context_lens.data_ptr(),
+            self.pages_allocated.data_ptr(), self.track_evictions().data_ptr(),
+            c.free_list.data_ptr(), c.free_head.data_ptr(), new_tables.data_ptr(),
+            lens.data_ptr(), self.batch_size, self.max_pages, self.block_size, keep,
+            c.free_list.numel())
+        lib, err = _lib.load(), c.dev_error.data_ptr()
+        with torch.cuda.device(dev):  # a launch goes to the current device
+            stream = _lib.stream_ptr(dev)
+            # changes nothing but the plan, so that the next call may still refuse
+            _lib.check(lib.cvsa_evict_reserve(args, err, stream), "cvsa_evict_reserve")
+            kept = evict(c.k_cache, c.v_cache, self.block_tables, lens, weights, new_tables,
+                         keep, sink, recent, dev_error=c.dev_error, k_scale=c.k_scale,
+                         v_scale=c.v_scale)
+            _lib.check(lib.cvsa_evict_commit(args, err, stream), "cvsa_evict_commit")
+        return kept
+
     def _append(self, k, v, ids):
         c = self.cache
+        if c.k_scale is not None:
+            _lib.require_cuda(k, v, c.k_cache)
+            cu = torch.arange(k.shape[0] + 1, dtype=torch.int32, device=k.device)
+            ids, starts = ids.contiguous(), torch.empty_like(ids)
+            rope_append(None, k, v, c.k_cache, c.v_cache, self.block_tables, self.context_lens,
+                        cu, seq_ids=ids, start_positions=starts, dev_error=c.dev_error,
+                        k_scale=c.k_scale, v_scale=c.v_scale,
+                        _reserve=lambda: self._reserve(cu, ids, starts))
+            return
         _lib.require_cuda(k, v, c.k_cache)
         k = k.to(c.k_cache.dtype).contiguous()
         v = v.to(c.v_cache.dtype).contiguous()

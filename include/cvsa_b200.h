@@ -45,7 +45,8 @@ extern "C" {
 enum {
   CVSA_DTYPE_F32 = 0,
   CVSA_DTYPE_F16 = 1,
-  CVSA_DTYPE_BF16 = 2
+  CVSA_DTYPE_BF16 = 2,
+  CVSA_DTYPE_E4M3 = 3 /* 8-bit floats; the pools of the calls that take scales */
 };
 
 /* status codes */
@@ -624,6 +625,112 @@ size_t cvsa_chunk_attend_workspace_size(const cvsa_kv_desc_t* kv, const cvsa_rag
 int cvsa_chunk_attend(const cvsa_kv_desc_t* kv, const cvsa_ragged_desc_t* rg,
                       const cvsa_chunk_attend_t* args, int32_t* dev_error, void* workspace,
                       size_t workspace_bytes, void* stream);
+
+/* ---- the 8-bit cache ---------------------------------------------------
+ * Pools of CVSA_DTYPE_E4M3 have a scale for each page and KV head, keys and
+ * values apart: k_scale, v_scale [num_blocks, num_kv_heads] float32. A value is
+ * its code times its page's scale. Scales are powers of two from 2^-15 to 2^7
+ * (the append writes them), so every value is an f16 and a bf16 number exactly.
+ * The reference has no counterpart. */
+
+/* cvsa_rope_append into pools of 8 bits (or, with NULL scales, of any other
+ * type). A page that begins with these tokens gets the least scale that holds
+ * their largest absolute value (infinities do not count and saturate); a page
+ * that holds tokens keeps its scale or moves to the larger one with the codes in
+ * use. Rounded once. position_shift (nullable) [num_seqs], by table row, is added
+ * to a token's position for the rotation (what was evicted before it). */
+int cvsa_rope_append_to(const cvsa_kv_desc_t* kv, float* k_scale, float* v_scale,
+                        const cvsa_ragged_desc_t* rg, const cvsa_rope_append_t* args,
+                        const int32_t* position_shift, int32_t* dev_error, void* stream);
+int cvsa_rope_append_to_check(const cvsa_kv_desc_t* kv, const float* k_scale,
+                              const float* v_scale, const cvsa_ragged_desc_t* rg,
+                              const cvsa_rope_append_t* args, const int32_t* position_shift);
+
+/* cvsa_chunk_attend over pools of 8 bits: the same values as over a 16-bit or
+ * float32 pool that holds code times scale. */
+int cvsa_chunk_attend_q8_check(const cvsa_kv_desc_t* kv, const float* k_scale,
+                               const float* v_scale, const cvsa_ragged_desc_t* rg,
+                               const cvsa_chunk_attend_t* args);
+size_t cvsa_chunk_attend_q8_workspace_size(const cvsa_kv_desc_t* kv, const float* k_scale,
+                                           const float* v_scale, const cvsa_ragged_desc_t* rg,
+                                           const cvsa_chunk_attend_t* args);
+int cvsa_chunk_attend_q8(const cvsa_kv_desc_t* kv, const float* k_scale, const float* v_scale,
+                         const cvsa_ragged_desc_t* rg, const cvsa_chunk_attend_t* args,
+                         int32_t* dev_error, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* ---- eviction by accumulated attention weight -------------------------- */
+
+typedef struct cvsa_key_weights {
+  const void* q;          /* [num_tokens, num_q_heads, head_dim], as given to the attention */
+  const float* lse;       /* [num_tokens, num_q_heads], the attention's */
+  int32_t dtype;
+  int32_t num_q_heads;
+  int64_t q_stride_token, q_stride_head;
+  float scale;            /* > 0, finite */
+  float decay;            /* >= 0, finite */
+  int32_t causal, window; /* as in cvsa_chunk_attend_t */
+  const float* prior;     /* [num_seqs, num_kv_heads, weights_stride]: weights so far */
+  float* out;             /* the same shape; may be prior */
+  int64_t weights_stride; /* >= max_pages * block_size */
+} cvsa_key_weights_t;
+
+/* What each cached key of the batch's sequences got of the new tokens' attention:
+ * out = decay * prior + sum of e^(scale q.k - lse) over the rows of its KV head's
+ * group that see it. Keys from a sequence's start position on (the new tokens'
+ * own) start from 0. Keys past a context, and sequences that were refused or have
+ * no table row, are not written. k_scale: of 8-bit pools, else NULL. v_cache of
+ * the descriptor is not read. fp32 sums in a fixed order. */
+int cvsa_key_weights(const cvsa_kv_desc_t* kv, const float* k_scale,
+                     const cvsa_ragged_desc_t* rg, const cvsa_key_weights_t* args,
+                     int32_t* dev_error, void* stream);
+int cvsa_key_weights_check(const cvsa_kv_desc_t* kv, const float* k_scale,
+                           const cvsa_ragged_desc_t* rg, const cvsa_key_weights_t* args);
+
+typedef struct cvsa_evict {
+  const float* weights;      /* [num_seqs, num_kv_heads, weights_stride] */
+  int64_t weights_stride;    /* >= max_pages * block_size */
+  float* out_weights;        /* [num_seqs, num_kv_heads, out_stride]; may be weights */
+  int64_t out_stride;        /* >= keep */
+  const int32_t* new_tables; /* [num_seqs, new_pages]: pages to move to, not in use */
+  int32_t new_pages;         /* pages that `keep` tokens take */
+  int32_t* kept;             /* [num_seqs, num_kv_heads, keep] out: the kept keys */
+  int32_t keep, sink, recent;
+} cvsa_evict_t;
+
+/* For every sequence longer than `keep`, and each KV head: the first `sink` keys,
+ * the last `recent` and the keep - sink - recent of largest weight between (equal
+ * weights: the earlier; NaN below everything), in their order, go to kept, their
+ * weights to out_weights, their keys and values to new_tables' pages. In 8-bit
+ * pools a new page's scale is the largest of its rows'. Rows of kept are -1 for
+ * shorter sequences, of which nothing else is written. Tables and lengths are
+ * the caller's to change (cvsa_evict_commit). */
+int cvsa_evict(const cvsa_kv_desc_t* kv, float* k_scale, float* v_scale,
+               const int32_t* block_tables, const int32_t* context_lens, int32_t num_seqs,
+               int32_t max_pages, const cvsa_evict_t* args, int32_t* dev_error, void* stream);
+
+typedef struct cvsa_evict_pages {
+  int32_t* block_tables;     /* [num_seqs, max_pages] */
+  int32_t* context_lens;     /* [num_seqs] */
+  int32_t* pages_allocated;  /* [num_seqs] */
+  int32_t* evicted;          /* [num_seqs]: keys evicted so far (position_shift) */
+  int32_t* free_list;
+  int32_t* free_head;
+  int32_t* new_tables;       /* [num_seqs, pages of keep] */
+  int32_t* plan_lens;        /* [num_seqs] */
+  int32_t num_seqs, max_pages, block_size, keep, free_list_len;
+} cvsa_evict_pages_t;
+
+/* The pages around cvsa_evict. reserve: every sequence longer than `keep` gets the
+ * pages for `keep` tokens at the head of the free list, in order, in new_tables
+ * (-1 for others); plan_lens is its length (0 for others), to be cvsa_evict's
+ * context_lens. A sequence that the list has no pages for is left as it is
+ * (CVSA_DEV_ERR_POOL). Nothing else changes before commit, which makes new_tables
+ * the sequences' tables, gives their old pages back to the list, and sets
+ * lengths, pages_allocated and evicted. Both on one stream, with the same
+ * arguments and nothing between that takes pages. */
+int cvsa_evict_reserve(const cvsa_evict_pages_t* args, int32_t* dev_error, void* stream);
+int cvsa_evict_commit(const cvsa_evict_pages_t* args, int32_t* dev_error, void* stream);
 
 /* ---- allocation-free decode ------------------------------------------ */
 
