@@ -151,8 +151,8 @@ chunk_general_kernel(const __grid_constant__ GenArgs a) {
         off = ok ? blk * a.kv.sb + (key % a.kv.bs) * a.kv.st + it.h * a.kv.sh : 0;
         if constexpr (sizeof(C) == 1) {
           const int64_t at = (int64_t)blk * a.kv.hkv + it.h;
-          sm.k_scale[k & 1][tid] = ok ? a.kv.ks[at] : 0.f;
-          sm.v_scale[k & 1][tid] = ok ? a.kv.vs[at] : 0.f;
+          sm.k_scale[k & 1][tid] = ok ? pow2(scale_exponent_of(a.kv.ks[at])) : 0.f;
+          sm.v_scale[k & 1][tid] = ok ? pow2(scale_exponent_of(a.kv.vs[at])) : 0.f;
         }
       }
       sm.key_off[k & 1][tid] = off;

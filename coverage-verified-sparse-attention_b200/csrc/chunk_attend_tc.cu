@@ -1,5 +1,5 @@
 // Attention of a ragged batch of new tokens over the paged cache on the tensor
-// cores: 16-bit pools of q's dtype, head_dim 64 or 128. Formulas as in
+// cores: 16-bit pools of q's dtype or 8-bit pools, head_dim 64 or 128. Formulas as in
 // chunk_attend.cu, work split as in chunk_plan.cuh.
 //
 // A persistent CTA an SM. An item's query rows (token, head of the group) are
@@ -61,6 +61,7 @@
 #include "cvsa_common.cuh"
 #include "cvsa_internal.h"
 #include "cvsa_launch.cuh"
+#include "fp8.cuh"
 #include "tcgen05.cuh"
 
 namespace cvsa {
@@ -87,6 +88,8 @@ struct Cfg {
   static_assert(kTile == kKT, "Q tiles and KV tiles share the copy code");
   static constexpr int kRing = 2 * kQTile;              // offset of the ring
   static constexpr int kMeta = kRing + kStages * kStage;
+  // 8-bit pools: a K and a V tile's codes, 128-byte lines of 8 lanes
+  static constexpr int kRaw8 = kKT * D;
 };
 
 // What the roles need of an item.
@@ -103,20 +106,24 @@ struct ItemRec {
 constexpr int kItems = 4;
 constexpr int kPairRows = 64;  // rows whose fp32 O fits the second Q tile's memory
 
-struct TcMeta {
+struct alignas(8) TcMeta {
   uint64_t kv_full[8], kv_empty[8];
   uint64_t q_full, q_empty;
+  uint64_t q_ready[2];                  // Q tiles that are scaled first: they were
   uint64_t s_full[2], s_free[2], p_half[2], p_full[2], o_full[2];  // per slot
   uint64_t it_full[kItems], it_empty[kItems];
   uint64_t joined, join_free;           // paired items: slot 1's part is there; was read
   uint64_t drain[2];
   uint32_t key_bad[kSlots][4];  // per tile (mod kSlots): bit per key no row may see
-  uint32_t v_odd[kSlots][4];    // per tile and loading warp: a V value is not finite
+  uint8_t v_odd[kSlots][4];     // per tile and loading warp: a V value is not finite
   ItemRec item[kItems];
   float pair_m[kPairRows], pair_l[kPairRows];
+  int8_t pair_exp[kPairRows];   // rows' powers of two (scale_query)
   uint32_t tmem;
   uint32_t abort;
 };
+
+constexpr int kMetaBytes = ((int)sizeof(TcMeta) + 15) / 16 * 16;
 
 struct TcArgs {
   RaggedView rg;
@@ -183,7 +190,7 @@ __device__ __forceinline__ bool tile_partial(const ItemRec& it, int base) {
 }
 
 __device__ __forceinline__ uint32_t any_odd(const TcMeta* m, uint32_t slot) {
-  return m->v_odd[slot][0] | m->v_odd[slot][1] | m->v_odd[slot][2] | m->v_odd[slot][3];
+  return *reinterpret_cast<const uint32_t*>(m->v_odd[slot]);
 }
 
 // A role's side of the item records. `next` is false at the end (or after a
@@ -424,6 +431,167 @@ struct Loader {
   }
 };
 
+// 8-bit pools. A tile's codes are copied (asynchronously) to a buffer of their own, one
+// for K and one for V, and widened from there to the 16-bit tile: each thread widens
+// the pieces that it copied, so it waits for nobody's copies but its own. V of one tile
+// is on its way while K of another is widened, and the other way round.
+//
+// The tensor cores take f16 whatever the queries' type: an instruction widens two codes
+// to f16, where bf16 takes thirteen for four (1024 tokens at 32K keys 975 us in bf16,
+// 739 in f16), and the weights keep 11 bits. Widening is exact (fp8.cuh). bf16 queries
+// are scaled by row (scale_query).
+template <int D>
+struct Loader8 : Loader<__half, D> {
+  using T = __half;
+  using L = Loader<T, D>;
+  using C = Cfg<D>;
+  using L::a; using L::m; using L::base; using L::w; using L::lane;
+  static constexpr int kCh = D / 16;           // 16-byte pieces of a row's codes
+  static constexpr int kRPI = 32 / kCh;        // rows a warp instruction
+  static constexpr int kPieces = 32 / kRPI;    // pieces a lane of a tile
+  uint32_t raw;                                // this thread's pieces: 512 bytes apart
+
+  __device__ Loader8(const TcArgs& a_, TcMeta* m_, uint32_t base_, uint32_t raw_, int w_, int lane_)
+      : L(a_, m_, base_, w_, lane_), raw(raw_ + w_ * kPieces * 512 + lane_ * 16) {}
+
+  // Lane i's row is off bytes into the pool (< 0: zeros); v: the V tile's buffer.
+  __device__ __forceinline__ void fetch(const void* src, int64_t off, int v) {
+    const int ch = lane % kCh;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int64_t o = __shfl_sync(0xffffffffu, off, i * kRPI + lane / kCh);
+      cp16(raw + v * C::kRaw8 + i * 512, static_cast<const char*>(src) + (o < 0 ? 0 : o + ch * 16),
+           o >= 0);
+    }
+    cp_async_commit();
+  }
+  // To the 16-bit tile; lane i holds row i's factor. Whether a code was NaN, if asked.
+  __device__ __forceinline__ bool widen(uint32_t tile, uint32_t factor, int v, bool ask) {
+    const int ch = lane % kCh;
+    const bool swap = ch >= 4;  // the two stores of a row's lanes then fall on different banks
+    bool nan = false;
+#pragma unroll 2
+    for (int i = 0; i < kPieces; ++i) {
+      const int r = i * kRPI + lane / kCh;
+      uint4 codes, x[2];
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(codes.x), "=r"(codes.y), "=r"(codes.z), "=r"(codes.w)
+                   : "r"(raw + v * C::kRaw8 + i * 512));
+      widen16(codes, __shfl_sync(0xffffffffu, factor, r), x);
+      if (ask) nan |= any_nan8(codes);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int e = swap ? 1 - half : half;
+        const uint4 y = e ? x[1] : x[0];
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(
+                         this->dst(tile, w * 32 + r, ch * 2 + e)),
+                     "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w)
+                     : "memory");
+      }
+    }
+    return ask && __any_sync(0xffffffffu, nan);
+  }
+
+  __device__ void run() {
+    ItemReader items(m, a);
+    uint32_t op = 0, tiles = 0, loads = 0, joins = 0;
+    const int G = a.g.G;
+    while (const ItemRec* it = items.next()) {
+      const int nt = it->nt;
+      if (nt == 0) {
+        items.done();
+        continue;
+      }
+      const int lag = it->pair ? 2 : 1;
+      const int lo = it->lo, hi = it->hi, h = it->h;
+      const int32_t* table = a.rg.tables + (int64_t)it->slot * a.rg.W;
+      auto block_of = [&](int key) {  // only of an item key
+        return key >= lo && key < hi ? table[a.bs_shift >= 0 ? key >> a.bs_shift : key / a.kv.bs]
+                                     : -1;
+      };
+      int key = it->kbase + w * 32 + lane;  // of the tile that is located next
+      int blk = block_of(key);
+      // rows and V factors of tiles j, j - 1, j - 2 at turn j; K's factor of tile j
+      int64_t off[4] = {-1, -1, -1, -1};
+      uint32_t fv[4] = {0, 0, 0, 0}, fk = 0;
+      // Finds tile j's rows and starts its K copies; the others move up.
+      auto locate = [&]() {
+#pragma unroll
+        for (int i = 3; i > 0; --i) off[i] = off[i - 1], fv[i] = fv[i - 1];
+        const int next = block_of(key + kKT);
+        off[0] = -1;
+        fk = fv[0] = 0;
+        if (key >= lo && key < hi) {
+          if (blk >= 0 && blk < a.kv.num_blocks) {
+            const int in = a.bs_shift >= 0 ? key & (a.kv.bs - 1) : key % a.kv.bs;
+            off[0] = blk * a.kv.sb + in * a.kv.st + h * a.kv.sh;
+            const int64_t at = (int64_t)blk * a.kv.hkv + h;
+            fk = widen_factor(a.kv.ks[at]);
+            fv[0] = widen_factor(a.kv.vs[at]);
+          } else {
+            set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);
+          }
+        }
+        blk = next;
+        key += kKT;
+        fetch(a.kv.k, off[0], 0);
+      };
+      locate();
+      for (int j = 0; j < nt + lag; ++j) {
+        // before tile j + 1 is located its predecessors are at 0, 1, ...; from nt on
+        // nothing is located, so tile j - lag stays where it was at turn nt - 1
+        const int back = lag - max(0, j - (nt - 1));
+        const uint32_t fvj = back == 0 ? fv[0] : back == 1 ? fv[1] : fv[2];
+        if (j >= lag) fetch(a.kv.v, back == 0 ? off[0] : back == 1 ? off[1] : off[2], 1);
+        if (j < nt) {
+          const uint32_t st = op % C::kStages, slot = (tiles + j) % kSlots;
+          if (!warp_wait(&m->kv_empty[st], ((op / C::kStages) & 1) ^ 1, m, a)) goto out;
+          const uint32_t bad = __ballot_sync(0xffffffffu, off[0] < 0);
+          if (lane == 0) m->key_bad[slot][w] = bad;
+          cp_async_wait_dyn(j >= lag ? 1 : 0);
+          widen(base + C::kRing + st * C::kStage, fk, 0, false);
+          mbar_arrive(&m->kv_full[st]);
+          if (lane == 0) mbar_arrive(&m->kv_full[st]);
+          ++op;
+          if (j + 1 < nt) locate();
+        }
+        if (j == lag - 1) {
+          // the queries; a group of their own behind the K tile on its way
+          if (!warp_wait(&m->q_empty, (loads & 1) ^ 1, m, a)) goto out;
+          ++loads;
+          if (joins && !warp_wait(&m->join_free, (joins - 1) & 1, m, a)) goto out;
+          joins += it->pair;
+          for (int q = 0; q < it->nq; ++q) {
+            const int r = w * 32 + lane;
+            const int rows = min(a.TQ, it->ntok - q * a.TQ) * G;
+            int64_t qo = -1;
+            if (r < rows)
+              qo = (int64_t)(it->tok + q * a.TQ + r / G) * a.c.q_st +
+                   (int64_t)(h * G + r % G) * a.c.q_sh;
+            this->copy_rows(base + q * C::kQTile, a.c.q, qo);
+          }
+          arrive_when_landed(&m->q_full);
+        }
+        if (j >= lag) {
+          const uint32_t st = op % C::kStages, slot = (tiles + j - lag) % kSlots;
+          if (!warp_wait(&m->kv_empty[st], ((op / C::kStages) & 1) ^ 1, m, a)) goto out;
+          cp_async_wait_dyn(j + 1 < nt ? 1 : 0);
+          const bool partial = tile_partial(*it, it->kbase + (j - lag) * kKT);
+          const bool odd = widen(base + C::kRing + st * C::kStage, fvj, 1, partial);
+          if (partial && lane == 0) m->v_odd[slot][w] = odd;
+          mbar_arrive(&m->kv_full[st]);
+          if (lane == 0) mbar_arrive(&m->kv_full[st]);
+          ++op;
+        }
+      }
+      tiles += nt;
+      items.done();
+    }
+  out:
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+};
+
 // ---------------------------------------------------------------------------
 // MMA issue (a warp a slot, one elected lane)
 // ---------------------------------------------------------------------------
@@ -433,7 +601,7 @@ struct Loader {
 // of moves, against the 64 that it runs.
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
-template <typename T, int D>
+template <typename T, int D, bool kScaled>
 __device__ __forceinline__ void mma_role(const TcArgs& a, TcMeta* m, uint32_t base, uint32_t tmem,
                                          const int s) {
   using C = Cfg<D>;
@@ -458,7 +626,7 @@ __device__ __forceinline__ void mma_role(const TcArgs& a, TcMeta* m, uint32_t ba
   // a barrier's parity says which of two phases is done, so no one may lag or
   // lead by more.
   ItemReader items(m, a);
-  uint32_t op = 0, tiles = 0, loads = 0;
+  uint32_t op = 0, tiles = 0, loads = 0, second = 0;
   uint32_t turn = 0;  // tiles of this slot before this item
   while (const ItemRec* it = items.next()) {
     const int nt = uniform(it->nt), nq = uniform(it->nq), kbase = uniform(it->kbase);
@@ -469,6 +637,11 @@ __device__ __forceinline__ void mma_role(const TcArgs& a, TcMeta* m, uint32_t ba
     }
     const int n = pair ? (nt + 1 - s) / 2 : s < nq ? nt : 0;  // tiles of this slot
     if (!warp_wait(&m->q_full, loads & 1, m, a)) break;
+    if (kScaled && n > 0) {
+      const bool one = s == 1 && !pair;  // the second Q tile
+      if (!warp_wait(&m->q_ready[one], (one ? second : loads) & 1, m, a)) break;
+      second += one;
+    }
     ++loads;
     if (n == 0 && elect_one()) mbar_arrive(&m->q_empty);
     const uint64_t qd = q_desc + (((pair ? 0 : s) * C::kQTile) >> 4);
@@ -584,19 +757,64 @@ __device__ __forceinline__ void transpose4(uint4* x) {
   }
 }
 
-template <typename T, int D>
+// bf16 queries for f16 tensor cores, one row a thread, in place: each row is brought to
+// a largest value in [2^13, 2^14) by a power of two, 2^-e of which is returned as e and
+// goes to the row's softmax scale. bf16's 8 bits fit f16's 11 down to 2^-27 of the
+// largest; what lies below errs by at most 2^-38 of it, far below the rounding of a
+// product's sum. (Where a row holds an infinity, its scores are that or NaN whatever
+// its other values are.)
+template <typename TI, int D>
+__device__ __forceinline__ int scale_query(uint32_t tile, int row) {
+  constexpr int kPanel = Cfg<D>::kPanel;
+  auto at = [&](int ch) {
+    return tile + (ch >> 3) * kPanel + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+  };
+  auto load = [&](int ch, float* f) {
+    uint4 x;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                 : "r"(at(ch)));
+    Vec16<TI>::unpack(x, f);
+  };
+  float top = 0.f;
+#pragma unroll 2
+  for (int ch = 0; ch < D / 8; ++ch) {
+    float f[8];
+    load(ch, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+  }
+  const int up = min(120, 13 + 127 - (__float_as_int(top) >> 23));  // >= -115
+  const float by = pow2(up);
+#pragma unroll 2
+  for (int ch = 0; ch < D / 8; ++ch) {
+    float f[8];
+    load(ch, f);
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at(ch)),
+                 "r"(Mma<__half>::pack(f[0] * by, f[1] * by)),
+                 "r"(Mma<__half>::pack(f[2] * by, f[3] * by)),
+                 "r"(Mma<__half>::pack(f[4] * by, f[5] * by)),
+                 "r"(Mma<__half>::pack(f[6] * by, f[7] * by))
+                 : "memory");
+  }
+  return -up;
+}
+
+template <typename TI, typename T, int D>  // T: of the tensor cores' operands
 __device__ __forceinline__ void softmax_role(const TcArgs& a, TcMeta* m, uint32_t base,
                                              uint32_t tmem, const int g) {
   using C = Cfg<D>;
   constexpr float kRaise = Weight<T>::kRaise, kUp = Weight<T>::kUp;
+  constexpr bool kScaled = !std::is_same<TI, T>::value;
   const int r = threadIdx.x & 127, warp = r >> 5;
   const uint32_t lanes = (uint32_t)(warp * 32) << 16;
   const uint32_t ts = tmem + g * kKT + lanes, to = tmem + 2 * kKT + g * D + lanes;
   const int G = a.g.G;
-  const float scale2 = a.scale2;
+  float scale2 = a.scale2;
   ItemReader items(m, a);
-  uint32_t op = 0, tiles = 0, turn = 0, ends = 0, joins = 0;
+  uint32_t op = 0, tiles = 0, turn = 0, ends = 0, joins = 0, loads = 0;
   while (const ItemRec* it = items.next()) {
+    loads += it->nt > 0;
     const int nt = it->nt, pair = it->pair, q = pair ? 0 : g, step = pair ? 2 : 1;
     const int rows = min(a.TQ, it->ntok - q * a.TQ) * G;
     if (rows <= 0) {
@@ -606,6 +824,15 @@ __device__ __forceinline__ void softmax_role(const TcArgs& a, TcMeta* m, uint32_
       continue;
     }
     const bool active = warp * 32 < rows;
+    if (kScaled && nt > 0 && !(pair && g == 1)) {
+      if (!warp_wait(&m->q_full, (loads - 1) & 1, m, a)) return;
+      if (active) {
+        const int e = scale_query<TI, D>(base + g * C::kQTile, r);
+        scale2 = a.scale2 * pow2(e);
+        if (pair && r < kPairRows) m->pair_exp[r] = (int8_t)e;  // for the other slot's softmax
+      }
+      mbar_arrive(&m->q_ready[g]);
+    }
     const int pos = it->pos0 + q * a.TQ + r / G;
     const int hi = a.g.causal ? min(it->ctx, pos + 1) : it->ctx;
     const int lo = a.g.window > 0 ? pos - a.g.window + 1 : 0;
@@ -614,6 +841,7 @@ __device__ __forceinline__ void softmax_role(const TcArgs& a, TcMeta* m, uint32_
     for (int j = first; j < nt; j += step, ++turn) {
       if (!warp_wait(&m->s_full[g], turn & 1, m, a)) return;
       tc_fence_after();
+      if (kScaled && j == 1 && first == 1 && r < kPairRows) scale2 = a.scale2 * pow2(m->pair_exp[r]);
       const int kbase = it->kbase + j * kKT;
       const uint32_t slot = (tiles + j) % kSlots;
       const bool partial = tile_partial(*it, kbase);
@@ -832,10 +1060,10 @@ __device__ __forceinline__ void softmax_role(const TcArgs& a, TcMeta* m, uint32_
       const int R = 2 * kTile, rr = q * a.TQ * G + r;
       float* part = a.parts + (size_t)it->pslot * chunk_slot_floats(R, D);
       const int64_t own = tok * a.c.o_st + head * a.c.o_sh;
-      T* dst[4];  // this lane's pieces of the rows of its 4 lanes
+      TI* dst[4];  // this lane's pieces of the rows of its 4 lanes
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        dst[i] = reinterpret_cast<T*>(a.c.out) + (r & 3) * 8 +
+        dst[i] = reinterpret_cast<TI*>(a.c.out) + (r & 3) * 8 +
                  __shfl_sync(0xffffffffu, own, (r & 28) + i);
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
@@ -865,10 +1093,10 @@ __device__ __forceinline__ void softmax_role(const TcArgs& a, TcMeta* m, uint32_
           uint4 x[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            x[i].x = Mma<T>::pack(o[8 * i] * inv, o[8 * i + 1] * inv);
-            x[i].y = Mma<T>::pack(o[8 * i + 2] * inv, o[8 * i + 3] * inv);
-            x[i].z = Mma<T>::pack(o[8 * i + 4] * inv, o[8 * i + 5] * inv);
-            x[i].w = Mma<T>::pack(o[8 * i + 6] * inv, o[8 * i + 7] * inv);
+            x[i].x = Mma<TI>::pack(o[8 * i] * inv, o[8 * i + 1] * inv);
+            x[i].y = Mma<TI>::pack(o[8 * i + 2] * inv, o[8 * i + 3] * inv);
+            x[i].z = Mma<TI>::pack(o[8 * i + 4] * inv, o[8 * i + 5] * inv);
+            x[i].w = Mma<TI>::pack(o[8 * i + 6] * inv, o[8 * i + 7] * inv);
           }
           transpose4(x);
 #pragma unroll
@@ -908,10 +1136,11 @@ __device__ __forceinline__ void softmax_role(const TcArgs& a, TcMeta* m, uint32_
   }
 }
 
-template <typename T, int D>
+template <typename TI, int D, bool F8>  // the queries' type; F8: an 8-bit pool
 __global__ void __launch_bounds__(kThreads, 1)
 chunk_tc_kernel(const __grid_constant__ TcArgs a) {
   using C = Cfg<D>;
+  using T = typename std::conditional<F8, __half, TI>::type;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -924,6 +1153,7 @@ chunk_tc_kernel(const __grid_constant__ TcArgs a) {
     }
     mbar_init(&m->q_full, 128);
     mbar_init(&m->q_empty, 2);
+    for (int i = 0; i < 2; ++i) mbar_init(&m->q_ready[i], 128);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&m->s_full[i], 2);
       mbar_init(&m->s_free[i], 128);
@@ -955,13 +1185,16 @@ chunk_tc_kernel(const __grid_constant__ TcArgs a) {
   const uint32_t base = smem_u32(smem), tmem = __shfl_sync(0xffffffffu, m->tmem, 0);
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-    softmax_role<T, D>(a, m, base, tmem, warp / 4);
+    softmax_role<TI, T, D>(a, m, base, tmem, warp / 4);
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    Loader<T, D>(a, m, base, warp - 8, lane).run();
+    if constexpr (F8)
+      Loader8<D>(a, m, base, base + C::kMeta + kMetaBytes, warp - 8, lane).run();
+    else
+      Loader<T, D>(a, m, base, warp - 8, lane).run();
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 12 || warp == 14) mma_role<T, D>(a, m, base, tmem, (warp - 12) / 2);
+    if (warp == 12 || warp == 14) mma_role<T, D, F8 && !std::is_same<TI, T>::value>(a, m, base, tmem, (warp - 12) / 2);
     if (warp == 13) item_role(a, m, rng);
     __syncwarp();
   }
@@ -973,22 +1206,28 @@ chunk_tc_kernel(const __grid_constant__ TcArgs a) {
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool F8>
 cudaError_t launch_tc(const TcArgs& a, int ctas, cudaStream_t s) {
   using C = Cfg<D>;
-  constexpr int kSmem = C::kMeta + (int)sizeof(TcMeta) + 1024;
+  constexpr int kSmem = C::kMeta + (F8 ? kMetaBytes + 2 * C::kRaw8 : (int)sizeof(TcMeta)) + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory");
-  cudaError_t e = cudaFuncSetAttribute(chunk_tc_kernel<T, D>,
+  cudaError_t e = cudaFuncSetAttribute(chunk_tc_kernel<T, D, F8>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  return launch_k(chunk_tc_kernel<T, D>, dim3(ctas), dim3(kThreads), kSmem, s, true, a);
+  return launch_k(chunk_tc_kernel<T, D, F8>, dim3(ctas), dim3(kThreads), kSmem, s, true, a);
+}
+
+template <typename T, int D>
+cudaError_t launch_tc(const TcArgs& a, int ctas, cudaStream_t s) {
+  return a.kv.dtype == CVSA_DTYPE_E4M3 ? launch_tc<T, D, true>(a, ctas, s)
+                                       : launch_tc<T, D, false>(a, ctas, s);
 }
 
 }  // namespace
 
 bool chunk_tc_eligible(const KvView& kv, const ChunkView& c) {
-  return c.dtype == kv.dtype && kv.dtype != CVSA_DTYPE_F32 && (kv.d == 64 || kv.d == 128) &&
-         c.hq / kv.hkv <= kTile;
+  return (c.dtype == kv.dtype || kv.dtype == CVSA_DTYPE_E4M3) && c.dtype != CVSA_DTYPE_F32 &&
+         (kv.d == 64 || kv.d == 128) && c.hq / kv.hkv <= kTile;
 }
 
 int chunk_tc_rows() { return 2 * kTile; }
@@ -1027,7 +1266,7 @@ cudaError_t launch_chunk_tc(const KvView& kv, const RaggedView& rg, const ChunkV
   a.desc = desc;
   a.dev_err = dev_err;
   a.wait_limit = wait_limit() ? wait_limit() : 1u << 18;  // a poll waits about 4 us: a second
-  if (kv.dtype == CVSA_DTYPE_BF16)
+  if (c.dtype == CVSA_DTYPE_BF16)
     return kv.d == 64 ? launch_tc<__nv_bfloat16, 64>(a, ctas, s)
                       : launch_tc<__nv_bfloat16, 128>(a, ctas, s);
   return kv.d == 64 ? launch_tc<__half, 64>(a, ctas, s) : launch_tc<__half, 128>(a, ctas, s);

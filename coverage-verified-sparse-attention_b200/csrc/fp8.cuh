@@ -48,4 +48,29 @@ __device__ __forceinline__ int scale_exponent_of(float scale) {
   return max(kScaleMin, min(kScaleMax, e));
 }
 
+// A page's factor as two f16, for widen16, from its scale.
+__device__ __forceinline__ uint32_t widen_factor(float scale) {
+  const uint32_t h = __half_as_ushort(__float2half_rn(pow2(scale_exponent_of(scale))));  // exact
+  return h | h << 16;
+}
+
+// Whether one of 16 codes is NaN.
+__device__ __forceinline__ bool any_nan8(const uint4& c) {
+  auto top = [](uint32_t w) { return (w & 0x7f7f7f7fu) + 0x01010101u; };
+  return ((top(c.x) | top(c.y) | top(c.z) | top(c.w)) & 0x80808080u) != 0;
+}
+
+// 16 codes times their page's factor, as f16; exact.
+__device__ __forceinline__ void widen16(const uint4& codes, uint32_t factor, uint4* out) {
+  const uint32_t* c = reinterpret_cast<const uint32_t*>(&codes);
+  uint32_t* o = reinterpret_cast<uint32_t*>(out);
+  const __half2 f = *reinterpret_cast<const __half2*>(&factor);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t two = e4m3x2_to_f16x2(i & 1 ? c[i / 2] >> 16 : c[i / 2] & 0xffffu);
+    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&two), f);
+    o[i] = *reinterpret_cast<const uint32_t*>(&x);
+  }
+}
+
 }  // namespace cvsa

@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kThreads) key_weights_kernel(const __grid_cons
       if (!ok) set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);
       if (ok) {
         off = blk * a.kv.sb + (key % a.kv.bs) * a.kv.st + h * a.kv.sh;
-        if (a.kv.ks) scale = a.kv.ks[(int64_t)blk * a.kv.hkv + h];
+        if (a.kv.ks) scale = pow2(scale_exponent_of(a.kv.ks[(int64_t)blk * a.kv.hkv + h]));
       }
     }
     sm.off[tid] = off;
