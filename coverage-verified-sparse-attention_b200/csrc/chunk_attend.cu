@@ -482,9 +482,11 @@ ChunkGeo general_geo(const KvView& kv, const RaggedView& rg, const ChunkView& c)
 }  // namespace
 
 bool chunk_attend_supported(const KvView& kv, const RaggedView& rg, const ChunkView& c) {
+  const int few = chunk_few_rows(kv, rg, c);
   return (kv.d == 64 || kv.d == 128 || kv.d == 256) && c.hq / kv.hkv <= 64 &&
-         chunk_fits(rg, chunk_tc_eligible(kv, c) ? chunk_tc_geo(kv, rg, c)
-                                                 : general_geo(kv, rg, c));
+         chunk_fits(rg, few ? chunk_few_geo(kv, rg, c, few)
+                        : chunk_tc_eligible(kv, c) ? chunk_tc_geo(kv, rg, c)
+                                                   : general_geo(kv, rg, c));
 }
 
 size_t chunk_attend_workspace_bytes(const KvView& kv, const RaggedView& rg, const ChunkView& c) {
@@ -494,14 +496,18 @@ size_t chunk_attend_workspace_bytes(const KvView& kv, const RaggedView& rg, cons
 
 cudaError_t launch_chunk_attend(const KvView& kv, const RaggedView& rg, const ChunkView& c,
                                 void* ws, int32_t* dev_err, cudaStream_t s) {
-  const bool tc = chunk_tc_eligible(kv, c);
-  const int ctas = chunk_ctas(kv, tc);
-  const int rows = tc ? chunk_tc_rows() : gen_rows(rg, kv, c.hq / kv.hkv);  // of an item
+  const int few = chunk_few_rows(kv, rg, c);
+  const bool tc = !few && chunk_tc_eligible(kv, c);
+  const int ctas = few ? chunk_few_ctas() : chunk_ctas(kv, tc);
+  // of an item
+  const int rows = few ? few : tc ? chunk_tc_rows() : gen_rows(rg, kv, c.hq / kv.hkv);
   ChunkMergeDesc* desc = reinterpret_cast<ChunkMergeDesc*>(ws);
   float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kDescBytes);
   const bool split = tc ? chunk_tc_geo(kv, rg, c).split : general_geo(kv, rg, c).split;
   cudaError_t e;
-  if (tc) {
+  if (few) {
+    return launch_chunk_few(kv, rg, c, few, ctas, parts, desc, dev_err, s);
+  } else if (tc) {
     e = launch_chunk_tc(kv, rg, c, ctas, parts, desc, dev_err, s);
   } else {
     GenArgs a;

@@ -289,4 +289,12 @@ int chunk_tc_rows();  // query rows of an item at most (a partial slot's rows)
 cudaError_t launch_chunk_tc(const KvView& kv, const RaggedView& rg, const ChunkView& c, int ctas,
                             float* parts, ChunkMergeDesc* desc, int32_t* dev_err, cudaStream_t s);
 
+// ---- chunk_attend_few.cu ----
+int chunk_few_rows(const KvView& kv, const RaggedView& rg, const ChunkView& c);
+int chunk_few_ctas();
+ChunkGeo chunk_few_geo(const KvView& kv, const RaggedView& rg, const ChunkView& c, int rows);
+cudaError_t launch_chunk_few(const KvView& kv, const RaggedView& rg, const ChunkView& c, int rows,
+                             int ctas, float* parts, ChunkMergeDesc* desc, int32_t* dev_err,
+                             cudaStream_t s);
+
 }  // namespace cvsa

@@ -16,15 +16,19 @@ namespace cvsa {
 
 constexpr int kScaleMin = -15, kScaleMax = 7;
 
-// Two codes (low byte first) as f16; exact.
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-  return (uint32_t)h.x | (uint32_t)h.y << 16;
+// Four codes (low byte first) as f16, two a word; exact.
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four));
 }
 // Four codes as floats; exact.
 __device__ __forceinline__ void e4m3x4_to_f4(uint32_t four, float* f) {
-  f16x2_to_f2(e4m3x2_to_f16x2(four & 0xffffu), f[0], f[1]);
-  f16x2_to_f2(e4m3x2_to_f16x2(four >> 16), f[2], f[3]);
+  uint32_t lo, hi;
+  e4m3x4_to_f16x4(four, lo, hi);
+  f16x2_to_f2(lo, f[0], f[1]);
+  f16x2_to_f2(hi, f[2], f[3]);
 }
 // Four floats as codes: nearest, halves to even, beyond 448 saturated, NaN kept.
 __device__ __forceinline__ uint32_t f4_to_e4m3x4(float a, float b, float c, float d) {
@@ -66,10 +70,14 @@ __device__ __forceinline__ void widen16(const uint4& codes, uint32_t factor, uin
   uint32_t* o = reinterpret_cast<uint32_t*>(out);
   const __half2 f = *reinterpret_cast<const __half2*>(&factor);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t two = e4m3x2_to_f16x2(i & 1 ? c[i / 2] >> 16 : c[i / 2] & 0xffffu);
-    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&two), f);
-    o[i] = *reinterpret_cast<const uint32_t*>(&x);
+  for (int i = 0; i < 4; ++i) {
+    uint32_t two[2];
+    e4m3x4_to_f16x4(c[i], two[0], two[1]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&two[j]), f);
+      o[2 * i + j] = *reinterpret_cast<const uint32_t*>(&x);
+    }
   }
 }
 
