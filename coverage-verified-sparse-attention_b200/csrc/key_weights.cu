@@ -15,6 +15,7 @@
 #include "cvsa_common.cuh"
 #include "cvsa_internal.h"
 #include "fp8.cuh"
+#include "weights_plan.cuh"
 
 namespace cvsa {
 namespace {
@@ -186,6 +187,8 @@ bool key_weights_supported(const KvView& kv, const RaggedView& rg, const KeyWeig
 
 cudaError_t launch_key_weights(const KvView& kv, const RaggedView& rg, const KeyWeightsView& w,
                                int32_t* dev_err, cudaStream_t s) {
+  if (const int rows = weights_few_rows(kv, rg, w))
+    return launch_weights_few(kv, rg, w, rows, dev_err, s);
   WeightArgs a;
   a.rg = rg;
   a.kv = kv;
