@@ -1,0 +1,443 @@
+// Key weights of many rows on the tensor cores: 16-bit queries over a cache of their type
+// or of 8 bits, head_dim 64 or 128. Formula in key_weights.cu, work split as in
+// weights_plan.cuh.
+//
+// A persistent CTA an SM. An item is 256 keys of one KV head, kept in shared memory as two
+// tiles of M, against the rows that see them, 128 at a time (N):
+//   S' = K Q'   (fp32 in tensor memory, two buffers of two tiles)
+// so that a thread owns a key and its sum over rows never leaves it. The scores of the
+// next rows form while these are summed; the next item's keys are loaded meanwhile. 8-bit
+// keys are widened to the queries' type as they are copied, once an item.
+// Roles: warps 0-3 and 4-7 sum the first and the second tile, warps 8-11 load keys, warp
+// 12 issues the products, warps 13 and 14 load queries with their log-sum-exps and
+// positions. Each follows the same list of items on its own.
+// Bound by the exponentials (16 a clock and SM; 256 tokens of 32 heads at 32K keys: 60 us
+// of them, against 41 us of products at the tensor cores' rate).
+#include <cstddef>
+#include <type_traits>
+
+#include "cvsa_common.cuh"
+#include "cvsa_internal.h"
+#include "fp8.cuh"
+#include "tcgen05.cuh"
+#include "weights_plan.cuh"
+
+namespace cvsa {
+namespace {
+
+constexpr int kThreads = 512, kTile = 128, kKeys = 2 * kTile, kRing = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct WMeta {
+  uint64_t k_full[2], k_empty[2], q_full[2], q_empty[2], s_full[2], s_free[2], drain;
+  // rows of a step, in a ring: the rows of step n are written over once the products of
+  // step n + kRing - 2 are done, which wait for scores of step n + kRing - 4 to be taken
+  // by every warp that sums, and so for its sums of step n
+  alignas(16) float c[kRing][kTile];  // minus the log-sum-exp; -inf: the row takes no part
+  int pos[kRing][kTile];
+  uint8_t some[kRing][4];    // of 32 rows, some take no part
+  uint32_t tmem, abort;
+};
+static_assert(offsetof(WMeta, c) % 16 == 0 && offsetof(WMeta, some) % 4 == 0, "wide loads");
+
+struct WArgs {
+  RaggedView rg;
+  KvView kv;
+  KeyWeightsView w;
+  WeightGeo g;
+  int P;  // tokens of a step
+  int32_t* dev_err;
+  uint32_t wait_limit;
+};
+
+// Bounded wait; false (with the CTA's abort flag and CVSA_DEV_ERR_TIMEOUT set) when the
+// phase does not complete, or another warp gave up. Whole warp, one answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, WMeta* m, const WArgs& a) {
+  bool ok = false;
+  for (uint32_t i = 0; i < a.wait_limit && !ok; ++i) {
+    ok = mbar_try_wait(bar, parity);
+    if (!ok && (i & 15) == 15 && *reinterpret_cast<volatile uint32_t*>(&m->abort)) break;
+  }
+  if (!ok && !*reinterpret_cast<volatile uint32_t*>(&m->abort)) {
+    *reinterpret_cast<volatile uint32_t*>(&m->abort) = 1;
+    set_dev_error(a.dev_err, CVSA_DEV_ERR_TIMEOUT);
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  // weights below 2^-126 are flushed to 0, far below the rounding of any sum
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(ok ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void arrive_when_landed(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+// 16-byte piece `ch` of row `row` of a tile of 128 rows, 128-byte swizzle.
+__device__ __forceinline__ uint32_t piece(uint32_t tile, int row, int ch) {
+  return tile + (ch >> 3) * (kTile * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+}
+
+template <int D>
+struct WCfg {
+  static constexpr int kTileBytes = kTile * D * 2;
+  static constexpr int kQ = 4 * kTileBytes;                // two buffers of two K tiles first
+  static constexpr int kMeta = kQ + 2 * kTileBytes;
+  static constexpr int kSmem = kMeta + (int)sizeof(WMeta) + 1024;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+// 32 rows r0.. of a tile; lane i's row is off elements into src (< 0: zeros).
+template <typename T, int D>
+__device__ __forceinline__ void copy_rows(uint32_t tile, int r0, const void* src, int64_t off) {
+  constexpr int kCh = D / 8, kRPI = 32 / kCh;
+  const int lane = threadIdx.x & 31, ch = lane % kCh;
+#pragma unroll 4
+  for (int i = 0; i < 32 / kRPI; ++i) {
+    const int r = i * kRPI + lane / kCh;
+    const int64_t o = __shfl_sync(0xffffffffu, off, r);
+    cp16(piece(tile, r0 + r, ch), static_cast<const T*>(src) + (o < 0 ? 0 : o + ch * 8), o >= 0);
+  }
+}
+
+// The same of 8-bit codes, widened to T with the rows' factors.
+template <typename T, int D>
+__device__ __forceinline__ void widen_rows(uint32_t tile, int r0, const void* src, int64_t off,
+                                           float scale) {
+  constexpr int kCh = D / 16, kRPI = 32 / kCh, kN = 32 / kRPI;
+  const int lane = threadIdx.x & 31, ch = lane % kCh;
+  uint4 codes[kN];  // all loads before the first store
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    const int64_t o = __shfl_sync(0xffffffffu, off, i * kRPI + lane / kCh);
+    codes[i] = o < 0 ? make_uint4(0, 0, 0, 0)
+                     : ldg_stream16(static_cast<const char*>(src) + o + ch * 16);
+  }
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    const int r = i * kRPI + lane / kCh;
+    const float f = __shfl_sync(0xffffffffu, scale, r);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&codes[i]);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t y[4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float x[4];
+        e4m3x4_to_f4(w[half * 2 + j], x);
+        y[2 * j] = Mma<T>::pack(x[0] * f, x[1] * f);
+        y[2 * j + 1] = Mma<T>::pack(x[2] * f, x[3] * f);
+      }
+      asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(piece(tile, r0 + r, ch * 2 + half)),
+                   "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3])
+                   : "memory");
+    }
+  }
+}
+
+template <typename T, int D, bool F8>
+__device__ __forceinline__ void key_role(const WArgs& a, WMeta* m, uint32_t base, WeightWalk walk,
+                                         int w) {
+  using C = WCfg<D>;
+  const int lane = threadIdx.x & 31;
+  uint32_t n = 0;
+  for (; walk.next(a.rg, a.g); walk.step()) {
+    int t0, t1;
+    weight_tokens(walk.q, a.g, walk.i, t0, t1);
+    if (t0 >= t1) continue;
+    const uint32_t buf = n & 1;
+    const int32_t* const table = a.rg.tables + (int64_t)walk.q.slot * a.rg.W;
+    // keys w * 64 + 32 k + lane of the tiles
+    int64_t off[2];
+    float scale[2] = {1.f, 1.f};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int key = walk.i * kKeys + w * 64 + k * 32 + lane;
+      off[k] = -1;
+      if (key >= walk.q.ctx) continue;
+      const int page = key / a.g.bs, blk = table[page];
+      if (blk < 0 || blk >= a.kv.num_blocks) {
+        set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);
+        continue;
+      }
+      off[k] = blk * a.kv.sb + (key - page * a.g.bs) * a.kv.st + walk.h * a.kv.sh;
+      if constexpr (F8)
+        scale[k] = pow2(scale_exponent_of(a.kv.ks[(int64_t)blk * a.kv.hkv + walk.h]));
+    }
+    if (!warp_wait(&m->k_empty[buf], ((n >> 1) & 1) ^ 1, m, a)) break;
+    const uint32_t tile = base + (buf * 2 + w / 2) * C::kTileBytes;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r0 = (w & 1) * 64 + k * 32;
+      if constexpr (F8) widen_rows<T, D>(tile, r0, a.kv.k, off[k], scale[k]);
+      else copy_rows<T, D>(tile, r0, a.kv.k, off[k]);
+    }
+    if constexpr (F8) mbar_arrive(&m->k_full[buf]);
+    else arrive_when_landed(&m->k_full[buf]);
+    ++n;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void query_role(const WArgs& a, WMeta* m, uint32_t base, WeightWalk walk,
+                                           int w) {
+  using C = WCfg<D>;
+  const int lane = threadIdx.x & 31, G = a.g.G;
+  uint32_t n = 0;
+  bool ok = true;
+  for (; ok && walk.next(a.rg, a.g); walk.step()) {
+    int t0, t1;
+    weight_tokens(walk.q, a.g, walk.i, t0, t1);
+    for (int ta = t0; ta < t1; ta += a.P, ++n) {
+      const uint32_t buf = n & 1, slot = n % kRing;
+      const int rows = min(a.P, t1 - ta) * G;
+      int64_t off[2];
+      float lse[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {  // rows w * 64 + 32 k + lane
+        const int r = w * 64 + k * 32 + lane;
+        off[k] = -1;
+        lse[k] = neg_inf();
+        if (r >= rows) continue;
+        const int64_t tok = walk.q.tok0 + ta + r / G;
+        off[k] = tok * a.w.q_st + (int64_t)(walk.h * G + r % G) * a.w.q_sh;
+        lse[k] = a.w.lse[tok * a.w.hq + walk.h * G + r % G];
+      }
+      ok = warp_wait(&m->q_empty[buf], ((n >> 1) & 1) ^ 1, m, a);
+      if (!ok) break;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int r = w * 64 + k * 32 + lane;
+        copy_rows<T, D>(base + C::kQ + buf * C::kTileBytes, w * 64 + k * 32, a.w.q, off[k]);
+        const bool none = lse[k] == neg_inf();
+        m->c[slot][r] = none ? neg_inf() : -lse[k];
+        m->pos[slot][r] = walk.q.start + ta + r / G;
+        const bool some = __any_sync(0xffffffffu, none);
+        if (lane == 0) m->some[slot][w * 2 + k] = some;
+      }
+      __syncwarp();
+      arrive_when_landed(&m->q_full[buf]);
+      mbar_arrive(&m->q_full[buf]);
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// The whole warp runs the loop, one elected lane issues.
+template <typename T, int D>
+__device__ __forceinline__ void mma_role(const WArgs& a, WMeta* m, uint32_t base, uint32_t tmem,
+                                         WeightWalk walk) {
+  using C = WCfg<D>;
+  constexpr uint32_t kId = mma_idesc(!std::is_same<T, __half>::value, kTile, kTile, false);
+  const uint64_t k_desc = smem_desc(base, 16, 1024), q_desc = smem_desc(base + C::kQ, 16, 1024);
+  uint32_t nk = 0, n = 0;
+  for (; walk.next(a.rg, a.g); walk.step()) {
+    int t0, t1;
+    weight_tokens(walk.q, a.g, walk.i, t0, t1);
+    const int steps = __shfl_sync(0xffffffffu, (t1 - t0 + a.P - 1) / a.P, 0);
+    if (steps <= 0) continue;
+    const uint32_t kb = nk & 1;
+    if (!warp_wait(&m->k_full[kb], (nk >> 1) & 1, m, a)) goto out;
+    for (int j = 0; j < steps; ++j, ++n) {
+      const uint32_t b = n & 1;
+      if (!warp_wait(&m->q_full[b], (n >> 1) & 1, m, a)) goto out;
+      if (!warp_wait(&m->s_free[b], ((n >> 1) & 1) ^ 1, m, a)) goto out;
+      fence_proxy_async_smem();  // the tiles were written through the generic proxy
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          const uint64_t kd = k_desc + (((kb * 2 + mt) * C::kTileBytes) >> 4);
+          const uint64_t qd = q_desc + ((b * C::kTileBytes) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t o = ((kk / 4) * (kTile * 128) + (kk % 4) * 32) >> 4;
+            mma_ss(tmem + (b * 2 + mt) * kTile, kd + o, qd + o, kId, kk > 0);
+          }
+        }
+        mma_commit(smem_u32(&m->s_full[b]));
+        mma_commit(smem_u32(&m->q_empty[b]));
+        if (j == steps - 1) mma_commit(smem_u32(&m->k_empty[kb]));
+      }
+      __syncwarp();
+    }
+    ++nk;
+  }
+out:
+  // nothing of this CTA may be in flight when its tensor memory is freed
+  if (elect_one()) mma_commit(smem_u32(&m->drain));
+  __syncwarp();
+  mbar_wait_bounded(&m->drain, 0, 1u << 18);
+  __syncwarp();
+}
+
+__device__ __forceinline__ void sum_role(const WArgs& a, WMeta* m, uint32_t tmem, WeightWalk walk,
+                                         int mt) {
+  const int warp = threadIdx.x >> 5 & 3, lane = threadIdx.x & 31, G = a.g.G;
+  const uint64_t sc = f2_pack(a.w.scale, a.w.scale), l2 = f2_pack(kLog2e, kLog2e);
+  uint32_t n = 0;
+  for (; walk.next(a.rg, a.g); walk.step()) {
+    const SeqInfo& q = walk.q;
+    int t0, t1;
+    weight_tokens(q, a.g, walk.i, t0, t1);
+    const int first = walk.i * kKeys + mt * kTile, key = first + warp * 32 + lane;
+    const int last = min(first + kTile, q.ctx) - 1;  // of the tile's keys
+    const bool there = key < q.ctx;
+    const int64_t at = ((int64_t)q.slot * a.kv.hkv + walk.h) * a.w.stride + key;
+    float had = 0.f;
+    bool good = false;
+    if (there) {
+      if (key < q.start) had = a.w.decay * a.w.prior[at];
+      const int blk = a.rg.tables[(int64_t)q.slot * a.rg.W + key / a.g.bs];
+      good = blk >= 0 && blk < a.kv.num_blocks;
+    }
+    float total = 0.f;
+    for (int ta = t0; ta < t1; ta += a.P, ++n) {
+      const uint32_t b = n & 1, slot = n % kRing;
+      const int rows = min(a.P, t1 - ta) * G;
+      // some row does not see every key of the tile
+      const bool partial = (a.g.causal && q.start + ta < last) ||
+                           (a.g.window > 0 && first <= q.start + ta + (rows - 1) / G - a.g.window);
+      if (!warp_wait(&m->s_full[b], (n >> 1) & 1, m, a)) return;
+      tc_fence_after();
+      const uint32_t ts = tmem + (b * 2 + mt) * kTile + ((uint32_t)(warp * 32) << 16);
+      const uint32_t some = *reinterpret_cast<const uint32_t*>(m->some[slot]);
+      uint64_t sum0 = 0, sum1 = 0;
+#pragma unroll 1
+      for (int x = 0; x < rows; x += 32) {
+        float s[32];
+        tmem_ld32(ts + x, s);
+        tmem_wait_ld();
+        if (x + 32 >= rows) {  // the next products may go there
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&m->s_free[b]);
+        }
+        const float4* const c4 = reinterpret_cast<const float4*>(m->c[slot] + x);
+        if (!partial && !(some >> (x / 32 * 8) & 0xff)) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 c = c4[i];
+            float u, v;
+            f2_unpack(f2_mul(f2_fma(f2_pack(s[4 * i], s[4 * i + 1]), sc, f2_pack(c.x, c.y)), l2), u, v);
+            sum0 = f2_add(sum0, f2_pack(ex2(u), ex2(v)));
+            f2_unpack(f2_mul(f2_fma(f2_pack(s[4 * i + 2], s[4 * i + 3]), sc, f2_pack(c.z, c.w)), l2), u, v);
+            sum1 = f2_add(sum1, f2_pack(ex2(u), ex2(v)));
+          }
+        } else {
+          float add = 0.f;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float c = m->c[slot][x + i];
+            const int p = m->pos[slot][x + i];
+            const bool sees = c != neg_inf() && (!a.g.causal || key <= p) &&
+                              (a.g.window == 0 || key > p - a.g.window);
+            const float e = ex2(fmaf(s[i], a.w.scale, c) * kLog2e);
+            add += sees ? e : 0.f;
+          }
+          sum0 = f2_add(sum0, f2_pack(add, 0.f));
+        }
+      }
+      float u, v;
+      f2_unpack(f2_add(sum0, sum1), u, v);
+      total += u + v;
+    }
+    if (there) a.w.out[at] = good ? had + total : had;
+  }
+}
+
+template <typename T, int D, bool F8>
+__global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_constant__ WArgs a) {
+  using C = WCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  WMeta* m = reinterpret_cast<WMeta*>(smem + C::kMeta);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&m->k_full[i], 128);
+      mbar_init(&m->k_empty[i], 1);
+      mbar_init(&m->q_full[i], 128);  // copies and plain writes of 64 threads
+      mbar_init(&m->q_empty[i], 1);
+      mbar_init(&m->s_full[i], 1);
+      mbar_init(&m->s_free[i], 8);
+    }
+    mbar_init(&m->drain, 1);
+    m->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) tmem_alloc(smem_u32(&m->tmem), 512);
+  const WeightRange r = weight_range(a.rg, a.g, blockIdx.x, gridDim.x,
+                                     warp == 0 ? a.dev_err : nullptr);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t base = smem_u32(smem), tmem = __shfl_sync(0xffffffffu, m->tmem, 0);
+  const WeightWalk walk(r);
+  if (warp < 8) sum_role(a, m, tmem, walk, warp / 4);
+  else if (warp < 12) key_role<T, D, F8>(a, m, base, walk, warp - 8);
+  else if (warp == 12) mma_role<T, D>(a, m, base, tmem, walk);
+  else if (warp < 15) query_role<T, D>(a, m, base, walk, warp - 13);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int D, bool F8>
+cudaError_t launch_one(const WArgs& a, cudaStream_t s) {
+  constexpr int kSmem = WCfg<D>::kSmem;
+  const cudaError_t e = cudaFuncSetAttribute(weights_tc_kernel<T, D, F8>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  weights_tc_kernel<T, D, F8><<<num_sms(), kThreads, kSmem, s>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_t(const WArgs& a, cudaStream_t s) {
+  const bool f8 = a.kv.dtype == CVSA_DTYPE_E4M3;
+  if (a.kv.d == 64) return f8 ? launch_one<T, 64, true>(a, s) : launch_one<T, 64, false>(a, s);
+  return f8 ? launch_one<T, 128, true>(a, s) : launch_one<T, 128, false>(a, s);
+}
+
+}  // namespace
+
+bool weights_tc_eligible(const KvView& kv, const KeyWeightsView& w) {
+  return (kv.dtype == w.dtype || kv.dtype == CVSA_DTYPE_E4M3) && w.dtype != CVSA_DTYPE_F32 &&
+         (kv.d == 64 || kv.d == 128);
+}
+
+cudaError_t launch_weights_tc(const KvView& kv, const RaggedView& rg, const KeyWeightsView& w,
+                              int32_t* dev_err, cudaStream_t s) {
+  WArgs a;
+  a.rg = rg;
+  a.kv = kv;
+  a.w = w;
+  a.g.bs = kv.bs;
+  a.g.hkv = kv.hkv;
+  a.g.G = w.hq / kv.hkv;
+  a.g.KT = kKeys;
+  a.P = kTile / a.g.G;
+  a.g.rows = a.P * a.g.G;
+  a.g.fixed = 1;
+  a.g.causal = w.causal;
+  a.g.window = w.window;
+  a.dev_err = dev_err;
+  a.wait_limit = wait_limit() ? wait_limit() : 1u << 18;  // a poll waits about 4 us: a second
+  return w.dtype == CVSA_DTYPE_BF16 ? launch_t<__nv_bfloat16>(a, s) : launch_t<__half>(a, s);
+}
+
+}  // namespace cvsa

@@ -102,6 +102,12 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   return r;
 }
 
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // ---- MMA -----------------------------------------------------------------
 // Shared-memory matrix descriptor, 128-byte swizzle. K-major operand: rows of
 // 64 16-bit elements (128 bytes), 8-row groups `sbo` bytes apart. MN-major

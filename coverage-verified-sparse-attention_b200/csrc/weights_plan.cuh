@@ -181,4 +181,9 @@ int weights_few_rows(const KvView& kv, const RaggedView& rg, const KeyWeightsVie
 cudaError_t launch_weights_few(const KvView& kv, const RaggedView& rg, const KeyWeightsView& w,
                                int rows, int32_t* dev_err, cudaStream_t s);
 
+// ---- key_weights_tc.cu ----
+bool weights_tc_eligible(const KvView& kv, const KeyWeightsView& w);
+cudaError_t launch_weights_tc(const KvView& kv, const RaggedView& rg, const KeyWeightsView& w,
+                              int32_t* dev_err, cudaStream_t s);
+
 }  // namespace cvsa
