@@ -189,7 +189,10 @@ cudaError_t launch_key_weights(const KvView& kv, const RaggedView& rg, const Key
                                int32_t* dev_err, cudaStream_t s) {
   if (const int rows = weights_few_rows(kv, rg, w))
     return launch_weights_few(kv, rg, w, rows, dev_err, s);
-  if (weights_tc_eligible(kv, w)) return launch_weights_tc(kv, rg, w, dev_err, s);
+  if (weights_tc_eligible(kv, rg, w)) {
+    const cudaError_t e = launch_weights_tc(kv, rg, w, dev_err, s);
+    if (e != cudaErrorNotSupported) return e;
+  }
   WeightArgs a;
   a.rg = rg;
   a.kv = kv;

@@ -20,6 +20,7 @@
 #include "cvsa_internal.h"
 #include "fp8.cuh"
 #include "tcgen05.cuh"
+#include "tma.cuh"
 #include "weights_plan.cuh"
 
 namespace cvsa {
@@ -29,16 +30,16 @@ constexpr int kThreads = 512, kTile = 128, kKeys = 2 * kTile, kRing = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct WMeta {
-  uint64_t k_full[2], k_empty[2], q_full[2], q_empty[2], s_full[2], s_free[2], drain;
+  uint64_t k_full[2], k_empty[2], q_full[2], q_copied[2], q_empty[2], drain;
+  uint64_t s_full[2][2], s_free[2][2];  // buffer, tile
   // rows of a step, in a ring: the rows of step n are written over once the products of
   // step n + kRing - 2 are done, which wait for scores of step n + kRing - 4 to be taken
   // by every warp that sums, and so for its sums of step n
-  alignas(16) float c[kRing][kTile];  // minus the log-sum-exp; -inf: the row takes no part
-  int pos[kRing][kTile];
-  uint8_t some[kRing][4];    // of 32 rows, some take no part
+  alignas(16) float c[kRing][kTile];  // minus the log-sum-exp
+  uint32_t live[kRing][4];            // bit per row that takes part (is there, saw a key)
   uint32_t tmem, abort;
 };
-static_assert(offsetof(WMeta, c) % 16 == 0 && offsetof(WMeta, some) % 4 == 0, "wide loads");
+static_assert(offsetof(WMeta, c) % 16 == 0, "wide loads");
 
 struct WArgs {
   RaggedView rg;
@@ -48,6 +49,7 @@ struct WArgs {
   int P;  // tokens of a step
   int32_t* dev_err;
   uint32_t wait_limit;
+  alignas(64) CUtensorMap q_map;  // tiles of P tokens of a KV head's group
 };
 
 // Bounded wait; false (with the CTA's abort flag and CVSA_DEV_ERR_TIMEOUT set) when the
@@ -187,49 +189,70 @@ __device__ __forceinline__ void key_role(const WArgs& a, WMeta* m, uint32_t base
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <typename T, int D>
+// A step's query rows, (token, head of the group) in order, are a tile of their array: one
+// tensor copy for each 64 elements. What else a step needs of them is written by two
+// warps, 64 rows each; the next step's is looked up while this step's is on its way.
+template <int D>
 __device__ __forceinline__ void query_role(const WArgs& a, WMeta* m, uint32_t base, WeightWalk walk,
                                            int w) {
   using C = WCfg<D>;
   const int lane = threadIdx.x & 31, G = a.g.G;
-  uint32_t n = 0;
-  bool ok = true;
-  for (; ok && walk.next(a.rg, a.g); walk.step()) {
-    int t0, t1;
-    weight_tokens(walk.q, a.g, walk.i, t0, t1);
-    for (int ta = t0; ta < t1; ta += a.P, ++n) {
-      const uint32_t buf = n & 1, slot = n % kRing;
-      const int rows = min(a.P, t1 - ta) * G;
-      int64_t off[2];
-      float lse[2];
+  int rt[2], rh[2];  // token and head of rows w * 64 + 32 k + lane
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {  // rows w * 64 + 32 k + lane
-        const int r = w * 64 + k * 32 + lane;
-        off[k] = -1;
-        lse[k] = neg_inf();
-        if (r >= rows) continue;
-        const int64_t tok = walk.q.tok0 + ta + r / G;
-        off[k] = tok * a.w.q_st + (int64_t)(walk.h * G + r % G) * a.w.q_sh;
-        lse[k] = a.w.lse[tok * a.w.hq + walk.h * G + r % G];
-      }
-      ok = warp_wait(&m->q_empty[buf], ((n >> 1) & 1) ^ 1, m, a);
-      if (!ok) break;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int r = w * 64 + k * 32 + lane;
-        copy_rows<T, D>(base + C::kQ + buf * C::kTileBytes, w * 64 + k * 32, a.w.q, off[k]);
-        const bool none = lse[k] == neg_inf();
-        m->c[slot][r] = none ? neg_inf() : -lse[k];
-        m->pos[slot][r] = walk.q.start + ta + r / G;
-        const bool some = __any_sync(0xffffffffu, none);
-        if (lane == 0) m->some[slot][w * 2 + k] = some;
-      }
-      __syncwarp();
-      arrive_when_landed(&m->q_full[buf]);
-      mbar_arrive(&m->q_full[buf]);
-    }
+  for (int k = 0; k < 2; ++k) {
+    rt[k] = (w * 64 + k * 32 + lane) / G;
+    rh[k] = w * 64 + k * 32 + lane - rt[k] * G;
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  int ta = 0, t0 = 0, t1 = 0;
+  bool more = true, first = true;
+  float lse[2];
+  auto look = [&]() {  // the first step, or the next one; more: there is one
+    if (!first) ta += a.P;
+    while (more && ta >= t1) {
+      if (!first) walk.step();
+      first = false;
+      more = walk.next(a.rg, a.g);
+      if (more) {
+        weight_tokens(walk.q, a.g, walk.i, t0, t1);
+        ta = t0;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      lse[k] = neg_inf();
+      if (more && rt[k] < min(a.P, t1 - ta))
+        lse[k] = a.w.lse[(int64_t)(walk.q.tok0 + ta + rt[k]) * a.w.hq + walk.h * G + rh[k]];
+    }
+  };
+  look();
+  uint32_t n = 0;
+  for (; more; ++n) {
+    const uint32_t buf = n & 1, slot = n % kRing;
+    if (!warp_wait(&m->q_empty[buf], ((n >> 1) & 1) ^ 1, m, a)) break;
+    if (w == 0 && elect_one()) {
+      mbar_arrive_expect_tx(&m->q_copied[buf], a.P * G * D * 2);
+#pragma unroll
+      for (int x = 0; x < D; x += 64)
+        token_load(base + C::kQ + buf * C::kTileBytes + x / 64 * (kTile * 128), &a.q_map, x,
+                   walk.h * G, walk.q.tok0 + ta, &m->q_copied[buf]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r = w * 64 + k * 32 + lane;
+      const bool live = lse[k] != neg_inf();
+      m->c[slot][r] = live ? -lse[k] : neg_inf();
+      const uint32_t bits = __ballot_sync(0xffffffffu, live);
+      if (lane == 0) m->live[slot][w * 2 + k] = bits;
+    }
+    mbar_arrive(&m->q_full[buf]);
+    look();
+  }
+  // no copy outlives the CTA, whatever gave up
+  if (w == 0)
+    for (uint32_t i = n > 2 ? n - 2 : 0; i < n; ++i)
+      mbar_wait_bounded(&m->q_copied[i & 1], (i >> 1) & 1, 1u << 18);
+  __syncwarp();
 }
 
 // The whole warp runs the loop, one elected lane issues.
@@ -250,12 +273,13 @@ __device__ __forceinline__ void mma_role(const WArgs& a, WMeta* m, uint32_t base
     for (int j = 0; j < steps; ++j, ++n) {
       const uint32_t b = n & 1;
       if (!warp_wait(&m->q_full[b], (n >> 1) & 1, m, a)) goto out;
-      if (!warp_wait(&m->s_free[b], ((n >> 1) & 1) ^ 1, m, a)) goto out;
+      if (!warp_wait(&m->q_copied[b], (n >> 1) & 1, m, a)) goto out;
       fence_proxy_async_smem();  // the tiles were written through the generic proxy
-      tc_fence_after();
-      if (elect_one()) {
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+      for (int mt = 0; mt < 2; ++mt) {
+        if (!warp_wait(&m->s_free[b][mt], ((n >> 1) & 1) ^ 1, m, a)) goto out;
+        tc_fence_after();
+        if (elect_one()) {
           const uint64_t kd = k_desc + (((kb * 2 + mt) * C::kTileBytes) >> 4);
           const uint64_t qd = q_desc + ((b * C::kTileBytes) >> 4);
 #pragma unroll
@@ -263,12 +287,12 @@ __device__ __forceinline__ void mma_role(const WArgs& a, WMeta* m, uint32_t base
             const uint32_t o = ((kk / 4) * (kTile * 128) + (kk % 4) * 32) >> 4;
             mma_ss(tmem + (b * 2 + mt) * kTile, kd + o, qd + o, kId, kk > 0);
           }
+          mma_commit(smem_u32(&m->s_full[b][mt]));
+          if (mt) mma_commit(smem_u32(&m->q_empty[b]));
+          if (mt && j == steps - 1) mma_commit(smem_u32(&m->k_empty[kb]));
         }
-        mma_commit(smem_u32(&m->s_full[b]));
-        mma_commit(smem_u32(&m->q_empty[b]));
-        if (j == steps - 1) mma_commit(smem_u32(&m->k_empty[kb]));
+        __syncwarp();
       }
-      __syncwarp();
     }
     ++nk;
   }
@@ -278,6 +302,12 @@ out:
   __syncwarp();
   mbar_wait_bounded(&m->drain, 0, 1u << 18);
   __syncwarp();
+}
+
+// Bits e of [from, to) that lie in [x, x + 32), at e - x.
+__device__ __forceinline__ uint32_t bits_of(int from, int to, int x) {
+  const int a = max(from - x, 0), b = to - x;
+  return a >= 32 || b <= a ? 0u : (b >= 32 ? ~0u : (1u << b) - 1) & (~0u << a);
 }
 
 __device__ __forceinline__ void sum_role(const WArgs& a, WMeta* m, uint32_t tmem, WeightWalk walk,
@@ -293,37 +323,40 @@ __device__ __forceinline__ void sum_role(const WArgs& a, WMeta* m, uint32_t tmem
     const int last = min(first + kTile, q.ctx) - 1;  // of the tile's keys
     const bool there = key < q.ctx;
     const int64_t at = ((int64_t)q.slot * a.kv.hkv + walk.h) * a.w.stride + key;
-    float had = 0.f;
-    bool good = false;
-    if (there) {
-      if (key < q.start) had = a.w.decay * a.w.prior[at];
-      const int blk = a.rg.tables[(int64_t)q.slot * a.rg.W + key / a.g.bs];
-      good = blk >= 0 && blk < a.kv.num_blocks;
-    }
+    // what the key had and its page, not looked at before the sums are done
+    const float prior = there && key < q.start ? a.w.prior[at] : 0.f;
+    const int blk = there ? a.rg.tables[(int64_t)q.slot * a.rg.W + key / a.g.bs] : -1;
+    // the tokens that see the key: ta and those after it, up to tb
+    const int see0 = a.g.causal ? key - q.start : 0;
+    const int see1 = a.g.window > 0 ? see0 + a.g.window : q.n;
     float total = 0.f;
     for (int ta = t0; ta < t1; ta += a.P, ++n) {
       const uint32_t b = n & 1, slot = n % kRing;
-      const int rows = min(a.P, t1 - ta) * G;
+      const int tokens = min(a.P, t1 - ta), rows = tokens * G;
       // some row does not see every key of the tile
       const bool partial = (a.g.causal && q.start + ta < last) ||
-                           (a.g.window > 0 && first <= q.start + ta + (rows - 1) / G - a.g.window);
-      if (!warp_wait(&m->s_full[b], (n >> 1) & 1, m, a)) return;
+                           (a.g.window > 0 && first <= q.start + ta + tokens - 1 - a.g.window);
+      // rows [from, to) see the key
+      const int from = partial ? min(max(see0 - ta, 0), a.P) * G : 0;
+      const int to = partial ? min(max(see1 - ta, 0), a.P) * G : kTile;
+      if (!warp_wait(&m->s_full[b][mt], (n >> 1) & 1, m, a)) return;
       tc_fence_after();
       const uint32_t ts = tmem + (b * 2 + mt) * kTile + ((uint32_t)(warp * 32) << 16);
-      const uint32_t some = *reinterpret_cast<const uint32_t*>(m->some[slot]);
       uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll 1
       for (int x = 0; x < rows; x += 32) {
         float s[32];
         tmem_ld32(ts + x, s);
+        const uint32_t sees = bits_of(from, to, x) & m->live[slot][x / 32];
+        const bool all = __all_sync(0xffffffffu, sees == ~0u);
         tmem_wait_ld();
         if (x + 32 >= rows) {  // the next products may go there
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&m->s_free[b]);
+          if (lane == 0) mbar_arrive(&m->s_free[b][mt]);
         }
         const float4* const c4 = reinterpret_cast<const float4*>(m->c[slot] + x);
-        if (!partial && !(some >> (x / 32 * 8) & 0xff)) {
+        if (all) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float4 c = c4[i];
@@ -333,16 +366,14 @@ __device__ __forceinline__ void sum_role(const WArgs& a, WMeta* m, uint32_t tmem
             f2_unpack(f2_mul(f2_fma(f2_pack(s[4 * i + 2], s[4 * i + 3]), sc, f2_pack(c.z, c.w)), l2), u, v);
             sum1 = f2_add(sum1, f2_pack(ex2(u), ex2(v)));
           }
-        } else {
+        } else if (__any_sync(0xffffffffu, sees != 0)) {
           float add = 0.f;
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const float c = m->c[slot][x + i];
-            const int p = m->pos[slot][x + i];
-            const bool sees = c != neg_inf() && (!a.g.causal || key <= p) &&
-                              (a.g.window == 0 || key > p - a.g.window);
-            const float e = ex2(fmaf(s[i], a.w.scale, c) * kLog2e);
-            add += sees ? e : 0.f;
+            const float4 c = c4[i / 4];
+            const float y = i % 4 == 0 ? c.x : i % 4 == 1 ? c.y : i % 4 == 2 ? c.z : c.w;
+            const float e = ex2(fmaf(s[i], a.w.scale, y) * kLog2e);
+            add += sees >> i & 1 ? e : 0.f;
           }
           sum0 = f2_add(sum0, f2_pack(add, 0.f));
         }
@@ -351,7 +382,10 @@ __device__ __forceinline__ void sum_role(const WArgs& a, WMeta* m, uint32_t tmem
       f2_unpack(f2_add(sum0, sum1), u, v);
       total += u + v;
     }
-    if (there) a.w.out[at] = good ? had + total : had;
+    if (there) {
+      const float had = a.w.decay * prior;
+      a.w.out[at] = blk >= 0 && blk < a.kv.num_blocks ? had + total : had;
+    }
   }
 }
 
@@ -367,10 +401,13 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
     for (int i = 0; i < 2; ++i) {
       mbar_init(&m->k_full[i], 128);
       mbar_init(&m->k_empty[i], 1);
-      mbar_init(&m->q_full[i], 128);  // copies and plain writes of 64 threads
+      mbar_init(&m->q_full[i], 64);  // the plain writes
+      mbar_init(&m->q_copied[i], 1);
       mbar_init(&m->q_empty[i], 1);
-      mbar_init(&m->s_full[i], 1);
-      mbar_init(&m->s_free[i], 8);
+      for (int mt = 0; mt < 2; ++mt) {
+        mbar_init(&m->s_full[i][mt], 1);
+        mbar_init(&m->s_free[i][mt], 4);
+      }
     }
     mbar_init(&m->drain, 1);
     m->abort = 0;
@@ -387,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
   if (warp < 8) sum_role(a, m, tmem, walk, warp / 4);
   else if (warp < 12) key_role<T, D, F8>(a, m, base, walk, warp - 8);
   else if (warp == 12) mma_role<T, D>(a, m, base, tmem, walk);
-  else if (warp < 15) query_role<T, D>(a, m, base, walk, warp - 13);
+  else if (warp < 15) query_role<D>(a, m, base, walk, warp - 13);
   tc_fence_before();
   __syncthreads();
   if (warp == 12) {
@@ -415,8 +452,8 @@ cudaError_t launch_t(const WArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-bool weights_tc_eligible(const KvView& kv, const KeyWeightsView& w) {
-  return (kv.dtype == w.dtype || kv.dtype == CVSA_DTYPE_E4M3) && w.dtype != CVSA_DTYPE_F32 &&
+bool weights_tc_eligible(const KvView& kv, const RaggedView& rg, const KeyWeightsView& w) {
+  return rg.T > 0 && (kv.dtype == w.dtype || kv.dtype == CVSA_DTYPE_E4M3) && w.dtype != CVSA_DTYPE_F32 &&
          (kv.d == 64 || kv.d == 128);
 }
 
@@ -436,6 +473,9 @@ cudaError_t launch_weights_tc(const KvView& kv, const RaggedView& rg, const KeyW
   a.g.causal = w.causal;
   a.g.window = w.window;
   a.dev_err = dev_err;
+  if (!token_map(&a.q_map, w.q, w.dtype == CVSA_DTYPE_BF16, rg.T, w.hq, kv.d, w.q_st, w.q_sh, a.P,
+                 a.g.G))
+    return cudaErrorNotSupported;
   a.wait_limit = wait_limit() ? wait_limit() : 1u << 18;  // a poll waits about 4 us: a second
   return w.dtype == CVSA_DTYPE_BF16 ? launch_t<__nv_bfloat16>(a, s) : launch_t<__half>(a, s);
 }

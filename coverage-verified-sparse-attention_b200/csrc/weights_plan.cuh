@@ -182,7 +182,8 @@ cudaError_t launch_weights_few(const KvView& kv, const RaggedView& rg, const Key
                                int rows, int32_t* dev_err, cudaStream_t s);
 
 // ---- key_weights_tc.cu ----
-bool weights_tc_eligible(const KvView& kv, const KeyWeightsView& w);
+bool weights_tc_eligible(const KvView& kv, const RaggedView& rg, const KeyWeightsView& w);
+// cudaErrorNotSupported, with nothing launched, for queries whose strides no tensor map takes
 cudaError_t launch_weights_tc(const KvView& kv, const RaggedView& rg, const KeyWeightsView& w,
                               int32_t* dev_err, cudaStream_t s);
 
