@@ -6,17 +6,24 @@
 // weights move to the front: rows to new pages, so that no row is written over
 // before it is read and all rows can move at once.
 //
-// select: one block a (sequence, KV head). The cut, the n-th largest weight, is found
-//   by a radix select over the weights' order-preserving keys, 11, 11 and 10 bits a
-//   pass; a pass in order then writes the kept keys, placed by a prefix sum.
+// select: a cluster of 1 to 8 blocks a (sequence, KV head), each with a piece of the row
+//   in shared memory. The cut, the n-th largest weight, is found by a radix select over
+//   the weights' order-preserving keys, 11, 11 and 10 bits a pass, over the sum of the
+//   blocks' histograms; a pass in order then writes the kept keys, placed by a prefix sum.
+//   Bound by latency: one block over 32K keys took 70 us.
 // gather: one warp a new page and KV head; bound by bytes. In an 8-bit cache a new
 //   page gets the largest scale of the rows that go there, so none overflows; rows of
 //   smaller scale move to it (exact but for values that become subnormal).
 // reserve, commit: the page bookkeeping around them, one block each.
+#include <cooperative_groups.h>
+
 #include "block_scan.cuh"
 #include "cvsa_common.cuh"
 #include "cvsa_internal.h"
+#include "cvsa_launch.cuh"
 #include "fp8.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace cvsa {
 namespace {
@@ -26,7 +33,8 @@ constexpr int kThreads = 1024, kBins = 2048, kEach = 8;
 struct SelectArgs {
   EvictView e;
   int hkv, bs;
-  int cached;  // keys of a row that shared memory holds
+  int parts;   // blocks a row
+  int cached;  // keys of a piece that shared memory holds (all of it unless parts is 1)
   int32_t* dev_err;
 };
 
@@ -41,26 +49,27 @@ __device__ __forceinline__ int evict_len(const EvictView& e, int bs, int s, int3
 }
 
 __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_constant__ SelectArgs a) {
-  extern __shared__ uint32_t keys[];  // [cached]
-  __shared__ int hist[kBins];
+  extern __shared__ float piece[];  // [cached]
+  __shared__ int hist[2][kBins];
   __shared__ int sums[32];
   __shared__ int s_bin, s_left;
-  const int tid = threadIdx.x, lane = tid & 31;
-  const int s = blockIdx.x / a.hkv, h = blockIdx.x % a.hkv;
-  const int len = evict_len(a.e, a.bs, s, tid == 0 && h == 0 ? a.dev_err : nullptr);
+  __shared__ int counts[2];  // of this piece: taken above the cut or in any case, equal to it
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, parts = a.parts, part = blockIdx.x % parts;
+  const int s = blockIdx.x / parts / a.hkv, h = blockIdx.x / parts % a.hkv;
+  const int len = evict_len(a.e, a.bs, s, tid == 0 && part == 0 && h == 0 ? a.dev_err : nullptr);
   int32_t* const kept = a.e.kept + ((int64_t)s * a.hkv + h) * a.e.keep;
-  if (len == 0) {
-    for (int i = tid; i < a.e.keep; i += kThreads) kept[i] = -1;
+  if (len == 0) {  // the same in all blocks of the row
+    for (int i = part * kThreads + tid; i < a.e.keep; i += parts * kThreads) kept[i] = -1;
     return;
   }
   const float* const w = a.e.weights + ((int64_t)s * a.hkv + h) * a.e.w_stride;
   float* const out = a.e.out_weights + ((int64_t)s * a.hkv + h) * a.e.o_stride;
   const int lo = a.e.sink, hi = len - a.e.recent;
+  const int size = (len + parts - 1) / parts, p0 = min(len, part * size), p1 = min(len, p0 + size);
+  for (int i = p0 + tid; i < min(p1, p0 + a.cached); i += kThreads) piece[i - p0] = w[i];
+  auto weight = [&](int i) { return i - p0 < a.cached ? piece[i - p0] : w[i]; };
   int left = a.e.keep - a.e.sink - a.e.recent;  // to take of [lo, hi)
-  const int cached = min(a.cached, hi - lo);
-  for (int i = tid; i < cached; i += kThreads) keys[i] = float_key(w[lo + i]);
-  // key of candidate i
-  auto key_at = [&](int i) { return i < cached ? keys[i] : float_key(w[lo + i]); };
   uint32_t cut = 0xffffffffu;  // keys above are taken
   int room = 0;                // and this many of those equal to it
   if (left > 0) {
@@ -68,20 +77,29 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass < 2 ? 11 : 10;
-      for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
+      int* const mine = hist[pass & 1];
+      for (int i = tid; i < kBins; i += kThreads) mine[i] = 0;
       __syncthreads();
-      for (int i0 = 0; i0 < hi - lo; i0 += kThreads) {
+      for (int i0 = p0; i0 < p1; i0 += kThreads) {
         const int i = i0 + tid;
-        const uint32_t k = i < hi - lo ? key_at(i) : 0;
-        const int bin = i < hi - lo && (k & mask) == prefix ? (int)(k >> shift & ((1 << bits) - 1)) : -1;
+        const bool in = i < p1 && i >= lo && i < hi;
+        const uint32_t k = in ? float_key(weight(i)) : 0;
+        const int bin = in && (k & mask) == prefix ? (int)(k >> shift & ((1 << bits) - 1)) : -1;
         // neighbouring keys share bins: one addition a warp and bin
         const unsigned same = __match_any_sync(0xffffffffu, bin);
-        if (bin >= 0 && __ffs(same) - 1 == lane) atomicAdd(&hist[bin], __popc(same));
+        if (bin >= 0 && __ffs(same) - 1 == lane) atomicAdd(&mine[bin], __popc(same));
       }
-      __syncthreads();
+      // Every block sums the row's histograms. (The other buffer is cleared a pass later,
+      // when all blocks have passed this point and so are done with it.)
+      if (parts > 1) cluster.sync(); else __syncthreads();
       // bin that holds the left-th key from the top: sums from the highest bin
       const int top = kBins - 1 - 2 * tid;
-      const int c0 = hist[top], c1 = hist[top - 1];
+      int c0 = 0, c1 = 0;
+      for (int p = 0; p < parts; ++p) {
+        const int* const theirs = parts > 1 ? cluster.map_shared_rank(mine, p) : mine;
+        c0 += theirs[top];
+        c1 += theirs[top - 1];
+      }
       const int incl = block_scan_incl(c0 + c1, sums);
       const int before = incl - c0 - c1;
       if (before < left && incl >= left) {
@@ -97,22 +115,54 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
     }
     cut = prefix;
     room = left;
+  } else {
+    __syncthreads();
   }
-  // in order, kEach neighbours a thread; a key's place is the number taken before it
-  int taken = 0, equal = 0;  // before this round: taken without those equal to the cut, and these
-  for (int i0 = 0; i0 < len; i0 += kThreads * kEach) {
-    const int base = i0 + tid * kEach;
-    float x[kEach];
-    uint32_t above = 0, same = 0;
+  // kEach neighbours a thread from i0 on: which are taken in any case or above the cut,
+  // and which are equal to it
+  auto look = [&](int i0, float* x, uint32_t& above, uint32_t& same) {
+    above = same = 0;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      const int i = base + j;
-      x[j] = i < len ? w[i] : 0.f;
+      const int i = i0 + tid * kEach + j;
+      x[j] = i < p1 ? weight(i) : 0.f;
       const uint32_t k = float_key(x[j]);
       const bool forced = i < lo || i >= hi;
-      if (i < len && (forced || k > cut)) above |= 1u << j;
-      if (i < len && !forced && k == cut && room > 0) same |= 1u << j;
+      if (i < p1 && (forced || k > cut)) above |= 1u << j;
+      if (i < p1 && !forced && k == cut && room > 0) same |= 1u << j;
     }
+  };
+  int taken = 0, equal = 0;  // before the keys at hand
+  float x[kEach];
+  uint32_t above, same;
+  if (parts > 1) {
+    if (tid < 2) counts[tid] = 0;
+    __syncthreads();
+    int n_above = 0, n_same = 0;
+    for (int i0 = p0; i0 < p1; i0 += kThreads * kEach) {
+      look(i0, x, above, same);
+      n_above += __popc(above);
+      n_same += __popc(same);
+    }
+    n_above = __reduce_add_sync(0xffffffffu, n_above);
+    n_same = __reduce_add_sync(0xffffffffu, n_same);
+    if (lane == 0) {
+      atomicAdd(&counts[0], n_above);
+      atomicAdd(&counts[1], n_same);
+    }
+    // beyond this point weights may be written over: every block holds its piece
+    cluster.sync();
+    for (int p = 0; p < part; ++p) {
+      const int* const theirs = cluster.map_shared_rank(counts, p);
+      taken += theirs[0];
+      equal += theirs[1];
+    }
+    cluster.sync();  // the others' counts were read
+  }
+  // in order; a key's place is the number taken before it
+  for (int i0 = p0; i0 < p1; i0 += kThreads * kEach) {
+    const int base = i0 + tid * kEach;
+    look(i0, x, above, same);
     // both counts in one scan: at most kThreads * kEach = 8192 of each
     const int mine = __popc(above) | __popc(same) << 16;
     const int incl = block_scan_incl(mine, sums);
@@ -123,7 +173,7 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
       if (is_above || (is_same && q0 < room)) {
         const int at = a0 + min(q0, room);
         kept[at] = base + j;
-        out[at] = x[j];  // at <= base + j: read by this round or an earlier one
+        out[at] = x[j];  // at <= base + j: held by a block, or read by this round or before
       }
       a0 += is_above;
       q0 += is_same;
@@ -134,6 +184,7 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
     equal += sums[0] >> 16;
     __syncthreads();
   }
+  pdl_launch_dependents();
 }
 
 struct GatherArgs {
@@ -152,8 +203,11 @@ __global__ void __launch_bounds__(kGatherWarps * 32) evict_gather_kernel(const _
   const int64_t warp = (int64_t)blockIdx.x * kGatherWarps + (threadIdx.x >> 5);
   const int h = (int)(warp % hkv), page = (int)(warp / hkv % a.e.new_pages);
   const int64_t s = warp / hkv / a.e.new_pages;
-  if (s >= a.e.S || evict_len(a.e, bs, (int)s, nullptr) == 0) return;
+  if (s >= a.e.S) return;
   const int to = a.e.new_tables[s * a.e.new_pages + page];
+  const int len = evict_len(a.e, bs, (int)s, nullptr);
+  pdl_wait();  // the kept keys
+  if (len == 0) return;
   if (to < 0 || to >= a.kv.num_blocks) {
     if (lane == 0) set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);
     return;
@@ -176,13 +230,18 @@ __global__ void __launch_bounds__(kGatherWarps * 32) evict_gather_kernel(const _
     return (blk * a.kv.sb + (key % bs) * a.kv.st + h * a.kv.sh) * a.eb;
   };
   int ek = kScaleMin, ev = kScaleMin;  // exponents of the new page
+  int blk0;
+  const int64_t off0 = locate(0, blk0);
+  int mk = kScaleMin, mv = kScaleMin;  // of the lane's row's page
   if constexpr (F8) {
     for (int r0 = 0; r0 < n; r0 += 32) {
-      int blk;
-      locate(r0, blk);
+      int blk = blk0;
+      if (r0 > 0) locate(r0, blk);
       if (blk >= 0) {
-        ek = max(ek, scale_exponent_of(a.kv.ks[(int64_t)blk * hkv + h]));
-        ev = max(ev, scale_exponent_of(a.kv.vs[(int64_t)blk * hkv + h]));
+        mk = scale_exponent_of(a.kv.ks[(int64_t)blk * hkv + h]);
+        mv = scale_exponent_of(a.kv.vs[(int64_t)blk * hkv + h]);
+        ek = max(ek, mk);
+        ev = max(ev, mv);
       }
     }
     ek = __reduce_max_sync(0xffffffffu, ek);
@@ -196,14 +255,16 @@ __global__ void __launch_bounds__(kGatherWarps * 32) evict_gather_kernel(const _
   uint8_t* const base_v = const_cast<uint8_t*>(pv) + (to * a.kv.sb + h * a.kv.sh) * a.eb;
   const int64_t st = a.kv.st * a.eb;
   for (int r0 = 0; r0 < n; r0 += 32) {
-    int blk;
-    const int64_t off = locate(r0, blk);
+    int blk = blk0;
+    const int64_t off = n > 32 ? locate(r0, blk) : off0;
     float fk = 1.f, fv = 1.f;
     if constexpr (F8) {
-      if (blk >= 0) {
-        fk = pow2(scale_exponent_of(a.kv.ks[(int64_t)blk * hkv + h]) - ek);
-        fv = pow2(scale_exponent_of(a.kv.vs[(int64_t)blk * hkv + h]) - ev);
+      if (n > 32 && blk >= 0) {
+        mk = scale_exponent_of(a.kv.ks[(int64_t)blk * hkv + h]);
+        mv = scale_exponent_of(a.kv.vs[(int64_t)blk * hkv + h]);
       }
+      fk = pow2(mk - ek);
+      fv = pow2(mv - ev);
     }
     const int pieces = min(32, n - r0) * a.chunks;
     for (int e0 = 0; e0 < pieces; e0 += 32 * kBatch) {
@@ -223,7 +284,7 @@ __global__ void __launch_bounds__(kGatherWarps * 32) evict_gather_kernel(const _
       for (int i = 0; i < kBatch; ++i) {
         const int e = e0 + i * 32 + lane, r = min(e / a.chunks, 31);
         if constexpr (F8) {
-          const float mk = __shfl_sync(0xffffffffu, fk, r), mv = __shfl_sync(0xffffffffu, fv, r);
+          const float yk = __shfl_sync(0xffffffffu, fk, r), yv = __shfl_sync(0xffffffffu, fv, r);
           if (from[i] >= 0) {
             uint32_t* wk = reinterpret_cast<uint32_t*>(&xk[i]);
             uint32_t* wv = reinterpret_cast<uint32_t*>(&xv[i]);
@@ -231,9 +292,9 @@ __global__ void __launch_bounds__(kGatherWarps * 32) evict_gather_kernel(const _
             for (int j = 0; j < 4; ++j) {
               float f[4];
               e4m3x4_to_f4(wk[j], f);
-              wk[j] = f4_to_e4m3x4(f[0] * mk, f[1] * mk, f[2] * mk, f[3] * mk);
+              wk[j] = f4_to_e4m3x4(f[0] * yk, f[1] * yk, f[2] * yk, f[3] * yk);
               e4m3x4_to_f4(wv[j], f);
-              wv[j] = f4_to_e4m3x4(f[0] * mv, f[1] * mv, f[2] * mv, f[3] * mv);
+              wv[j] = f4_to_e4m3x4(f[0] * yv, f[1] * yv, f[2] * yv, f[3] * yv);
             }
           }
         }
@@ -357,7 +418,7 @@ __global__ void __launch_bounds__(kThreads) evict_commit_kernel(const __grid_con
 }  // namespace
 
 bool evict_supported(const KvView& kv, const EvictView& e) {
-  return (int64_t)e.S * kv.hkv < (int64_t(1) << 31) && (int64_t)e.W * kv.bs < (int64_t(1) << 30) &&
+  return (int64_t)e.S * kv.hkv < (int64_t(1) << 28) && (int64_t)e.W * kv.bs < (int64_t(1) << 30) &&
          (int64_t)e.S * e.new_pages * kv.hkv / kGatherWarps < (int64_t(1) << 31) - 1;
 }
 
@@ -367,14 +428,33 @@ cudaError_t launch_evict(const KvView& kv, const EvictView& e, int32_t* dev_err,
   a.hkv = kv.hkv;
   a.bs = kv.bs;
   a.dev_err = dev_err;
-  const int64_t row = (int64_t)e.W * kv.bs;
-  constexpr int kCached = 48 * 1024;
-  a.cached = row < kCached ? (int)row : kCached;
+  // Blocks a row: two for each SM in all while their pieces are of 4096 keys or more (32K
+  // keys of 8 heads: 70 us with 1, 14 with 8), and as many as hold the row, if any do:
+  // alone, a block reads what it cannot hold again.
+  constexpr int kCached = 48 * 1024, kMost = 8;
+  const int64_t row = (int64_t)e.W * kv.bs, rows = (int64_t)e.S * kv.hkv;
+  a.parts = 1;
+  while (a.parts < kMost && ((row > (int64_t)a.parts * 4096 && rows * a.parts < 2 * num_sms()) ||
+                             row > (int64_t)a.parts * kCached))
+    a.parts *= 2;
+  if (row > (int64_t)a.parts * kCached) a.parts = 1;
+  const int64_t size = (row + a.parts - 1) / a.parts;
+  a.cached = size < kCached ? (int)size : kCached;
+  if (rows * a.parts >= (int64_t(1) << 31)) return cudaErrorInvalidValue;
   cudaError_t err = cudaFuncSetAttribute(
       evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCached * 4);
   if (err != cudaSuccess) return err;
-  evict_select_kernel<<<e.S * kv.hkv, kThreads, a.cached * 4, s>>>(a);
-  err = cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * a.parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = (size_t)a.cached * 4;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)a.parts, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  err = cudaLaunchKernelEx(&cfg, evict_select_kernel, a);
   if (err != cudaSuccess) return err;
   GatherArgs g;
   g.e = e;
@@ -384,11 +464,8 @@ cudaError_t launch_evict(const KvView& kv, const EvictView& e, int32_t* dev_err,
   g.dev_err = dev_err;
   const int64_t warps = (int64_t)e.S * e.new_pages * kv.hkv;
   const unsigned blocks = (unsigned)((warps + kGatherWarps - 1) / kGatherWarps);
-  if (kv.dtype == CVSA_DTYPE_E4M3)
-    evict_gather_kernel<true><<<blocks, kGatherWarps * 32, 0, s>>>(g);
-  else
-    evict_gather_kernel<false><<<blocks, kGatherWarps * 32, 0, s>>>(g);
-  return cudaGetLastError();
+  return launch_k(kv.dtype == CVSA_DTYPE_E4M3 ? evict_gather_kernel<true> : evict_gather_kernel<false>,
+                  dim3(blocks), dim3(kGatherWarps * 32), 0, s, true, g);
 }
 
 cudaError_t launch_evict_reserve(const EvictPages& p, int32_t* dev_err, cudaStream_t s) {
