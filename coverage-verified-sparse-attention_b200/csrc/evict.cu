@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
   extern __shared__ float piece[];  // [cached]
   __shared__ int hist[2][kBins];
   __shared__ int sums[32];
-  __shared__ int s_bin, s_left;
+  __shared__ int s_bin, s_left, s_all;
   __shared__ int counts[2];  // of this piece: taken above the cut or in any case, equal to it
   const cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, parts = a.parts, part = blockIdx.x % parts;
@@ -106,15 +106,22 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
         const bool first = before + c0 >= left;
         s_bin = first ? top : top - 1;
         s_left = left - (first ? before : before + c0);
+        s_all = s_left == (first ? c0 : c1);
       }
       __syncthreads();
       prefix |= (uint32_t)s_bin << shift;
       mask |= (uint32_t)((1 << bits) - 1) << shift;
       left = s_left;
+      const bool all = s_all && prefix > 0;
       __syncthreads();
+      cut = prefix;
+      room = left;
+      if (all) {  // the whole bin is taken (22 bits mostly tell weights apart): no more passes
+        cut = prefix - 1;
+        room = 0;
+        break;
+      }
     }
-    cut = prefix;
-    room = left;
   } else {
     __syncthreads();
   }
@@ -428,13 +435,12 @@ cudaError_t launch_evict(const KvView& kv, const EvictView& e, int32_t* dev_err,
   a.hkv = kv.hkv;
   a.bs = kv.bs;
   a.dev_err = dev_err;
-  // Blocks a row: two for each SM in all while their pieces are of 4096 keys or more (32K
-  // keys of 8 heads: 70 us with 1, 14 with 8), and as many as hold the row, if any do:
-  // alone, a block reads what it cannot hold again.
+  // Blocks a row: two for each SM in all while their pieces are of 8192 keys or more, and as
+  // many as hold the row, if any do: alone, a block reads what it cannot hold again.
   constexpr int kCached = 48 * 1024, kMost = 8;
   const int64_t row = (int64_t)e.W * kv.bs, rows = (int64_t)e.S * kv.hkv;
   a.parts = 1;
-  while (a.parts < kMost && ((row > (int64_t)a.parts * 4096 && rows * a.parts < 2 * num_sms()) ||
+  while (a.parts < kMost && ((row > (int64_t)a.parts * 8192 && rows * a.parts < 2 * num_sms()) ||
                              row > (int64_t)a.parts * kCached))
     a.parts *= 2;
   if (row > (int64_t)a.parts * kCached) a.parts = 1;
