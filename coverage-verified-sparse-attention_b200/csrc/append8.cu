@@ -138,14 +138,8 @@ __device__ __forceinline__ void page_block(const Append8Args& a, int bid) {
     if (tid == 0) set_dev_error(a.dev_err, CVSA_DEV_ERR_RAGGED);
     return;
   }
-  const int blk = a.rg.tables[(int64_t)slot * a.rg.W + page];
-  if (blk < 0 || blk >= a.kv.num_blocks) {
-    if (tid == 0) set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);
-    return;
-  }
+  const int blk = a.rg.tables[(int64_t)slot * a.rg.W + page];  // looked at behind the rows' loads
   const int r0 = (int)max((int64_t)0, p0 - page * bs), r1 = (int)min((int64_t)bs, p1 - page * bs);
-  float* const scale = const_cast<float*>(is_k ? a.kv.ks : a.kv.vs) + (int64_t)blk * hkv + h;
-  const int had = r0 > 0 ? scale_exponent_of(*scale) : kScaleMin;
   const int64_t shift = a.r.shift ? a.r.shift[slot] : 0;
   const Runs e(a.r, u);
   const void* const src = is_k ? a.r.k : a.r.v;
@@ -186,6 +180,12 @@ __device__ __forceinline__ void page_block(const Append8Args& a, int bid) {
       top = ok && m <= 3.402823466e38f ? fmaxf(top, m) : top;
     }
   }
+  if (blk < 0 || blk >= a.kv.num_blocks) {
+    if (tid == 0) set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);
+    return;
+  }
+  float* const scale = const_cast<float*>(is_k ? a.kv.ks : a.kv.vs) + (int64_t)blk * hkv + h;
+  const int had = r0 > 0 ? scale_exponent_of(*scale) : kScaleMin;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (tid % 32 == 0) s_max[tid / 32] = top;
@@ -227,7 +227,7 @@ __device__ __forceinline__ void page_block(const Append8Args& a, int bid) {
 }
 
 template <typename T, int U>
-__global__ void __launch_bounds__(kThreads) append8_kernel(const __grid_constant__ Append8Args a) {
+__global__ void __launch_bounds__(kThreads, 10) append8_kernel(const __grid_constant__ Append8Args a) {
   if ((int)blockIdx.x < a.page_blocks)
     page_block<T, U>(a, blockIdx.x);
   else

@@ -416,11 +416,13 @@ class _ArgMemory(threading.local):
         self.chunk = ChunkAttend.from_buffer(self.buf, 120)
         self.rope = RopeAppend.from_buffer(self.buf, 120)
         self.weights = KeyWeights.from_buffer(self.buf, 120)
+        self.evict = Evict.from_buffer(self.buf, 64)
         self.pack_chunk = struct.Struct("<" + self._KV + self._RG + "QQQiiqqqqfii").pack_into
         self.pack_rope = struct.Struct("<" + self._KV + self._RG
                                        + "QQQQiiqqqqqqqqQiiiiQQf").pack_into
         self.pack_weights = struct.Struct("<" + self._KV + self._RG
                                           + "QQiiqqffiiQQq").pack_into
+        self.pack_evict = struct.Struct("<" + self._KV + "QqQqQi4xQiii4x").pack_into
 
 
 ARGS = _ArgMemory()

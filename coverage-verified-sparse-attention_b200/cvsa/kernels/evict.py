@@ -6,6 +6,7 @@ the last ones and those of largest weight between, and moves them to new pages
 The reference has no counterpart: it keeps every page and reads few of them.
 """
 
+import struct
 from typing import Optional
 
 import torch
@@ -40,8 +41,9 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tens
     scaled = k_scale is not None
     if scaled != (v_scale is not None):
         raise ValueError("k_scale and v_scale go together")
-    kv = _lib.KvDesc(*_lib.kv_fields(k_cache, v_cache, scaled))
-    i32 = torch.int32
+    i32, f32, mem = torch.int32, torch.float32, _lib.ARGS
+    kv = _lib.kv_fields(k_cache, v_cache, scaled)
+    page, H = kv[4], kv[5]
     for t in (block_tables, context_lens, new_tables):
         if t.dtype is not i32 or not t.is_contiguous():
             raise ValueError("block_tables, context_lens and new_tables must be contiguous int32")
@@ -50,31 +52,34 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tens
     if not 0 < keep < 2 ** 31 or not 0 <= sink <= keep or not 0 <= recent <= keep - sink:
         raise ValueError("keep must be positive, sink and recent >= 0 and together at most keep")
     S, W = block_tables.shape
-    H = k_cache.shape[2]
-    if new_tables.shape != (S, -(-keep // k_cache.shape[1])):
+    if new_tables.shape != (S, -(-keep // page)):
         raise ValueError("new_tables must be [num_seqs, ceil(keep / block_size)]")
     if out_weights is None:
         out_weights = weights
-    elif _overlap(weights, out_weights) and (
-            weights.data_ptr() != out_weights.data_ptr() or weights.shape != out_weights.shape):
-        raise ValueError("out_weights must be weights itself or memory of its own")
     for t in (weights, out_weights):
-        if (t.dim() != 3 or t.dtype is not torch.float32 or not t.is_contiguous()
-                or t.shape[:2] != (S, H)):
+        if t.dim() != 3 or t.dtype is not f32 or not t.is_contiguous() or t.shape[:2] != (S, H):
             raise ValueError("weights and out_weights must be contiguous float32 "
                              "[num_seqs, H_kv, keys]")
+    w, o = weights.data_ptr(), out_weights.data_ptr()
+    if out_weights is not weights and _overlap(weights, out_weights) and (
+            w != o or weights.shape != out_weights.shape):
+        raise ValueError("out_weights must be weights itself or memory of its own")
     if kept is None:
         kept = torch.empty((S, H, keep), dtype=i32, device=weights.device)
     elif kept.shape != (S, H, keep) or kept.dtype is not i32 or not kept.is_contiguous():
         raise ValueError("kept must be a contiguous int32 [num_seqs, H_kv, keep]")
-    args = _lib.Evict(weights.data_ptr(), weights.shape[2], out_weights.data_ptr(),
-                      out_weights.shape[2], new_tables.data_ptr(), new_tables.shape[1],
-                      kept.data_ptr(), keep, sink, recent)
-    _lib.check(_lib.load().cvsa_evict(
-        kv, _lib.scale_ptr(k_scale, k_cache, "k_scale"),
+    try:
+        mem.pack_evict(mem.buf, 0, *kv, w, weights.shape[2], o, out_weights.shape[2],
+                       new_tables.data_ptr(), new_tables.shape[1], kept.data_ptr(), keep, sink,
+                       recent)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"evict: an argument is out of range ({e})") from None
+    st = _lib.load().cvsa_evict(
+        mem.kv, _lib.scale_ptr(k_scale, k_cache, "k_scale"),
         _lib.scale_ptr(v_scale, k_cache, "v_scale"), block_tables.data_ptr(),
-        context_lens.data_ptr(), S, W, args, _lib.ptr(dev_error), _lib.raw_stream(dev)),
-        "cvsa_evict")
+        context_lens.data_ptr(), S, W, mem.evict, _lib.ptr(dev_error), _lib.raw_stream(dev))
+    if st:
+        _lib.check(st, "cvsa_evict")
     return kept
 
 
