@@ -8,9 +8,9 @@
 // so that a thread owns a key and its sum over rows never leaves it. The scores of the
 // next rows form while these are summed; the next item's keys are loaded meanwhile. 8-bit
 // keys are widened to the queries' type as they are copied, once an item.
-// Roles: warps 0-3 and 4-7 sum the first and the second tile, warps 8-11 load keys, warp
-// 12 issues the products, warps 13 and 14 load queries with their log-sum-exps and
-// positions. Each follows the same list of items on its own.
+// Roles: warps 0-3 and 4-7 sum the first and the second tile of an item's even steps, warps
+// 8-15 of its odd ones, warps 16-19 load keys, warp 20 issues the products,
+// warps 21 and 22 load queries and their log-sum-exps. Each follows the same list of items on its own.
 // Bound by the exponentials (16 a clock and SM; 256 tokens of 32 heads at 32K keys: 60 us
 // of them, against 41 us of products at the tensor cores' rate).
 #include <cstddef>
@@ -26,17 +26,18 @@
 namespace cvsa {
 namespace {
 
-constexpr int kThreads = 512, kTile = 128, kKeys = 2 * kTile, kRing = 8;
+constexpr int kThreads = 768, kTile = 128, kKeys = 2 * kTile, kRing = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct WMeta {
   uint64_t k_full[2], k_empty[2], q_full[2], q_copied[2], q_empty[2], drain;
   uint64_t s_full[2][2], s_free[2][2];  // buffer, tile
-  // rows of a step, in a ring: the rows of step n are written over once the products of
-  // step n + kRing - 2 are done, which wait for scores of step n + kRing - 4 to be taken
-  // by every warp that sums, and so for its sums of step n
+  uint64_t joined[2][2], taken[2][2];   // items in turn, tile: the second group's sums
+  // rows of a step, in a ring: those of step n are written over once the products of step
+  // n + 2 are done, which wait for the sums of step n
   alignas(16) float c[kRing][kTile];  // minus the log-sum-exp
   uint32_t live[kRing][4];            // bit per row that takes part (is there, saw a key)
+  float second[2][2][kTile];          // items in turn, tile: the second group's sums
   uint32_t tmem, abort;
 };
 static_assert(offsetof(WMeta, c) % 16 == 0, "wide loads");
@@ -255,7 +256,10 @@ __device__ __forceinline__ void query_role(const WArgs& a, WMeta* m, uint32_t ba
   __syncwarp();
 }
 
-// The whole warp runs the loop, one elected lane issues.
+// The whole warp runs the loop, its conditions broadcast, so that the compiler keeps the
+// descriptors in uniform registers, where the instruction wants them; one elected lane issues.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 template <typename T, int D>
 __device__ __forceinline__ void mma_role(const WArgs& a, WMeta* m, uint32_t base, uint32_t tmem,
                                          WeightWalk walk) {
@@ -263,10 +267,10 @@ __device__ __forceinline__ void mma_role(const WArgs& a, WMeta* m, uint32_t base
   constexpr uint32_t kId = mma_idesc(!std::is_same<T, __half>::value, kTile, kTile, false);
   const uint64_t k_desc = smem_desc(base, 16, 1024), q_desc = smem_desc(base + C::kQ, 16, 1024);
   uint32_t nk = 0, n = 0;
-  for (; walk.next(a.rg, a.g); walk.step()) {
+  for (; uniform(walk.next(a.rg, a.g)); walk.step()) {
     int t0, t1;
     weight_tokens(walk.q, a.g, walk.i, t0, t1);
-    const int steps = __shfl_sync(0xffffffffu, (t1 - t0 + a.P - 1) / a.P, 0);
+    const int steps = uniform((t1 - t0 + a.P - 1) / a.P);
     if (steps <= 0) continue;
     const uint32_t kb = nk & 1;
     if (!warp_wait(&m->k_full[kb], (nk >> 1) & 1, m, a)) goto out;
@@ -310,12 +314,14 @@ __device__ __forceinline__ uint32_t bits_of(int from, int to, int x) {
   return a >= 32 || b <= a ? 0u : (b >= 32 ? ~0u : (1u << b) - 1) & (~0u << a);
 }
 
+// Two groups of warps take an item's steps in turn, so that one's waits fall beside the
+// other's exponentials.
 __device__ __forceinline__ void sum_role(const WArgs& a, WMeta* m, uint32_t tmem, WeightWalk walk,
-                                         int mt) {
+                                         int mt, int group) {
   const int warp = threadIdx.x >> 5 & 3, lane = threadIdx.x & 31, G = a.g.G;
   const uint64_t sc = f2_pack(a.w.scale, a.w.scale), l2 = f2_pack(kLog2e, kLog2e);
-  uint32_t n = 0;
-  for (; walk.next(a.rg, a.g); walk.step()) {
+  uint32_t n = 0, items = 0;
+  for (; walk.next(a.rg, a.g); walk.step(), ++items) {
     const SeqInfo& q = walk.q;
     int t0, t1;
     weight_tokens(q, a.g, walk.i, t0, t1);
@@ -324,13 +330,15 @@ __device__ __forceinline__ void sum_role(const WArgs& a, WMeta* m, uint32_t tmem
     const bool there = key < q.ctx;
     const int64_t at = ((int64_t)q.slot * a.kv.hkv + walk.h) * a.w.stride + key;
     // what the key had and its page, not looked at before the sums are done
-    const float prior = there && key < q.start ? a.w.prior[at] : 0.f;
-    const int blk = there ? a.rg.tables[(int64_t)q.slot * a.rg.W + key / a.g.bs] : -1;
+    const float prior = group == 0 && there && key < q.start ? a.w.prior[at] : 0.f;
+    const int blk = group == 0 && there ? a.rg.tables[(int64_t)q.slot * a.rg.W + key / a.g.bs] : -1;
     // the tokens that see the key: ta and those after it, up to tb
     const int see0 = a.g.causal ? key - q.start : 0;
     const int see1 = a.g.window > 0 ? see0 + a.g.window : q.n;
     float total = 0.f;
-    for (int ta = t0; ta < t1; ta += a.P, ++n) {
+    int mine = group;  // 0: this step is the group's
+    for (int ta = t0; ta < t1; ta += a.P, ++n, mine ^= 1) {
+      if (mine) continue;
       const uint32_t b = n & 1, slot = n % kRing;
       const int tokens = min(a.P, t1 - ta), rows = tokens * G;
       // some row does not see every key of the tile
@@ -350,11 +358,6 @@ __device__ __forceinline__ void sum_role(const WArgs& a, WMeta* m, uint32_t tmem
         const uint32_t sees = bits_of(from, to, x) & m->live[slot][x / 32];
         const bool all = __all_sync(0xffffffffu, sees == ~0u);
         tmem_wait_ld();
-        if (x + 32 >= rows) {  // the next products may go there
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&m->s_free[b][mt]);
-        }
         const float4* const c4 = reinterpret_cast<const float4*>(m->c[slot] + x);
         if (all) {
 #pragma unroll
@@ -378,10 +381,26 @@ __device__ __forceinline__ void sum_role(const WArgs& a, WMeta* m, uint32_t tmem
           sum0 = f2_add(sum0, f2_pack(add, 0.f));
         }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m->s_free[b][mt]);  // the next products may go there
       float u, v;
       f2_unpack(f2_add(sum0, sum1), u, v);
       total += u + v;
     }
+    const uint32_t ib = items & 1, turn = (items >> 1) & 1;
+    float* const other = &m->second[ib][mt][warp * 32 + lane];
+    if (group) {
+      if (!warp_wait(&m->taken[ib][mt], turn ^ 1, m, a)) return;
+      *other = total;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m->joined[ib][mt]);
+      continue;
+    }
+    if (!warp_wait(&m->joined[ib][mt], turn, m, a)) return;
+    total += *other;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&m->taken[ib][mt]);
     if (there) {
       const float had = a.w.decay * prior;
       a.w.out[at] = blk >= 0 && blk < a.kv.num_blocks ? had + total : had;
@@ -407,13 +426,15 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
       for (int mt = 0; mt < 2; ++mt) {
         mbar_init(&m->s_full[i][mt], 1);
         mbar_init(&m->s_free[i][mt], 4);
+        mbar_init(&m->joined[i][mt], 4);
+        mbar_init(&m->taken[i][mt], 4);
       }
     }
     mbar_init(&m->drain, 1);
     m->abort = 0;
     fence_mbar_init();
   }
-  if (warp == 12) tmem_alloc(smem_u32(&m->tmem), 512);
+  if (warp == 20) tmem_alloc(smem_u32(&m->tmem), 512);
   const WeightRange r = weight_range(a.rg, a.g, blockIdx.x, gridDim.x,
                                      warp == 0 ? a.dev_err : nullptr);
   tc_fence_before();
@@ -421,13 +442,13 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
   tc_fence_after();
   const uint32_t base = smem_u32(smem), tmem = __shfl_sync(0xffffffffu, m->tmem, 0);
   const WeightWalk walk(r);
-  if (warp < 8) sum_role(a, m, tmem, walk, warp / 4);
-  else if (warp < 12) key_role<T, D, F8>(a, m, base, walk, warp - 8);
-  else if (warp == 12) mma_role<T, D>(a, m, base, tmem, walk);
-  else if (warp < 15) query_role<D>(a, m, base, walk, warp - 13);
+  if (warp < 16) sum_role(a, m, tmem, walk, warp / 4 & 1, warp / 8);
+  else if (warp < 20) key_role<T, D, F8>(a, m, base, walk, warp - 16);
+  else if (warp == 20) mma_role<T, D>(a, m, base, tmem, walk);
+  else if (warp < 23) query_role<D>(a, m, base, walk, warp - 21);
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 20) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
