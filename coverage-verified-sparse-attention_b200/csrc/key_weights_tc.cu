@@ -3,8 +3,10 @@
 // weights_plan.cuh.
 //
 // A persistent CTA an SM. An item is 256 keys of one KV head, kept in shared memory as two
-// tiles of M, against the rows that see them, 128 at a time (N):
-//   S' = K Q'   (fp32 in tensor memory, two buffers of two tiles)
+// tiles of M, against the rows that see them, 64 at a time (N):
+//   S' = K Q'   (fp32 in tensor memory, two buffers of two tiles, each half of the elements
+//                a sum of its own: the tensor core cuts where an addition rounds, and one sum
+//                of 128 products left twice the error of fp32's own)
 // so that a thread owns a key and its sum over rows never leaves it. The scores of the
 // next rows form while these are summed; the next item's keys are loaded meanwhile. 8-bit
 // keys are widened to the queries' type as they are copied, once an item.
@@ -26,17 +28,19 @@
 namespace cvsa {
 namespace {
 
-constexpr int kThreads = 768, kTile = 128, kKeys = 2 * kTile, kRing = 4;
+constexpr int kThreads = 768, kTile = 128, kKeys = 2 * kTile, kRows = 64;
+constexpr int kQBufs = 4, kRing = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct WMeta {
-  uint64_t k_full[2], k_empty[2], q_full[2], q_copied[2], q_empty[2], drain;
+  uint64_t k_full[2], k_empty[2], q_full[kQBufs], q_copied[kQBufs], q_empty[kQBufs], drain;
   uint64_t s_full[2][2], s_free[2][2];  // buffer, tile
   uint64_t joined[2][2], taken[2][2];   // items in turn, tile: the second group's sums
   // rows of a step, in a ring: those of step n are written over once the products of step
-  // n + 2 are done, which wait for the sums of step n
-  alignas(16) float c[kRing][kTile];  // minus the log-sum-exp
-  uint32_t live[kRing][4];            // bit per row that takes part (is there, saw a key)
+  // n + 4 are done. By then the sums of n are: one of the steps between waits for n's
+  // buffer, or for group 0 to be done with a step of a later item than n's.
+  alignas(16) float c[kRing][kRows];  // minus the log-sum-exp
+  uint32_t live[kRing][2];            // bit per row that takes part (is there, saw a key)
   float second[2][2][kTile];          // items in turn, tile: the second group's sums
   uint32_t tmem, abort;
 };
@@ -93,7 +97,8 @@ template <int D>
 struct WCfg {
   static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kQ = 4 * kTileBytes;                // two buffers of two K tiles first
-  static constexpr int kMeta = kQ + 2 * kTileBytes;
+  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kMeta = kQ + kQBufs * kQBytes;
   static constexpr int kSmem = kMeta + (int)sizeof(WMeta) + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -192,21 +197,16 @@ __device__ __forceinline__ void key_role(const WArgs& a, WMeta* m, uint32_t base
 
 // A step's query rows, (token, head of the group) in order, are a tile of their array: one
 // tensor copy for each 64 elements. What else a step needs of them is written by two
-// warps, 64 rows each; the next step's is looked up while this step's is on its way.
+// warps, 32 rows each; the next step's is looked up while this step's is on its way.
 template <int D>
 __device__ __forceinline__ void query_role(const WArgs& a, WMeta* m, uint32_t base, WeightWalk walk,
                                            int w) {
   using C = WCfg<D>;
   const int lane = threadIdx.x & 31, G = a.g.G;
-  int rt[2], rh[2];  // token and head of rows w * 64 + 32 k + lane
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    rt[k] = (w * 64 + k * 32 + lane) / G;
-    rh[k] = w * 64 + k * 32 + lane - rt[k] * G;
-  }
+  const int r = w * 32 + lane, rt = r / G, rh = r - rt * G;  // row, its token and head
   int ta = 0, t0 = 0, t1 = 0;
   bool more = true, first = true;
-  float lse[2];
+  float lse = neg_inf();
   auto look = [&]() {  // the first step, or the next one; more: there is one
     if (!first) ta += a.P;
     while (more && ta >= t1) {
@@ -218,41 +218,34 @@ __device__ __forceinline__ void query_role(const WArgs& a, WMeta* m, uint32_t ba
         ta = t0;
       }
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      lse[k] = neg_inf();
-      if (more && rt[k] < min(a.P, t1 - ta))
-        lse[k] = a.w.lse[(int64_t)(walk.q.tok0 + ta + rt[k]) * a.w.hq + walk.h * G + rh[k]];
-    }
+    lse = neg_inf();
+    if (more && rt < min(a.P, t1 - ta))
+      lse = a.w.lse[(int64_t)(walk.q.tok0 + ta + rt) * a.w.hq + walk.h * G + rh];
   };
   look();
   uint32_t n = 0;
   for (; more; ++n) {
-    const uint32_t buf = n & 1, slot = n % kRing;
-    if (!warp_wait(&m->q_empty[buf], ((n >> 1) & 1) ^ 1, m, a)) break;
+    const uint32_t buf = n % kQBufs, slot = n % kRing;
+    if (!warp_wait(&m->q_empty[buf], ((n / kQBufs) & 1) ^ 1, m, a)) break;
     if (w == 0 && elect_one()) {
       mbar_arrive_expect_tx(&m->q_copied[buf], a.P * G * D * 2);
 #pragma unroll
       for (int x = 0; x < D; x += 64)
-        token_load(base + C::kQ + buf * C::kTileBytes + x / 64 * (kTile * 128), &a.q_map, x,
+        token_load(base + C::kQ + buf * C::kQBytes + x / 64 * (kRows * 128), &a.q_map, x,
                    walk.h * G, walk.q.tok0 + ta, &m->q_copied[buf]);
     }
     __syncwarp();
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int r = w * 64 + k * 32 + lane;
-      const bool live = lse[k] != neg_inf();
-      m->c[slot][r] = live ? -lse[k] : neg_inf();
-      const uint32_t bits = __ballot_sync(0xffffffffu, live);
-      if (lane == 0) m->live[slot][w * 2 + k] = bits;
-    }
+    const bool live = lse != neg_inf();
+    m->c[slot][r] = live ? -lse : neg_inf();
+    const uint32_t bits = __ballot_sync(0xffffffffu, live);
+    if (lane == 0) m->live[slot][w] = bits;
     mbar_arrive(&m->q_full[buf]);
     look();
   }
   // no copy outlives the CTA, whatever gave up
   if (w == 0)
-    for (uint32_t i = n > 2 ? n - 2 : 0; i < n; ++i)
-      mbar_wait_bounded(&m->q_copied[i & 1], (i >> 1) & 1, 1u << 18);
+    for (uint32_t i = n > kQBufs ? n - kQBufs : 0; i < n; ++i)
+      mbar_wait_bounded(&m->q_copied[i % kQBufs], (i / kQBufs) & 1, 1u << 18);
   __syncwarp();
 }
 
@@ -264,9 +257,9 @@ template <typename T, int D>
 __device__ __forceinline__ void mma_role(const WArgs& a, WMeta* m, uint32_t base, uint32_t tmem,
                                          WeightWalk walk) {
   using C = WCfg<D>;
-  constexpr uint32_t kId = mma_idesc(!std::is_same<T, __half>::value, kTile, kTile, false);
+  constexpr uint32_t kId = mma_idesc(!std::is_same<T, __half>::value, kTile, kRows, false);
   const uint64_t k_desc = smem_desc(base, 16, 1024), q_desc = smem_desc(base + C::kQ, 16, 1024);
-  uint32_t nk = 0, n = 0;
+  uint32_t nk = 0, n = 0, odd = 0;  // bit b: buffer b was used an odd number of times
   for (; uniform(walk.next(a.rg, a.g)); walk.step()) {
     int t0, t1;
     weight_tokens(walk.q, a.g, walk.i, t0, t1);
@@ -275,28 +268,32 @@ __device__ __forceinline__ void mma_role(const WArgs& a, WMeta* m, uint32_t base
     const uint32_t kb = nk & 1;
     if (!warp_wait(&m->k_full[kb], (nk >> 1) & 1, m, a)) goto out;
     for (int j = 0; j < steps; ++j, ++n) {
-      const uint32_t b = n & 1;
-      if (!warp_wait(&m->q_full[b], (n >> 1) & 1, m, a)) goto out;
-      if (!warp_wait(&m->q_copied[b], (n >> 1) & 1, m, a)) goto out;
+      const uint32_t b = j & 1, qb = n % kQBufs, turn = (n / kQBufs) & 1;
+      if (!warp_wait(&m->q_full[qb], turn, m, a)) goto out;
+      if (!warp_wait(&m->q_copied[qb], turn, m, a)) goto out;
       fence_proxy_async_smem();  // the tiles were written through the generic proxy
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        if (!warp_wait(&m->s_free[b][mt], ((n >> 1) & 1) ^ 1, m, a)) goto out;
+        if (!warp_wait(&m->s_free[b][mt], (odd >> b & 1) ^ 1, m, a)) goto out;
         tc_fence_after();
         if (elect_one()) {
           const uint64_t kd = k_desc + (((kb * 2 + mt) * C::kTileBytes) >> 4);
-          const uint64_t qd = q_desc + ((b * C::kTileBytes) >> 4);
+          const uint64_t qd = q_desc + ((qb * C::kQBytes) >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t o = ((kk / 4) * (kTile * 128) + (kk % 4) * 32) >> 4;
-            mma_ss(tmem + (b * 2 + mt) * kTile, kd + o, qd + o, kId, kk > 0);
+            const uint32_t ko = ((kk / 4) * (kTile * 128) + (kk % 4) * 32) >> 4;
+            const uint32_t qo = ((kk / 4) * (kRows * 128) + (kk % 4) * 32) >> 4;
+            constexpr int kHalf = D / 32;  // each half of the elements has a sum of its own
+            mma_ss(tmem + (b * 2 + mt) * 2 * kRows + kk / kHalf * kRows, kd + ko, qd + qo, kId,
+                   kk % kHalf > 0);
           }
           mma_commit(smem_u32(&m->s_full[b][mt]));
-          if (mt) mma_commit(smem_u32(&m->q_empty[b]));
+          if (mt) mma_commit(smem_u32(&m->q_empty[qb]));
           if (mt && j == steps - 1) mma_commit(smem_u32(&m->k_empty[kb]));
         }
         __syncwarp();
       }
+      odd ^= 1u << b;
     }
     ++nk;
   }
@@ -314,13 +311,15 @@ __device__ __forceinline__ uint32_t bits_of(int from, int to, int x) {
   return a >= 32 || b <= a ? 0u : (b >= 32 ? ~0u : (1u << b) - 1) & (~0u << a);
 }
 
-// Two groups of warps take an item's steps in turn, so that one's waits fall beside the
-// other's exponentials.
+// Two groups of warps take an item's steps in turn, each those of its own buffer of scores,
+// so that one's waits fall beside the other's exponentials. (A buffer is one group's: a
+// barrier's parity says which of two phases is done, so who waits on it may not leave out
+// a phase.)
 __device__ __forceinline__ void sum_role(const WArgs& a, WMeta* m, uint32_t tmem, WeightWalk walk,
                                          int mt, int group) {
   const int warp = threadIdx.x >> 5 & 3, lane = threadIdx.x & 31, G = a.g.G;
   const uint64_t sc = f2_pack(a.w.scale, a.w.scale), l2 = f2_pack(kLog2e, kLog2e);
-  uint32_t n = 0, items = 0;
+  uint32_t n = 0, items = 0, turns = 0;  // turns: steps of this group
   for (; walk.next(a.rg, a.g); walk.step(), ++items) {
     const SeqInfo& q = walk.q;
     int t0, t1;
@@ -339,43 +338,48 @@ __device__ __forceinline__ void sum_role(const WArgs& a, WMeta* m, uint32_t tmem
     int mine = group;  // 0: this step is the group's
     for (int ta = t0; ta < t1; ta += a.P, ++n, mine ^= 1) {
       if (mine) continue;
-      const uint32_t b = n & 1, slot = n % kRing;
+      const uint32_t b = group, slot = n % kRing;
       const int tokens = min(a.P, t1 - ta), rows = tokens * G;
       // some row does not see every key of the tile
       const bool partial = (a.g.causal && q.start + ta < last) ||
                            (a.g.window > 0 && first <= q.start + ta + tokens - 1 - a.g.window);
       // rows [from, to) see the key
       const int from = partial ? min(max(see0 - ta, 0), a.P) * G : 0;
-      const int to = partial ? min(max(see1 - ta, 0), a.P) * G : kTile;
-      if (!warp_wait(&m->s_full[b][mt], (n >> 1) & 1, m, a)) return;
+      const int to = partial ? min(max(see1 - ta, 0), a.P) * G : kRows;
+      if (!warp_wait(&m->s_full[b][mt], turns & 1, m, a)) return;
+      ++turns;
       tc_fence_after();
-      const uint32_t ts = tmem + (b * 2 + mt) * kTile + ((uint32_t)(warp * 32) << 16);
+      const uint32_t ts = tmem + (b * 2 + mt) * 2 * kRows + ((uint32_t)(warp * 32) << 16);
       uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll 1
-      for (int x = 0; x < rows; x += 32) {
-        float s[32];
-        tmem_ld32(ts + x, s);
-        const uint32_t sees = bits_of(from, to, x) & m->live[slot][x / 32];
-        const bool all = __all_sync(0xffffffffu, sees == ~0u);
+      for (int x = 0; x < rows; x += 16) {
+        float s[16], s2[16];
+        tmem_ld16(ts + x, s);
+        tmem_ld16(ts + kRows + x, s2);
+        const uint32_t sees = (bits_of(from, to, x) & m->live[slot][x / 32] >> x % 32) & 0xffff;
+        const bool all = __all_sync(0xffffffffu, sees == 0xffff);
         tmem_wait_ld();
         const float4* const c4 = reinterpret_cast<const float4*>(m->c[slot] + x);
         if (all) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 4; ++i) {
             const float4 c = c4[i];
             float u, v;
-            f2_unpack(f2_mul(f2_fma(f2_pack(s[4 * i], s[4 * i + 1]), sc, f2_pack(c.x, c.y)), l2), u, v);
+            const uint64_t lo = f2_add(f2_pack(s[4 * i], s[4 * i + 1]), f2_pack(s2[4 * i], s2[4 * i + 1]));
+            f2_unpack(f2_mul(f2_fma(lo, sc, f2_pack(c.x, c.y)), l2), u, v);
             sum0 = f2_add(sum0, f2_pack(ex2(u), ex2(v)));
-            f2_unpack(f2_mul(f2_fma(f2_pack(s[4 * i + 2], s[4 * i + 3]), sc, f2_pack(c.z, c.w)), l2), u, v);
+            const uint64_t hi = f2_add(f2_pack(s[4 * i + 2], s[4 * i + 3]),
+                                       f2_pack(s2[4 * i + 2], s2[4 * i + 3]));
+            f2_unpack(f2_mul(f2_fma(hi, sc, f2_pack(c.z, c.w)), l2), u, v);
             sum1 = f2_add(sum1, f2_pack(ex2(u), ex2(v)));
           }
         } else if (__any_sync(0xffffffffu, sees != 0)) {
           float add = 0.f;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < 16; ++i) {
             const float4 c = c4[i / 4];
             const float y = i % 4 == 0 ? c.x : i % 4 == 1 ? c.y : i % 4 == 2 ? c.z : c.w;
-            const float e = ex2(fmaf(s[i], a.w.scale, y) * kLog2e);
+            const float e = ex2(fmaf(s[i] + s2[i], a.w.scale, y) * kLog2e);
             add += sees >> i & 1 ? e : 0.f;
           }
           sum0 = f2_add(sum0, f2_pack(add, 0.f));
@@ -420,15 +424,17 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
     for (int i = 0; i < 2; ++i) {
       mbar_init(&m->k_full[i], 128);
       mbar_init(&m->k_empty[i], 1);
-      mbar_init(&m->q_full[i], 64);  // the plain writes
-      mbar_init(&m->q_copied[i], 1);
-      mbar_init(&m->q_empty[i], 1);
       for (int mt = 0; mt < 2; ++mt) {
         mbar_init(&m->s_full[i][mt], 1);
         mbar_init(&m->s_free[i][mt], 4);
         mbar_init(&m->joined[i][mt], 4);
         mbar_init(&m->taken[i][mt], 4);
       }
+    }
+    for (int i = 0; i < kQBufs; ++i) {
+      mbar_init(&m->q_full[i], 64);  // the plain writes
+      mbar_init(&m->q_copied[i], 1);
+      mbar_init(&m->q_empty[i], 1);
     }
     mbar_init(&m->drain, 1);
     m->abort = 0;
@@ -488,7 +494,7 @@ cudaError_t launch_weights_tc(const KvView& kv, const RaggedView& rg, const KeyW
   a.g.hkv = kv.hkv;
   a.g.G = w.hq / kv.hkv;
   a.g.KT = kKeys;
-  a.P = kTile / a.g.G;
+  a.P = kRows / a.g.G;
   a.g.rows = a.P * a.g.G;
   a.g.fixed = 1;
   a.g.causal = w.causal;
