@@ -13,6 +13,7 @@ from typing import Optional
 import torch
 
 from cvsa import _lib
+from cvsa.kernels.evict import _overlap
 
 _ALL = 2 ** 31 - 1  # keys: more than a sequence can hold
 
@@ -58,6 +59,8 @@ def key_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor,
                 or t.shape != weights.shape):
             raise ValueError("weights and out must be contiguous float32 "
                              "[num_seqs, H_kv, capacity]")
+    if out is not weights and out.data_ptr() != weights.data_ptr() and _overlap(weights, out):
+        raise ValueError("out must be weights itself or memory of its own")
     qs, mem = q.stride(), _lib.ARGS
     try:
         mem.pack_weights(mem.buf, 0, *_lib.kv_fields(k_cache, k_cache, k_scale is not None),

@@ -223,6 +223,9 @@ class SequenceKVManager:
         adds to new tokens' positions. The first `evict` does it too; call it before a
         graph is captured that is to see later evictions."""
         if self.evicted is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("track_evictions: call it before the graph is captured, which "
+                                   "would count from 0 at every replay")
             self.evicted = torch.zeros_like(self.context_lens)
         return self.evicted
 
@@ -248,7 +251,8 @@ class SequenceKVManager:
             i32 = torch.int32
             plan = (torch.empty((self.batch_size, pages), dtype=i32, device=dev),
                     torch.empty((self.batch_size,), dtype=i32, device=dev))
-            self._evict_plan[pages] = plan
+            if not torch.cuda.is_current_stream_capturing():  # else memory of the graph
+                self._evict_plan[pages] = plan
         new_tables, lens = plan
         args = _lib.EvictPages(
             self.block_tables.data_ptr(), self.context_lens.data_ptr(),

@@ -310,3 +310,13 @@ def test_eight_bit_cache_has_scales():
     c = PagedKVCache(8, 16, 2, 64, dtype=F8, device="cpu")
     assert c.k_scale.shape == c.v_scale.shape == (8, 2) and c.k_cache.dtype is F8
     assert PagedKVCache(8, 16, 2, 64, device="cpu").k_scale is None
+
+
+def test_key_weights_into_part_of_what_was_there(fake):
+    a, w = args(), torch.zeros(128)
+    for i in (1, 32, 63):
+        with pytest.raises(ValueError, match="memory of its own"):
+            weigh(a, weights=w[:64].view(1, 2, 32), out=w[i:i + 64].view(1, 2, 32))
+    for out in (w[:64], w[64:]):
+        weigh(a, weights=w[:64].view(1, 2, 32), out=out.view(1, 2, 32))
+        assert fake.calls[-1][0] == "cvsa_key_weights"

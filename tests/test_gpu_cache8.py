@@ -520,3 +520,54 @@ def test_eight_bit_cache_refusals(cuda):
         c.write_kv_block(0, x, x, 3)
     with pytest.raises(ValueError):
         c.gather_pages(torch.zeros(1, dtype=torch.int32, device=cuda))
+
+
+@pytest.mark.parametrize("new", [[1, 1], [90, 40]])
+def test_graphs_with_pools_of_their_own(cuda, new):
+    """Two captured calls replayed at the same time on two streams."""
+    problems = [Problem8(new, [9000, 5000], 8, 2, 128, seed=s) for s in (21, 22)]
+    want = [run(P)[0] for P in problems]
+    graphs, outs = [], []
+    for P in problems:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(chunk_attention(P.q, P.k_cache, P.v_cache, P.tables, P.lens, P.cu,
+                                        **P.scales))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_wait_that_runs_out(cuda):
+    """A wait limit of one poll makes the tensor-core kernel give up: the timeout bit, and the
+    next call with the default limit is as before."""
+    P = Problem8([200, 64], [900, 333], 8, 2, 128, seed=23)
+    want, _ = run(P)
+    lib = _lib.load()
+    try:
+        lib.cvsa_set_wait_limit(1)
+        chunk_attention(P.q, P.k_cache, P.v_cache, P.tables, P.lens, P.cu, dev_error=P.dev_error,
+                        **P.scales)
+        torch.cuda.synchronize()
+    finally:
+        lib.cvsa_set_wait_limit(0)
+    assert int(P.dev_error.item()) == _lib.DEV_ERR_TIMEOUT
+    P.dev_error.zero_()
+    assert torch.equal(run(P)[0], want) and int(P.dev_error.item()) == 0
+
+
+def test_mean_of_rows_that_misleads(cuda):
+    """The kernel goes by the batch's mean of rows: sequences far from it, and padding that
+    no sequence owns, come out the same."""
+    check(Problem8([1, 60, 0, 0, 1, 0, 1, 2], [500, 700, 9, 40, 333, 0, 17, 2000], 8, 2, 128,
+                   seed=24))
+    check(Problem8([1, 2], [500, 700], 8, 2, 128, seed=25, pad_tokens=500))
+    check(Problem8([0, 0, 1], [500, 700, 300], 8, 2, 64, seed=26))

@@ -557,3 +557,74 @@ def test_eviction_of_another_manager(cuda):
     with pytest.raises(ValueError, match="another manager"):
         layer(a, x, x, x, cu_of([1], cuda), eviction=WeightedEviction(b, 16))
     assert a.context_lens.tolist() == [0]
+
+
+@pytest.mark.parametrize("cache8", [False, True])
+def test_weights_without_tokens_and_odd_queries(cuda, cache8):
+    """A batch of no tokens decays what was there; queries whose heads share memory (no
+    tensor copy takes them) give what copies of them give."""
+    P = problem([0, 0], [300, 40], 8, 2, 128, cache8)
+    check_weights(P, decay=0.5)
+    P = problem([100, 60], [300, 400], 8, 2, 128, cache8)
+    lse = lse_of(P)
+    P.q = P.q[:, :1].expand(-1, 8, -1)
+    w = torch.rand((2, 2, P.tables.shape[1] * 16), device=cuda)
+    got, want = (key_weights(q, lse, P.k_cache, P.tables, P.lens, P.cu, w,
+                             out=torch.zeros_like(w), **P.more) for q in (P.q, P.q.contiguous()))
+    assert torch.allclose(got, want, rtol=2e-5, atol=1e-6)  # two kernels' sums in 32 bits
+
+
+def test_weights_wait_that_runs_out(cuda):
+    """One poll of a wait lasts about 4 us. Each of the 4 * 157 items of 256 keys takes 32
+    steps of more than 0.3 us (its products alone), and a CTA has four: its third waits for
+    the first one's keys to be done with, which is longer than that."""
+    P = problem([1024], [39000], 8, 4, 128)
+    lse, w = lse_of(P), torch.rand((1, 4, P.tables.shape[1] * 16), device=cuda)
+    args = (P.q, lse, P.k_cache, P.tables, P.lens, P.cu, w)
+    want = key_weights(*args, out=torch.zeros_like(w))
+    lib = _lib.load()
+    try:
+        lib.cvsa_set_wait_limit(1)
+        key_weights(*args, out=torch.zeros_like(w), dev_error=P.dev_error)
+        torch.cuda.synchronize()
+    finally:
+        lib.cvsa_set_wait_limit(0)
+    assert int(P.dev_error.item()) == _lib.DEV_ERR_TIMEOUT
+    assert torch.equal(key_weights(*args, out=torch.zeros_like(w)), want)
+
+
+@pytest.mark.parametrize("cache8", [False, True])
+def test_weights_many_short_items(cuda, cache8):
+    """Items of one to nine steps in all orders: the groups of warps that share a CTA fall
+    behind and catch up with one another."""
+    new = [33, 300, 64, 1, 130, 500, 40, 65, 90, 200]
+    for reps in (1, 3):
+        check_weights(problem(new * reps, [n + 7 * i for i, n in enumerate(new * reps)], 16, 4, 64,
+                              cache8, seed=reps))
+
+
+def test_evict_in_a_graph(cuda):
+    """A captured eviction, replayed as the sequences grow; one captured before the counting
+    began is refused."""
+    m = SequenceKVManager(PagedKVCache(60, 16, 2, 64), 2, 256)
+    w = torch.rand((2, 2, 256), device=cuda)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            m.evict(w, 50, 2, 10)
+    m.track_evictions()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = m.evict(w, 50, 2, 10)
+    assert not m._evict_plan  # the graph's own memory is not kept for other calls
+    for step in range(3):
+        m.reserve(cu_of([100, 40], cuda))
+        lens, w0 = m.context_lens.tolist(), w.clone()
+        graph.replay()
+        m.cache.check()
+        for b in range(2):
+            for h in range(2):
+                idx = kept64(w0[b, h].tolist(), lens[b], 50, 2, 10) if lens[b] > 50 else [-1] * 50
+                assert kept[b, h].tolist() == idx
+        pages_of(m)
+    assert m.evicted.tolist() == [250, 70]
