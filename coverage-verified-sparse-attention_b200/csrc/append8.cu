@@ -140,6 +140,9 @@ __device__ __forceinline__ void page_block(const Append8Args& a, int bid) {
   }
   const int blk = a.rg.tables[(int64_t)slot * a.rg.W + page];  // looked at behind the rows' loads
   const int r0 = (int)max((int64_t)0, p0 - page * bs), r1 = (int)min((int64_t)bs, p1 - page * bs);
+  // rows behind the written ones that hold tokens (an append in the middle of a sequence)
+  const int used = (int)max((int64_t)r1, min((int64_t)bs, a.rg.lens[slot] - page * bs));
+  const bool begun = r0 > 0 || used > r1;
   const int64_t shift = a.r.shift ? a.r.shift[slot] : 0;
   const Runs e(a.r, u);
   const void* const src = is_k ? a.r.k : a.r.v;
@@ -185,7 +188,7 @@ __device__ __forceinline__ void page_block(const Append8Args& a, int bid) {
     return;
   }
   float* const scale = const_cast<float*>(is_k ? a.kv.ks : a.kv.vs) + (int64_t)blk * hkv + h;
-  const int had = r0 > 0 ? scale_exponent_of(*scale) : kScaleMin;
+  const int had = begun ? scale_exponent_of(*scale) : kScaleMin;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (tid % 32 == 0) s_max[tid / 32] = top;
@@ -196,10 +199,11 @@ __device__ __forceinline__ void page_block(const Append8Args& a, int bid) {
   uint8_t* const rows = reinterpret_cast<uint8_t*>(const_cast<void*>(is_k ? a.kv.k : a.kv.v)) +
                         (int64_t)blk * a.kv.sb + (int64_t)h * a.kv.sh;
   if (tid == 0) *scale = pow2(now);  // every thread holds the old one
-  if (now > had && r0 > 0) {
+  if (now > had && begun) {
     const float f = pow2(had - now);
-    for (int c = tid; c < r0 * U; c += kThreads) {
-      uint4* p = reinterpret_cast<uint4*>(rows + (int64_t)(c / U) * a.kv.st + (c % U) * 16);
+    for (int c = tid; c < (r0 + used - r1) * U; c += kThreads) {
+      const int r = c / U < r0 ? c / U : c / U - r0 + r1;
+      uint4* p = reinterpret_cast<uint4*>(rows + (int64_t)r * a.kv.st + (c % U) * 16);
       uint4 w = *p;
       uint32_t* words = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll

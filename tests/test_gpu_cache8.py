@@ -10,7 +10,7 @@ from cvsa.kernels.chunk_attend import chunk_attention
 from cvsa.kernels.rope_append import rope_append, rope_table
 from cvsa.runtime.chunked import ChunkedAttention
 from cvsa.runtime.kv_cache import PagedKVCache, SequenceKVManager
-from ragged_ref import E32, U, assert_within, attend64, cu_of, rope64
+from ragged_ref import E32, Problem, U, assert_within, attend64, cu_of, rope64
 
 pytestmark = pytest.mark.gpu
 
@@ -571,3 +571,60 @@ def test_mean_of_rows_that_misleads(cuda):
                    seed=24))
     check(Problem8([1, 2], [500, 700], 8, 2, 128, seed=25, pad_tokens=500))
     check(Problem8([0, 0, 1], [500, 700, 300], 8, 2, 64, seed=26))
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_append_in_the_middle(cuda, page):
+    """Tokens written over some in the middle of a sequence: those before and behind them on
+    their pages keep their values, moved to the pages' new scales."""
+    n, c, start = 37, 300, 101
+    P = Problem8([n], [c], 4, 2, 64, page=page, seed=30)
+    P.k_scale.fill_(2.0 ** -6), P.v_scale.fill_(2.0 ** -6)
+    old = {x: values(getattr(P, x + "_cache"), getattr(P, x + "_scale")) for x in "kv"}
+    g = torch.Generator(device="cuda").manual_seed(31)
+    k, v = (torch.randn((n, 2, 64), generator=g, device="cuda") * 100 for _ in range(2))
+    rope_append(None, k, v, P.k_cache, P.v_cache, P.tables, P.lens, P.cu, dev_error=P.dev_error,
+                start_positions=torch.tensor([start], dtype=torch.int32, device="cuda"),
+                **P.scales)
+    assert int(P.dev_error.item()) == 0
+    for x, new in (("k", k), ("v", v)):
+        pool, scale = getattr(P, x + "_cache"), getattr(P, x + "_scale").double()
+        got = values(pool, getattr(P, x + "_scale"))
+        for pos in range(c):
+            blk, off = P.slot(0, pos)
+            sc = scale[blk][:, None]
+            if start <= pos < start + n:
+                want = new[pos - start].double()
+                assert bool((sc > 2.0 ** -6).all())
+            else:
+                want = old[x][blk, off]
+            assert torch.equal(got[blk, off], near8(want / sc) * sc), (x, pos)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_shift_of_a_wider_cache(cuda, dtype):
+    """position_shift with pools of the tokens' own type: each sequence turns by its own."""
+    new, ctx, shift, d = [3, 1, 20], [50, 9, 20], [7, 0, 1000], 64
+    P = Problem(new, ctx, 4, 2, d, dtype=dtype, seed=33)
+    g = torch.Generator(device="cuda").manual_seed(34)
+    q, k, v = (torch.randn((P.T, h, d), generator=g, device="cuda").to(dtype) for h in (4, 2, 2))
+    tab = rope_table(1100, d, device="cuda")
+    out = rope_append(q, k, v, P.k_cache, P.v_cache, P.tables, P.lens, P.cu, cos_sin=tab,
+                      dev_error=P.dev_error, position_shift=torch.tensor(
+                          shift, dtype=torch.int32, device="cuda")[:P.lens.numel()])
+    assert int(P.dev_error.item()) == 0
+    t = 0
+    for b, (n, c, s) in enumerate(zip(new, ctx, shift)):
+        at = torch.arange(c - n, c, device="cuda") + s
+        for got, x in ((out[t:t + n], q), (None, k)):
+            y, mag = rope64(x[t:t + n], at, tab, d, False, None, 1e-5)
+            if got is None:
+                got = torch.stack([P.k_cache[P.slot(b, p)] for p in range(c - n, c)])
+            assert_within(got, y, U[dtype] * (y.abs() + 8 * E32 * mag) + 8 * E32 * mag + 2.0 ** -25,
+                          f"{b}")
+        assert all(torch.equal(P.v_cache[P.slot(b, c - n + i)], v[t + i]) for i in range(n))
+        t += n
+    P.dev_error.zero_()  # past the table of turns: the token is skipped
+    rope_append(q, k, v, P.k_cache, P.v_cache, P.tables, P.lens, P.cu, cos_sin=tab,
+                dev_error=P.dev_error, out=out, position_shift=torch.full_like(P.lens, 2 ** 31 - 1))
+    assert int(P.dev_error.item()) == _lib.DEV_ERR_RAGGED and float(out.abs().max()) == 0.0
