@@ -10,7 +10,13 @@
 // General kernel (any mix of fp32, bf16, f16, and 8-bit pools; head_dim 64, 128,
 // 256): a block owns 64 keys of one KV head and goes over the rows that see any of
 // them, 64 at a time, on the FMA units. A key's sum is one block's, so there are no
-// atomics and the order of the sum is fixed.
+// atomics and the order of the sum is fixed. Bound by the FMA units and the shared
+// memory that feeds them; it serves what the two others do not take (fp32, pools of
+// another 16-bit type, head_dim 256, small odd pages, queries that no tensor copy reads).
+//
+// Which kernel: key_weights_few.cu up to 32 rows a sequence and KV head in the batch's
+// mean (32 single tokens of 32 heads, 1 to 8192 bf16 keys: 70 us, here 805), beyond it
+// key_weights_tc.cu (256 tokens at 32K 8-bit keys: 166 us, here 2331).
 #include "chunk_plan.cuh"
 #include "cvsa_common.cuh"
 #include "cvsa_internal.h"

@@ -2,7 +2,9 @@
 // cache of their type or of 8 bits, head_dim 64 or 128, pages of a multiple of 16 tokens.
 // Formula in key_weights.cu, work split as in weights_plan.cuh, a range a warp.
 //
-// Bound by the keys' bytes. As in chunk_attend_few.cu, keys go from memory to the
+// Bound by the keys' bytes: 32 single tokens of 32 heads at 1 to 8192 bf16 keys take 70 us,
+// 50 of them the bytes at the rate of a copy, the rest the first loads and the ranges'
+// uneven ends (one at 128K keys 59 us, over 8 bits 48). As in chunk_attend_few.cu, keys go from memory to the
 // operands of mma.sync in the registers of the lane that loads them: S' = K Q', 16 keys
 // by 8 rows, lane (g, t) with 16-byte pieces of keys g and g + 8 and the same elements of
 // query row g. A key's weights are summed over the two rows of a lane, the row tiles and
@@ -271,7 +273,9 @@ cudaError_t launch_t(const FewWeightArgs& a, int rows, cudaStream_t s) {
 }  // namespace
 
 // Rows of a step, or 0 where the other kernels serve the call: by the batch's mean of
-// rows a sequence, as in chunk_attend_few.cu.
+// rows a sequence, as in chunk_attend_few.cu. At 32 rows (8 tokens of 4 heads a KV head)
+// two steps of 16 go over a block of keys; beyond, key_weights_tc.cu's tiles of 64 rows
+// fill better.
 int weights_few_rows(const KvView& kv, const RaggedView& rg, const KeyWeightsView& w) {
   if ((kv.dtype != w.dtype && kv.dtype != CVSA_DTYPE_E4M3) || w.dtype == CVSA_DTYPE_F32 ||
       (kv.d != 64 && kv.d != 128) || kv.bs % 16)

@@ -13,8 +13,14 @@
 // Roles: warps 0-3 and 4-7 sum the first and the second tile of an item's even steps, warps
 // 8-15 of its odd ones, warps 16-19 load keys, warp 20 issues the products,
 // warps 21 and 22 load queries and their log-sum-exps. Each follows the same list of items on its own.
-// Bound by the exponentials (16 a clock and SM; 256 tokens of 32 heads at 32K keys: 60 us
-// of them, against 41 us of products at the tensor cores' rate).
+//
+// 256 tokens of 32 heads at 32K 8-bit keys take 166 us: 41 us of products at the tensor
+// cores' rate, 60 us of exponentials (16 a clock and SM). Bound by neither but by a step's
+// round of barriers, products and reads of tensor memory: without any sums it still takes
+// 153 us, and cheaper descriptors or log-sum-exps change nothing. Measured and not kept:
+// one sum of all products (122 us, twice fp32's error), one tile of M and four buffers (231),
+// one group of warps reading 32 columns at a time (184), 64 columns at a time or reads ahead
+// of their use (slower).
 #include <cstddef>
 #include <type_traits>
 
