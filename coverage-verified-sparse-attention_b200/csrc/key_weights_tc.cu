@@ -273,11 +273,11 @@ __device__ __forceinline__ void mma_role(const WArgs& a, WMeta* m, uint32_t base
     if (steps <= 0) continue;
     const uint32_t kb = nk & 1;
     if (!warp_wait(&m->k_full[kb], (nk >> 1) & 1, m, a)) goto out;
+    fence_proxy_async_smem();  // the keys were written through the generic proxy
     for (int j = 0; j < steps; ++j, ++n) {
       const uint32_t b = j & 1, qb = n % kQBufs, turn = (n / kQBufs) & 1;
       if (!warp_wait(&m->q_full[qb], turn, m, a)) goto out;
       if (!warp_wait(&m->q_copied[qb], turn, m, a)) goto out;
-      fence_proxy_async_smem();  // the tiles were written through the generic proxy
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
         if (!warp_wait(&m->s_free[b][mt], (odd >> b & 1) ^ 1, m, a)) goto out;
