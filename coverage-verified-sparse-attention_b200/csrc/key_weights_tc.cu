@@ -39,7 +39,7 @@ constexpr int kQBufs = 4, kRing = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct WMeta {
-  uint64_t k_full[2], k_empty[2], q_full[kQBufs], q_copied[kQBufs], q_empty[kQBufs], drain;
+  uint64_t k_full[2], k_empty[2], q_full[kQBufs], q_copied[kQBufs], q_empty[kQBufs], drain[2];
   uint64_t s_full[2][2], s_free[2][2];  // buffer, tile
   uint64_t joined[2][2], taken[2][2];   // items in turn, tile: the second group's sums
   // rows of a step, in a ring: those of step n are written over once the products of step
@@ -261,7 +261,7 @@ __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, 
 
 template <typename T, int D>
 __device__ __forceinline__ void mma_role(const WArgs& a, WMeta* m, uint32_t base, uint32_t tmem,
-                                         WeightWalk walk) {
+                                         WeightWalk walk, int mt) {
   using C = WCfg<D>;
   constexpr uint32_t kId = mma_idesc(!std::is_same<T, __half>::value, kTile, kRows, false);
   const uint64_t k_desc = smem_desc(base, 16, 1024), q_desc = smem_desc(base + C::kQ, 16, 1024);
@@ -278,36 +278,33 @@ __device__ __forceinline__ void mma_role(const WArgs& a, WMeta* m, uint32_t base
       const uint32_t b = j & 1, qb = n % kQBufs, turn = (n / kQBufs) & 1;
       if (!warp_wait(&m->q_full[qb], turn, m, a)) goto out;
       if (!warp_wait(&m->q_copied[qb], turn, m, a)) goto out;
+      if (!warp_wait(&m->s_free[b][mt], (odd >> b & 1) ^ 1, m, a)) goto out;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t kd = k_desc + (((kb * 2 + mt) * C::kTileBytes) >> 4);
+        const uint64_t qd = q_desc + ((qb * C::kQBytes) >> 4);
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        if (!warp_wait(&m->s_free[b][mt], (odd >> b & 1) ^ 1, m, a)) goto out;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t kd = k_desc + (((kb * 2 + mt) * C::kTileBytes) >> 4);
-          const uint64_t qd = q_desc + ((qb * C::kQBytes) >> 4);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t ko = ((kk / 4) * (kTile * 128) + (kk % 4) * 32) >> 4;
-            const uint32_t qo = ((kk / 4) * (kRows * 128) + (kk % 4) * 32) >> 4;
-            constexpr int kHalf = D / 32;  // each half of the elements has a sum of its own
-            mma_ss(tmem + (b * 2 + mt) * 2 * kRows + kk / kHalf * kRows, kd + ko, qd + qo, kId,
-                   kk % kHalf > 0);
-          }
-          mma_commit(smem_u32(&m->s_full[b][mt]));
-          if (mt) mma_commit(smem_u32(&m->q_empty[qb]));
-          if (mt && j == steps - 1) mma_commit(smem_u32(&m->k_empty[kb]));
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t ko = ((kk / 4) * (kTile * 128) + (kk % 4) * 32) >> 4;
+          const uint32_t qo = ((kk / 4) * (kRows * 128) + (kk % 4) * 32) >> 4;
+          constexpr int kHalf = D / 32;  // each half of the elements has a sum of its own
+          mma_ss(tmem + (b * 2 + mt) * 2 * kRows + kk / kHalf * kRows, kd + ko, qd + qo, kId,
+                 kk % kHalf > 0);
         }
-        __syncwarp();
+        mma_commit(smem_u32(&m->s_full[b][mt]));
+        mma_commit(smem_u32(&m->q_empty[qb]));
+        if (j == steps - 1) mma_commit(smem_u32(&m->k_empty[kb]));
       }
+      __syncwarp();
       odd ^= 1u << b;
     }
     ++nk;
   }
 out:
   // nothing of this CTA may be in flight when its tensor memory is freed
-  if (elect_one()) mma_commit(smem_u32(&m->drain));
+  if (elect_one()) mma_commit(smem_u32(&m->drain[mt]));
   __syncwarp();
-  mbar_wait_bounded(&m->drain, 0, 1u << 18);
+  mbar_wait_bounded(&m->drain[mt], 0, 1u << 18);
   __syncwarp();
 }
 
@@ -429,7 +426,8 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&m->k_full[i], 128);
-      mbar_init(&m->k_empty[i], 1);
+      mbar_init(&m->k_empty[i], 2);
+      mbar_init(&m->drain[i], 1);
       for (int mt = 0; mt < 2; ++mt) {
         mbar_init(&m->s_full[i][mt], 1);
         mbar_init(&m->s_free[i][mt], 4);
@@ -440,9 +438,9 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
     for (int i = 0; i < kQBufs; ++i) {
       mbar_init(&m->q_full[i], 64);  // the plain writes
       mbar_init(&m->q_copied[i], 1);
-      mbar_init(&m->q_empty[i], 1);
+      mbar_init(&m->q_empty[i], 2);
     }
-    mbar_init(&m->drain, 1);
+    
     m->abort = 0;
     fence_mbar_init();
   }
@@ -456,8 +454,8 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
   const WeightWalk walk(r);
   if (warp < 16) sum_role(a, m, tmem, walk, warp / 4 & 1, warp / 8);
   else if (warp < 20) key_role<T, D, F8>(a, m, base, walk, warp - 16);
-  else if (warp == 20) mma_role<T, D>(a, m, base, tmem, walk);
-  else if (warp < 23) query_role<D>(a, m, base, walk, warp - 21);
+  else if (warp == 20 || warp == 23) mma_role<T, D>(a, m, base, tmem, walk, warp == 23);
+  else query_role<D>(a, m, base, walk, warp - 21);
   tc_fence_before();
   __syncthreads();
   if (warp == 20) {
