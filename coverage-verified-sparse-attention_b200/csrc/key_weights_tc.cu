@@ -11,16 +11,18 @@
 // next rows form while these are summed; the next item's keys are loaded meanwhile. 8-bit
 // keys are widened to the queries' type as they are copied, once an item.
 // Roles: warps 0-3 and 4-7 sum the first and the second tile of an item's even steps, warps
-// 8-15 of its odd ones, warps 16-19 load keys, warp 20 issues the products,
-// warps 21 and 22 load queries and their log-sum-exps. Each follows the same list of items on its own.
+// 8-15 of its odd ones, warps 16-19 load keys, warps 20 and 23 issue the products of the
+// first and the second tile (one warp for both was the bottleneck: 164 us), warps 21 and 22
+// load queries and their log-sum-exps. Each follows the same list of items on its own.
 //
-// 256 tokens of 32 heads at 32K 8-bit keys take 166 us: 41 us of products at the tensor
-// cores' rate, 60 us of exponentials (16 a clock and SM). Bound by neither but by a step's
-// round of barriers, products and reads of tensor memory: without any sums it still takes
-// 153 us, and cheaper descriptors or log-sum-exps change nothing. Measured and not kept:
-// one sum of all products (122 us, twice fp32's error), one tile of M and four buffers (231),
-// one group of warps reading 32 columns at a time (184), 64 columns at a time or reads ahead
-// of their use (slower).
+// 256 tokens of 32 heads at 32K 8-bit keys take 147 us: 41 us of products at the tensor
+// cores' rate, 60 us of exponentials (16 a clock and SM). Bound by the way of a buffer: its
+// group sums 64 rows in 2700 cycles of the 4700 from one use to the next, and waits for the
+// next products the rest (clocks read in the kernel: 460 cycles to issue a tile's, some 300
+// for each of the three waits before them). A third buffer does not fit in tensor memory.
+// Measured with one issuing warp and not kept: one sum of all products (122 us, twice fp32's
+// error), one tile of M and four buffers (231), one group of warps reading 32 columns at a time
+// (184), 64 columns at a time or reads ahead of their use (slower).
 #include <cstddef>
 #include <type_traits>
 
@@ -43,8 +45,9 @@ struct WMeta {
   uint64_t s_full[2][2], s_free[2][2];  // buffer, tile
   uint64_t joined[2][2], taken[2][2];   // items in turn, tile: the second group's sums
   // rows of a step, in a ring: those of step n are written over once the products of step
-  // n + 4 are done. By then the sums of n are: one of the steps between waits for n's
-  // buffer, or for group 0 to be done with a step of a later item than n's.
+  // n + 4 are done. By then they were read: one of the steps between waits for n's
+  // buffer, which is given back behind the last read, or for group 0 to be done with a step of a
+  // later item than n's.
   alignas(16) float c[kRing][kRows];  // minus the log-sum-exp
   uint32_t live[kRing][2];            // bit per row that takes part (is there, saw a key)
   float second[2][2][kTile];          // items in turn, tile: the second group's sums
@@ -362,18 +365,26 @@ __device__ __forceinline__ void sum_role(const WArgs& a, WMeta* m, uint32_t tmem
         const uint32_t sees = (bits_of(from, to, x) & m->live[slot][x / 32] >> x % 32) & 0xffff;
         const bool all = __all_sync(0xffffffffu, sees == 0xffff);
         tmem_wait_ld();
-        const float4* const c4 = reinterpret_cast<const float4*>(m->c[slot] + x);
+        uint64_t y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          y[i] = f2_add(f2_pack(s[2 * i], s[2 * i + 1]), f2_pack(s2[2 * i], s2[2 * i + 1]));
+        float4 c4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c4[i] = reinterpret_cast<const float4*>(m->c[slot] + x)[i];
+        if (x + 16 >= rows) {  // all was read: the next products may go there
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&m->s_free[b][mt]);
+        }
         if (all) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float4 c = c4[i];
             float u, v;
-            const uint64_t lo = f2_add(f2_pack(s[4 * i], s[4 * i + 1]), f2_pack(s2[4 * i], s2[4 * i + 1]));
-            f2_unpack(f2_mul(f2_fma(lo, sc, f2_pack(c.x, c.y)), l2), u, v);
+            f2_unpack(f2_mul(f2_fma(y[2 * i], sc, f2_pack(c.x, c.y)), l2), u, v);
             sum0 = f2_add(sum0, f2_pack(ex2(u), ex2(v)));
-            const uint64_t hi = f2_add(f2_pack(s[4 * i + 2], s[4 * i + 3]),
-                                       f2_pack(s2[4 * i + 2], s2[4 * i + 3]));
-            f2_unpack(f2_mul(f2_fma(hi, sc, f2_pack(c.z, c.w)), l2), u, v);
+            f2_unpack(f2_mul(f2_fma(y[2 * i + 1], sc, f2_pack(c.z, c.w)), l2), u, v);
             sum1 = f2_add(sum1, f2_pack(ex2(u), ex2(v)));
           }
         } else if (__any_sync(0xffffffffu, sees != 0)) {
@@ -381,16 +392,15 @@ __device__ __forceinline__ void sum_role(const WArgs& a, WMeta* m, uint32_t tmem
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float4 c = c4[i / 4];
-            const float y = i % 4 == 0 ? c.x : i % 4 == 1 ? c.y : i % 4 == 2 ? c.z : c.w;
-            const float e = ex2(fmaf(s[i] + s2[i], a.w.scale, y) * kLog2e);
+            const float z = i % 4 == 0 ? c.x : i % 4 == 1 ? c.y : i % 4 == 2 ? c.z : c.w;
+            float u, v;
+            f2_unpack(y[i / 2], u, v);
+            const float e = ex2(fmaf(i & 1 ? v : u, a.w.scale, z) * kLog2e);
             add += sees >> i & 1 ? e : 0.f;
           }
           sum0 = f2_add(sum0, f2_pack(add, 0.f));
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&m->s_free[b][mt]);  // the next products may go there
       float u, v;
       f2_unpack(f2_add(sum0, sum1), u, v);
       total += u + v;
@@ -440,7 +450,6 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
       mbar_init(&m->q_copied[i], 1);
       mbar_init(&m->q_empty[i], 2);
     }
-    
     m->abort = 0;
     fence_mbar_init();
   }
