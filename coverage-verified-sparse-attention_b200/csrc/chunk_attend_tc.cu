@@ -109,6 +109,8 @@ constexpr int kPairRows = 64;  // rows whose fp32 O fits the second Q tile's mem
 struct alignas(8) TcMeta {
   uint64_t kv_full[8], kv_empty[8];
   uint64_t q_full, q_empty;
+  uint64_t q_second;                    // a second Q tile is there (its softmax group skips
+                                        // items without one, so q_full's parity misleads it)
   uint64_t q_ready[2];                  // Q tiles that are scaled first: they were
   uint64_t s_full[2], s_free[2], p_half[2], p_full[2], o_full[2];  // per slot
   uint64_t it_full[kItems], it_empty[kItems];
@@ -571,6 +573,7 @@ struct Loader8 : Loader<__half, D> {
             this->copy_rows(base + q * C::kQTile, a.c.q, qo);
           }
           arrive_when_landed(&m->q_full);
+          if (it->nq > 1) arrive_when_landed(&m->q_second);
         }
         if (j >= lag) {
           const uint32_t st = op % C::kStages, slot = (tiles + j - lag) % kSlots;
@@ -812,7 +815,7 @@ __device__ __forceinline__ void softmax_role(const TcArgs& a, TcMeta* m, uint32_
   const int G = a.g.G;
   float scale2 = a.scale2;
   ItemReader items(m, a);
-  uint32_t op = 0, tiles = 0, turn = 0, ends = 0, joins = 0, loads = 0;
+  uint32_t op = 0, tiles = 0, turn = 0, ends = 0, joins = 0, loads = 0, seconds = 0;
   while (const ItemRec* it = items.next()) {
     loads += it->nt > 0;
     const int nt = it->nt, pair = it->pair, q = pair ? 0 : g, step = pair ? 2 : 1;
@@ -825,7 +828,8 @@ __device__ __forceinline__ void softmax_role(const TcArgs& a, TcMeta* m, uint32_
     }
     const bool active = warp * 32 < rows;
     if (kScaled && nt > 0 && !(pair && g == 1)) {
-      if (!warp_wait(&m->q_full, (loads - 1) & 1, m, a)) return;
+      ++seconds;
+      if (!warp_wait(g ? &m->q_second : &m->q_full, ((g ? seconds : loads) - 1) & 1, m, a)) return;
       if (active) {
         const int e = scale_query<TI, D>(base + g * C::kQTile, r);
         scale2 = a.scale2 * pow2(e);
@@ -1152,6 +1156,7 @@ chunk_tc_kernel(const __grid_constant__ TcArgs a) {
       mbar_init(&m->kv_empty[i], 2);
     }
     mbar_init(&m->q_full, 128);
+    mbar_init(&m->q_second, 128);
     mbar_init(&m->q_empty, 2);
     for (int i = 0; i < 2; ++i) mbar_init(&m->q_ready[i], 128);
     for (int i = 0; i < 2; ++i) {

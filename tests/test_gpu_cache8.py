@@ -628,3 +628,16 @@ def test_shift_of_a_wider_cache(cuda, dtype):
     rope_append(q, k, v, P.k_cache, P.v_cache, P.tables, P.lens, P.cu, cos_sin=tab,
                 dev_error=P.dev_error, out=out, position_shift=torch.full_like(P.lens, 2 ** 31 - 1))
     assert int(P.dev_error.item()) == _lib.DEV_ERR_RAGGED and float(out.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (8, 2, 64), (2, 2, 128), (40, 8, 64)])
+def test_items_with_and_without_a_second_tile(cuda, hq, hkv, d):
+    """Items of one tile of query rows before items of two: the warps of the second tile
+    have nothing to do in the former and must not run ahead of the latter's queries."""
+    G = hq // hkv
+    new = [max(1, n // G) for n in [70, 100, 222, 90, 250, 120, 256, 66, 80, 70, 240] * 6]
+    P = Problem8(new, [n + 300 + 37 * (i % 9) for i, n in enumerate(new)], hq, hkv, d, seed=41)
+    first, _ = run(P)
+    check(P)
+    for _ in range(20):
+        assert torch.equal(run(P)[0], first)
