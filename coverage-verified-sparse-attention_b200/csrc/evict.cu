@@ -4,7 +4,8 @@
 // last `recent` ones and those of largest weight between (equal weights: the earlier
 // key; NaN below everything), `keep` in all, in their order. Their keys, values and
 // weights move to the front: rows to new pages, so that no row is written over
-// before it is read and all rows can move at once.
+// before it is read and all rows can move at once. In place, the weights behind the
+// kept ones become 0, up to the old length.
 //
 // select: a cluster of 1 to 8 blocks a (sequence, KV head), each with a piece of the row
 //   in shared memory. The cut, the n-th largest weight, is found by a radix select over
@@ -193,6 +194,10 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const __grid_con
     equal += sums[0] >> 16;
     __syncthreads();
   }
+  // In place, what stood behind the kept weights belongs to no key any more: a key that takes
+  // such a slot without being counted begins at 0. (This piece was read by now, by its block.)
+  if (out == w)
+    for (int i = max(p0, a.e.keep) + tid; i < p1; i += kThreads) out[i] = 0.f;
   pdl_launch_dependents();
 }
 

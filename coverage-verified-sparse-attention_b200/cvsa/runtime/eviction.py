@@ -21,7 +21,8 @@ class WeightedEviction:
 
     manager is the layer's `SequenceKVManager`. A key's weight is the sum of the
     softmax weights of all query heads of its KV head's group, `decay` times
-    what it was a step before. The first `sink` and the last `recent` keys of a
+    what it was a step before; a key that came in a call without the counting begins
+    at 0 with the next one that counts. The first `sink` and the last `recent` keys of a
     sequence are kept whatever their weight. A sliding window counts the keys that
     are left, not positions."""
 

@@ -701,7 +701,8 @@ typedef struct cvsa_evict {
 /* For every sequence longer than `keep`, and each KV head: the first `sink` keys,
  * the last `recent` and the keep - sink - recent of largest weight between (equal
  * weights: the earlier; NaN below everything), in their order, go to kept, their
- * weights to out_weights, their keys and values to new_tables' pages. In 8-bit
+ * weights to out_weights (in place, those behind become 0 up to the old length),
+ * their keys and values to new_tables' pages. In 8-bit
  * pools a new page's scale is the largest of its rows'. Rows of kept are -1 for
  * shorter sequences, of which nothing else is written. Tables and lengths are
  * the caller's to change (cvsa_evict_commit). */

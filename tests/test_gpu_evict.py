@@ -628,3 +628,72 @@ def test_evict_in_a_graph(cuda):
                 assert kept[b, h].tolist() == idx
         pages_of(m)
     assert m.evicted.tolist() == [250, 70]
+
+
+# ---------------------------------------------------------------------------
+# weights of keys that no counted call appended
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("n,keep", [(33, 32), (500, 60), (20000, 4096), (131072, 100),
+                                    (400000, 30000)])
+def test_evict_clears_what_stood_behind(cuda, n, keep):
+    """In place, the slots between the kept weights and the old length belong to no key any
+    more and are 0; what lies past the length, shorter sequences and other memory stay. Rows
+    of one block and of several, and one that shared memory does not hold."""
+    c = Cut([n, n // 2 + 1, keep], keep, 2, keep // 10, hkv=1, seed=keep)
+    w0 = c.w.clone()
+    c.check()
+    for s, m in enumerate(c.lens_):
+        if m > keep:
+            assert not bool(c.w[s, :, keep:m].any())
+            assert torch.equal(c.w[s, :, m:], w0[s, :, m:])
+        else:
+            assert torch.equal(c.w[s], w0[s])
+    c = Cut([n, n // 2 + 1, keep], keep, 2, keep // 10, hkv=1, seed=keep)
+    out = torch.full((3, 1, keep + 40), 5.0, device=cuda)
+    c.run(out)
+    assert torch.equal(c.w, w0) and bool((out[..., keep:] == 5).all())
+
+
+def uniform(layer, m, ev, n, hq, cuda):
+    """n tokens whose queries are 0: a token gives each key it sees the same weight."""
+    H, d = m.cache.num_kv_heads, m.cache.head_dim
+    z = torch.zeros((n, hq, d), dtype=BF16, device=cuda)
+    layer(m, z, z[:, :H], z[:, :H], cu_of([n], cuda), eviction=ev)
+
+
+@pytest.mark.parametrize("how", ["layer", "append", "batch", "token"])
+def test_keys_that_were_not_counted_begin_at_zero(cuda, how):
+    """After an eviction, keys that come without the counting have no weight: not what the
+    keys that had their slots before it left there."""
+    H, hq, d, keep = 2, 4, 64, 50
+    m = SequenceKVManager(PagedKVCache(40, 16, H, d), 1, 400)
+    layer, ev = ChunkedAttention(), WeightedEviction(m, keep, 2, 5)
+    g = torch.Generator(device=cuda).manual_seed(3)
+    q, k, v = (torch.randn((200, h, d), generator=g, device=cuda).to(BF16) for h in (hq, H, H))
+    layer(m, q, k, v, cu_of([200], cuda), eviction=ev)
+    assert float(ev.weights[0, :, keep:200].min()) > 0
+    ev.evict()
+    if how == "layer":
+        layer(m, q[:60], k[:60], v[:60], cu_of([60], cuda))
+    elif how == "append":
+        layer.append(m, q[:60], k[:60], v[:60], cu_of([60], cuda))
+    else:
+        for i in range(60):
+            if how == "batch":
+                m.append_batch(k[i:i + 1], v[i:i + 1])
+            else:
+                m.append_token_kv(0, k[i], v[i])
+    assert m.context_lens.tolist() == [110]
+    assert not bool(ev.weights[0, :, keep:].any())
+    before = ev.weights.double()
+    uniform(layer, m, ev, 1, hq, cuda)
+    m.cache.check()
+    want = before + 0.0
+    want[0, :, :111] += (hq // H) / 111.0
+    # scores are 0, so a weight errs as the log of a sum of 111 terms does ((111 + 16) 2^-24 and
+    # 4 * 4.8 * 2^-24, and 2^-21 for each of two exponentials: below 2^-16), the sum by 2^-23
+    tol = 2.0 ** -16 * (hq // H) / 111.0 + 2.0 ** -22 * want
+    assert bool(((ev.weights.double() - want).abs() <= tol).all())
+    w0, kept = ev.weights[0].cpu(), ev.evict()
+    for h in range(H):
+        assert kept[0, h].tolist() == kept64(w0[h].tolist(), 111, keep, 2, 5)
