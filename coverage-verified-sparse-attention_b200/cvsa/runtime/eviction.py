@@ -40,6 +40,7 @@ class WeightedEviction:
         self.weights = torch.zeros(
             manager.batch_size, c.num_kv_heads, manager.max_pages * manager.block_size,
             device=c.k_cache.device)
+        manager._counting.add(self)  # prefill_kv clears a slot that it fills anew
 
     def observe(self, q: torch.Tensor, lse: torch.Tensor, cu_tokens: torch.Tensor,
                 seq_ids: Optional[torch.Tensor] = None,

@@ -9,6 +9,7 @@ one launch (cvsa_paged_append) instead of the reference's per-sequence Python
 loop with two `.item()` syncs each (kv_cache.py:133-150).
 """
 
+import weakref
 from dataclasses import dataclass
 from typing import Optional
 
@@ -141,6 +142,7 @@ class SequenceKVManager:
         # keys evicted from each sequence so far (None: this manager never evicted)
         self.evicted = None
         self._evict_plan = {}
+        self._counting = weakref.WeakSet()  # `WeightedEviction`s of this manager
 
     @property
     def _pages_allocated(self):
@@ -170,6 +172,8 @@ class SequenceKVManager:
         self.pages_allocated[seq_idx] = n_pages
         if self.evicted is not None:
             self.evicted[seq_idx] = 0
+        for counts in self._counting:  # what gathered in this slot was another sequence's
+            counts.weights[seq_idx] = 0
 
     def append_token_kv(self, seq_idx: int, k: torch.Tensor, v: torch.Tensor):
         """Append one decode token's K/V [num_kv_heads, head_dim] to one sequence."""

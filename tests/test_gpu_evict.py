@@ -697,3 +697,33 @@ def test_keys_that_were_not_counted_begin_at_zero(cuda, how):
     w0, kept = ev.weights[0].cpu(), ev.evict()
     for h in range(H):
         assert kept[0, h].tolist() == kept64(w0[h].tolist(), 111, keep, 2, 5)
+
+
+@pytest.mark.parametrize("registered", [1, 2])
+def test_a_slot_that_is_filled_anew_has_no_weights(cuda, registered):
+    """prefill_kv puts another sequence where one gathered weights: its keys begin at 0, the
+    other sequences' stay."""
+    H, hq, d, keep = 2, 4, 64, 50
+    m = SequenceKVManager(PagedKVCache(80, 16, H, d), 3, 200)
+    layer, evs = ChunkedAttention(), [WeightedEviction(m, keep) for _ in range(registered)]
+    g = torch.Generator(device=cuda).manual_seed(4)
+    q, k, v = (torch.randn((270, h, d), generator=g, device=cuda).to(BF16) for h in (hq, H, H))
+    for ev in evs:
+        layer(m, q, k, v, cu_of([90, 90, 90], cuda), eviction=ev)
+    was = [ev.weights.clone() for ev in evs]
+    m.prefill_kv(1, k[:120], v[:120])
+    for ev, w in zip(evs, was):
+        assert not bool(ev.weights[1].any())
+        for s in (0, 2):
+            assert torch.equal(ev.weights[s], w[s]) and bool(w[s].any())
+    ev = evs[0]
+    z = torch.zeros((1, hq, d), dtype=BF16, device=cuda)
+    layer(m, z, z[:, :H], z[:, :H], cu_of([1], cuda),
+          torch.ones(1, dtype=torch.int32, device=cuda), eviction=ev)
+    m.cache.check()
+    want = torch.zeros_like(ev.weights[1]).double()
+    want[:, :121] = (hq // H) / 121.0
+    assert bool(((ev.weights[1].double() - want).abs() <= 2.0 ** -16 * want).all())
+    evs.clear()
+    del ev
+    m.prefill_kv(2, k[:10], v[:10])  # nobody counts any more
