@@ -450,6 +450,17 @@ def scale_ptr(scale: Optional[torch.Tensor], cache: torch.Tensor, name: str) -> 
     return scale.data_ptr()
 
 
+# A selection names pages by their place in a sequence's table. An eviction puts other keys
+# there, so the tables' memory (views of it too) carries how often that happened, for who
+# keeps selections.
+def renumbered(tables: torch.Tensor) -> int:
+    return getattr(tables.untyped_storage(), "cvsa_renumbered", 0)
+
+
+def renumber(tables: torch.Tensor):
+    tables.untyped_storage().cvsa_renumbered = renumbered(tables) + 1
+
+
 def token_rows(t: torch.Tensor, name: str) -> torch.Tensor:
     """A [num_tokens, heads, head_dim] view the kernels can read: 16-byte rows (copied if not)."""
     if t.dim() != 3:

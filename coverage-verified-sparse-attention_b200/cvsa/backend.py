@@ -19,7 +19,8 @@ Scheduling follows the reference:
   * fixed interval R     -> scoring step every R steps, reuse between
                             (backend.py:361-366)
 A layer without a cached selection takes a scoring step (the reference's
-_reuse_step re-enters __call__ with step - 1 for that case).
+_reuse_step re-enters __call__ with step - 1 for that case), and so does one whose
+tables were evicted from since its last step: the selection names other keys now.
 
 Extensions (off by default): `sink_pages` / `local_pages` always-kept pages,
 the stable (score desc, page index asc) top-k order, and `process_group`:
@@ -176,6 +177,7 @@ class CVSABackend:
         self._decision_views: Dict[int, torch.Tensor] = {}  # workspace ptr -> int32 view
 
         self._layers: Dict[int, _LayerState] = {}
+        self._renumbered: Dict[int, int] = {}  # layer -> evictions of its tables so far
         self._ws: Dict[tuple, tuple] = {}  # (stream, private) -> (ptr, bytes, tensor)
         self._counters: Optional[torch.Tensor] = None   # int64[8] device
         self._dev_error: Optional[torch.Tensor] = None
@@ -246,6 +248,23 @@ class CVSABackend:
             self._kernel_times_ms[k] = 0.0
             self._kernel_counts[k] = 0
         self._pending_events.clear()
+
+    def forget_selections(self, layer_idx: Optional[int] = None):
+        """Drop the cached page selections of a layer (default: of all layers), and the scores
+        kept to gate them: the next step selects anew, steps and statistics go on. For tables
+        whose pages came to hold other keys. Steps over a `SequenceKVManager`'s own tables (or
+        views of them) do this by themselves behind its evictions."""
+        for i, st in self._layers.items():
+            if layer_idx is None or i == layer_idx:
+                st.has_cache = st.has_scored = False
+        if self._alt is not None:
+            self._alt.forget(layer_idx)
+
+    def _follow(self, block_tables: torch.Tensor, layer_idx: int):
+        n = _lib.renumbered(block_tables)
+        if self._renumbered.setdefault(layer_idx, n) != n:
+            self.forget_selections(layer_idx)
+            self._renumbered[layer_idx] = n
 
     @property
     def is_scoring_step(self):
@@ -352,6 +371,7 @@ class CVSABackend:
         if q.dim() == 4:
             q = q.squeeze(1)
         dev = _lib.require_cuda(q, k_cache, v_cache, block_tables, context_lens)
+        self._follow(block_tables, layer_idx)
         self._ensure(dev)
         if self._alt is not None and layer_idx not in self._dense_layers:
             bt_a = block_tables if block_tables.dtype == torch.int32 else \

@@ -244,7 +244,8 @@ class SequenceKVManager:
         has none for stays as it is (`cache.check()` raises). Returns the kept
         keys [batch_size, num_kv_heads, keep], -1 for sequences that were not
         cut. Keys keep the rotation of their first position; `evicted` counts
-        what went, for the positions of new tokens. Nothing synchronises."""
+        what went, for the positions of new tokens. A `CVSABackend` drops the page
+        selections that it made of these tables. Nothing synchronises."""
         c = self.cache
         dev = _lib.require_cuda(weights, c.k_cache)
         if not 0 < keep <= self.max_pages * self.block_size:
@@ -273,6 +274,7 @@ class SequenceKVManager:
                          keep, sink, recent, dev_error=c.dev_error, k_scale=c.k_scale,
                          v_scale=c.v_scale)
             _lib.check(lib.cvsa_evict_commit(args, err, stream), "cvsa_evict_commit")
+        _lib.renumber(self.block_tables)
         return kept
 
     def _append(self, k, v, ids):

@@ -104,6 +104,13 @@ class AltStep:
         self.cached = {}
         self.scores = {}
 
+    def forget(self, layer_idx: Optional[int] = None):
+        if layer_idx is None:
+            self.reset()
+        else:
+            self.cached.pop(layer_idx, None)
+            self.scores.pop(layer_idx, None)
+
     # ---- helpers ----------------------------------------------------------
     def _ctr(self, i, v):
         self.be._counters[i] += v
