@@ -454,11 +454,18 @@ def scale_ptr(scale: Optional[torch.Tensor], cache: torch.Tensor, name: str) -> 
 # there, so the tables' memory (views of it too) carries how often that happened, for who
 # keeps selections.
 def renumbered(tables: torch.Tensor) -> int:
-    return getattr(tables.untyped_storage(), "cvsa_renumbered", 0)
+    """How often so far; -1 where a replayed graph may have done it unseen."""
+    memory = tables.untyped_storage()
+    if getattr(memory, "cvsa_replays", False) and not torch.cuda.is_current_stream_capturing():
+        return -1
+    return getattr(memory, "cvsa_renumbered", 0)
 
 
 def renumber(tables: torch.Tensor):
-    tables.untyped_storage().cvsa_renumbered = renumbered(tables) + 1
+    memory = tables.untyped_storage()
+    memory.cvsa_renumbered = getattr(memory, "cvsa_renumbered", 0) + 1
+    if torch.cuda.is_current_stream_capturing():
+        memory.cvsa_replays = True
 
 
 def token_rows(t: torch.Tensor, name: str) -> torch.Tensor:

@@ -262,7 +262,7 @@ class CVSABackend:
 
     def _follow(self, block_tables: torch.Tensor, layer_idx: int):
         n = _lib.renumbered(block_tables)
-        if self._renumbered.setdefault(layer_idx, n) != n:
+        if n < 0 or self._renumbered.setdefault(layer_idx, n) != n:
             self.forget_selections(layer_idx)
             self._renumbered[layer_idx] = n
 

@@ -104,3 +104,52 @@ def test_forget_selections(cuda, kw):
         assert torch.equal(go(be, x), go(fresh, x))
     be.forget_selections()
     assert be.cached_selection(0) is None and be.get_stats()["total_decode_steps"] == 4
+
+
+@pytest.mark.parametrize("kw", FORMS[:4])
+def test_a_replayed_eviction(cuda, kw):
+    """The host does not see a graph that evicts being replayed: steps beside it select anew
+    every time. Steps in the graph reuse what the graph's own first step selected."""
+    m, ev, q = grown(cuda)
+    be, fresh = backend(kw), backend(kw)
+    graph, g = torch.cuda.CUDAGraph(), torch.Generator(device=cuda).manual_seed(9)
+    with torch.cuda.graph(graph):
+        ev.evict()
+    for i in range(2):
+        step(be, m, q[3 * i])
+        graph.replay()
+        m.cache.check()
+        assert m.context_lens.tolist() == [400, 400]
+        for x in q[3 * i + 1:3 * i + 3]:
+            assert torch.equal(step(be, m, x), step(fresh, m, x))
+        k, v = (torch.randn((900, H, D), generator=g, device=cuda).to(BF16) for _ in range(2))
+        zero = torch.zeros((900, HQ, D), dtype=BF16, device=cuda)
+        ChunkedAttention()(m, zero, k, v, cu_of([600, 300], cuda), eviction=ev)
+
+
+def test_an_eviction_and_its_steps_in_a_graph(cuda):
+    m, ev, q = grown(cuda)
+    be, fresh = backend(FORMS[0]), backend(FORMS[0])
+    step(be, m, q[0])
+    state = [t.clone() for t in (m.block_tables, m.context_lens, m.pages_allocated,
+                                 m.cache.free_list, m.cache.free_head, ev.weights)]
+    step(fresh, m, q[0])  # workspaces of both exist before the capture
+    fresh.forget_selections()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ev.evict()
+        out = [step(be, m, x) for x in q[1:4]]
+    for t, was in zip((m.block_tables, m.context_lens, m.pages_allocated, m.cache.free_list,
+                       m.cache.free_head, ev.weights), state):
+        assert torch.equal(t, was)  # a capture runs nothing
+    graph.replay()
+    m.cache.check()
+    assert m.context_lens.tolist() == [400, 400]
+    got = [x.clone() for x in out]
+    fresh.reset()
+    c = m.cache
+    bt = m.block_tables.clone()  # not known to be evicted from
+    for x, y in zip(q[1:4], got):
+        want = fresh(x, c.k_cache, c.v_cache, bt, m.context_lens, 0)
+        fresh.step_done(0, 1)
+        assert torch.equal(y, want)
