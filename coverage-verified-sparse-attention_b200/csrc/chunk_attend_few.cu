@@ -609,8 +609,8 @@ cudaError_t launch_rows(const FewArgs& a, int rows, int ctas, cudaStream_t s) {
 
 }  // namespace
 
-// Rows of an item, or 0 where the other kernels serve the call. By the batch's mean of
-// rows a sequence, rounded up: longer sequences take several items, which read its cache
+// Rows of an item, or 0 where the other kernels serve the call: never fewer than one token's.
+// By the batch's mean of rows a sequence, rounded up: longer sequences take several items, which read its cache
 // again each, so batches that hold a prompt are left to the tensor cores. Here against there:
 // 32 single tokens 72 and 291 us, 8 drafts of 2 to 8 tokens 80 and 101 us (64-wide heads),
 // 115 and 157 us (128-wide).
@@ -618,7 +618,8 @@ int chunk_few_rows(const KvView& kv, const RaggedView& rg, const ChunkView& c) {
   if (kv.dtype != CVSA_DTYPE_E4M3 || c.dtype == CVSA_DTYPE_F32 || (kv.d != 64 && kv.d != 128) ||
       kv.bs % 16)
     return 0;
-  const int64_t rows = ((int64_t)rg.T + rg.B - 1) / (rg.B > 0 ? rg.B : 1) * (c.hq / kv.hkv);
+  const int64_t mean = rg.B > 0 ? ((int64_t)rg.T + rg.B - 1) / rg.B : rg.T;
+  const int64_t rows = (mean > 0 ? mean : 1) * (c.hq / kv.hkv);
   return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 0;
 }
 

@@ -1,5 +1,8 @@
 """Argument checks of the 8-bit cache, the key weights and the eviction, without a GPU."""
 
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -320,3 +323,28 @@ def test_key_weights_into_part_of_what_was_there(fake):
     for out in (w[:64], w[64:]):
         weigh(a, weights=w[:64].view(1, 2, 32), out=out.view(1, 2, 32))
         assert fake.calls[-1][0] == "cvsa_key_weights"
+
+
+def alone(code):
+    """`code` in a process of its own, which may end badly."""
+    code = f"import sys\nsys.path[:0] = {sys.path!r}\n" + code
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert r.returncode == 0, (r.returncode, r.stdout[-200:], r.stderr[-500:])
+
+
+def test_a_batch_without_tokens():
+    """No tokens, any number of query heads a KV head: nothing to do. (The plan once divided by
+    its groups' tokens, 0 of them, which ends the process.)"""
+    alone(f"""
+from cvsa import _lib
+from test_ragged_host import chunk, kv, ragged
+lib, r8 = _lib.load(), kv(dt={E4M3})
+for hq in (2, 16, 18, 32, 64, 66, 128):
+    for B in (0, 1, 5):
+        for dt in ({BF16}, {_lib.DTYPE_F32}):
+            print(hq, B, dt, flush=True)
+            a = r8, 256, 256, ragged(T=0, B=B, S=5), chunk(hq=hq, dt=dt, q=None, out=None)
+            assert lib.cvsa_chunk_attend_q8_check(*a) == 0
+            assert lib.cvsa_chunk_attend_q8(*a, None, None, 0, None) == 0
+            assert lib.cvsa_chunk_attend_q8_workspace_size(*a) > 0
+""")
