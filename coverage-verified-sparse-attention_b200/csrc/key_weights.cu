@@ -78,8 +78,10 @@ __global__ void __launch_bounds__(kThreads) key_weights_kernel(const __grid_cons
   const int key0 = tile * kKeys;
   if (key0 >= q.ctx) return;
   if (tid < kKeys) {
+    int lo, hi;
+    weight_keys(q, a.w.causal, a.w.window, lo, hi);
     const int key = key0 + tid;
-    bool ok = key < q.ctx;
+    bool ok = key >= lo && key < hi;
     int64_t off = 0;
     float scale = 1.f;
     if (ok) {

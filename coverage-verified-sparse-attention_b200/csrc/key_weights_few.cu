@@ -54,18 +54,30 @@ __global__ void __launch_bounds__(kThreads) weights_few_kernel(const __grid_cons
   const int64_t st = a.kv.st * (F8 ? 1 : 2);  // bytes between keys
   while (more) {
     // a run of tiles of one head
-    const int b = walk.b, h = walk.h, key0 = walk.i * kTileKeys;
+    const int b = walk.b, h = walk.h, first = walk.i * kTileKeys;
     const SeqInfo q = walk.q;
-    int end = key0;
+    int end = first;
     do {
       end = min(q.ctx, (walk.i + 1) * kTileKeys);
       walk.step();
       more = walk.next(a.rg, a.g);
     } while (more && walk.b == b && walk.h == h);
     const int rows = q.n * G;  // at most 2^31 by the call's check
-    const int n = (end - key0 + 15) / 16;
     const int32_t* const table = a.rg.tables + (int64_t)q.slot * a.rg.W;
     const int64_t at_out = ((int64_t)q.slot * hkv + h) * a.w.stride;
+    // n blocks of 16 keys from key0 on hold all keys of the run that some row sees
+    int lo, stop;
+    weight_keys(q, a.g.causal, a.g.window, lo, stop);
+    lo = max(first, lo & ~15);
+    stop = min(stop, end);
+    const int n = lo < stop ? (stop - lo + 15) / 16 : 0, key0 = n ? lo : end;
+    auto unseen = [&](int from, int to) {
+      for (int key = from + lane; key < to; key += 32)
+        a.w.out[at_out + key] = key < q.start ? a.w.decay * a.w.prior[at_out + key] : 0.f;
+    };
+    unseen(first, key0);
+    unseen(key0 + 16 * n, end);
+    if (n == 0) continue;
     // Queries r0.. as operands, their factors and what is subtracted; rows that are not
     // there or saw no key take no part.
     uint32_t qb[kNt][kSteps][2];
@@ -142,7 +154,7 @@ __global__ void __launch_bounds__(kThreads) weights_few_kernel(const __grid_cons
       const int key = key0 + (i0 + lane) * 16;
       blk = -1;
       ks = 1.f;
-      if (key >= end) return;
+      if (key >= stop) return;
       blk = table[key / bs];
       if (blk < 0 || blk >= a.kv.num_blocks) {
         set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);
@@ -203,9 +215,9 @@ __global__ void __launch_bounds__(kThreads) weights_few_kernel(const __grid_cons
       for (int r0 = 0;; r0 += ROWS) {
         if (r0 > 0 || (rows > ROWS && i > 0)) queries(r0);
         // some row does not see every key, or takes no part
-        const int first = q.start + r0 / G, last = q.start + (min(rows, r0 + ROWS) - 1) / G;
-        const bool partial = live != (1u << 2 * kNt) - 1 || (a.g.causal && key + 15 > first) ||
-                             (a.g.window > 0 && key <= last - a.g.window);
+        const int pos0 = q.start + r0 / G, pos1 = q.start + (min(rows, r0 + ROWS) - 1) / G;
+        const bool partial = live != (1u << 2 * kNt) - 1 || (a.g.causal && key + 15 > pos0) ||
+                             (a.g.window > 0 && key <= pos1 - a.g.window);
 #pragma unroll
         for (int x = 0; x < kNt; ++x) {
           // The tensor core cuts its sums where an addition rounds them: pairs of steps, whose

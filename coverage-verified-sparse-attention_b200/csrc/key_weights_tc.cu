@@ -172,6 +172,8 @@ __device__ __forceinline__ void key_role(const WArgs& a, WMeta* m, uint32_t base
     if (t0 >= t1) continue;
     const uint32_t buf = n & 1;
     const int32_t* const table = a.rg.tables + (int64_t)walk.q.slot * a.rg.W;
+    int lo, hi;
+    weight_keys(walk.q, a.g.causal, a.g.window, lo, hi);
     // keys w * 64 + 32 k + lane of the tiles
     int64_t off[2];
     float scale[2] = {1.f, 1.f};
@@ -179,7 +181,7 @@ __device__ __forceinline__ void key_role(const WArgs& a, WMeta* m, uint32_t base
     for (int k = 0; k < 2; ++k) {
       const int key = walk.i * kKeys + w * 64 + k * 32 + lane;
       off[k] = -1;
-      if (key >= walk.q.ctx) continue;
+      if (key < lo || key >= hi) continue;
       const int page = key / a.g.bs, blk = table[page];
       if (blk < 0 || blk >= a.kv.num_blocks) {
         set_dev_error(a.dev_err, CVSA_DEV_ERR_BLOCK_RANGE);

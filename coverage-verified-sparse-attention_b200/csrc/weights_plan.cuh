@@ -22,6 +22,15 @@ __device__ __forceinline__ int weight_tiles(const SeqInfo& q, int KT) {
   return (q.ctx + KT - 1) / KT;
 }
 
+// Keys [lo, hi) of the sequence that some row sees. Others keep their decayed weight, and a page
+// of such keys alone is not looked up, as in the attention.
+__device__ __forceinline__ void weight_keys(const SeqInfo& q, int causal, int window, int& lo,
+                                            int& hi) {
+  const int64_t end = causal ? (int64_t)q.start + q.n : q.ctx;
+  lo = window > 0 ? (int)max((int64_t)0, (int64_t)q.start - window + 1) : 0;
+  hi = q.n > 0 ? (int)max((int64_t)0, min(end, (int64_t)q.ctx)) : 0;
+}
+
 // Tokens [t0, t1) of the sequence see some key of tile i.
 __device__ __forceinline__ void weight_tokens(const SeqInfo& q, const WeightGeo& g, int i, int& t0,
                                               int& t1) {

@@ -679,7 +679,8 @@ typedef struct cvsa_key_weights {
  * out = decay * prior + sum of e^(scale q.k - lse) over the rows of its KV head's
  * group that see it. Keys from a sequence's start position on (the new tokens'
  * own) start from 0. Keys past a context, and sequences that were refused or have
- * no table row, are not written. k_scale: of 8-bit pools, else NULL. v_cache of
+ * no table row, are not written. A page none of whose keys a row sees is not looked
+ * up, as in cvsa_chunk_attend. k_scale: of 8-bit pools, else NULL. v_cache of
  * the descriptor is not read. fp32 sums in a fixed order. */
 int cvsa_key_weights(const cvsa_kv_desc_t* kv, const float* k_scale,
                      const cvsa_ragged_desc_t* rg, const cvsa_key_weights_t* args,

@@ -727,3 +727,51 @@ def test_a_slot_that_is_filled_anew_has_no_weights(cuda, registered):
     evs.clear()
     del ev
     m.prefill_kv(2, k[:10], v[:10])  # nobody counts any more
+
+
+# ---------------------------------------------------------------------------
+# keys that no row sees
+# ---------------------------------------------------------------------------
+def hidden_pages(P, window, starts=None, causal=True):
+    """(table row, page) of the pages that hold keys of a context but none that a row sees."""
+    out = []
+    for b, (n, c) in enumerate(zip(P.new, P.ctx)):
+        first = c - n if starts is None else starts[b]
+        lo = max(0, first - window + 1) if window else 0
+        hi = (min(c, first + n) if causal else c) if n else 0
+        for p in range(-(-c // P.page)):
+            if min(c, (p + 1) * P.page) <= lo or p * P.page >= hi:
+                out.append((P.rows[b], p))
+    return out
+
+
+@pytest.mark.parametrize("dtype,cache8,d,page", [
+    (BF16, False, 128, 16), (BF16, True, 128, 16), (F16, True, 64, 64), (F16, False, 64, 32),
+    (F32, False, 128, 16), (BF16, True, 256, 16), (BF16, False, 64, 24)])
+@pytest.mark.parametrize("new,kw", [
+    ([1, 1, 0], dict(window=16)), ([1, 3, 2], dict(window=40)), ([100, 64, 1], dict(window=33)),
+    ([150, 20, 0], dict(window=1)), ([1, 2, 0], dict()), ([4, 0, 90], dict())])
+@pytest.mark.parametrize("early", [False, True])
+def test_weights_of_pages_nobody_sees(cuda, dtype, cache8, d, page, new, kw, early):
+    """Pages behind a window, past the last row's position or of a sequence without new
+    tokens are not looked up, as in the attention: table entries out of range there are no
+    error, and their keys keep decay times what they had."""
+    P = problem(new, [901, 640, 333], 8, 2, d, cache8, dtype=dtype, page=page, seed=d)
+    starts = [c - n - 150 for n, c in zip(new, P.ctx)] if early else None
+    lse = lse_of(P, starts=starts, **kw)
+    hidden = hidden_pages(P, kw.get("window", 0), starts)
+    assert hidden
+    prior = torch.rand((3, 2, P.tables.shape[1] * page), device=cuda)
+    st = None if starts is None else torch.tensor(starts, **I32)
+    args = (P.q, lse, P.k_cache, P.tables, P.lens, P.cu, prior)
+    form = dict(decay=0.5, start_positions=st, dev_error=P.dev_error, **P.more, **kw)
+    want = key_weights(*args, out=torch.full_like(prior, 7.0), **form)
+    for i, (r, p) in enumerate(hidden):
+        P.tables[r, p] = -1 - i if i % 2 else P.k_cache.shape[0] + i
+    got = key_weights(*args, out=torch.full_like(prior, 7.0), **form)
+    scales = dict(k_scale=P.k_scale, v_scale=P.v_scale) if cache8 else {}
+    chunk_attention(P.q, P.k_cache, P.v_cache, P.tables, P.lens, P.cu, start_positions=st,
+                    dev_error=P.dev_error, **scales, **kw)
+    torch.cuda.synchronize()
+    assert int(P.dev_error.item()) == 0
+    assert torch.equal(got, want)
