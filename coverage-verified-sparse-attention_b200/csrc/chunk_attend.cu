@@ -361,7 +361,6 @@ cudaError_t launch_general_c(const GenArgs& a, int rows, int ctas, cudaStream_t 
 // Block (x, y): rows [32 x, 32 x + 32) of the item that begins in CTA y's range
 // and leaves it. Lanes own rows, warps own float4 columns. Parts are summed in
 // CTA order. Most blocks find no item and leave at once.
-constexpr int kMaxCtas = 320;
 
 struct MergeArgs {
   const float* parts;
@@ -460,8 +459,7 @@ constexpr size_t kDescBytes = ((kMaxCtas * sizeof(ChunkMergeDesc) + 255) / 256) 
 // One CTA an SM; the general kernel's two where shared memory and registers
 // hold two (64-wide heads): one hides the other's barriers.
 int chunk_ctas(const KvView& kv, bool tc) {
-  const int n = num_sms() * (!tc && kv.d == 64 ? 2 : 1);
-  return n < kMaxCtas ? n : kMaxCtas;
+  return chunk_grid(!tc && kv.d == 64 ? 2 : 1);
 }
 
 ChunkGeo general_geo(const KvView& kv, const RaggedView& rg, const ChunkView& c) {

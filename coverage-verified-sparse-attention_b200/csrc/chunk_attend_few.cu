@@ -521,12 +521,12 @@ chunk_few_kernel(const __grid_constant__ FewArgs a) {
 // Joins the pieces of the item that begins in CTA y's range: block (x, y) its row x.
 // Warps take pieces in turn, lanes columns; sums in a fixed order. A slot is
 // m [rows], l [rows], o [rows][D].
-constexpr int kJoin = 4, kMaxParts = 320;
+constexpr int kJoin = 4;
 template <typename TI, int D>
 __global__ void __launch_bounds__(32 * kJoin) few_merge_kernel(const float* parts,
                                                                const ChunkMergeDesc* desc,
                                                                ChunkView c, int slot_rows, int G) {
-  __shared__ float weight[kMaxParts];
+  __shared__ float weight[kMaxCtas];
   __shared__ float red[kJoin][2];
   __shared__ float sums[kJoin][D];
   const int cta = blockIdx.y, r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -624,7 +624,7 @@ int chunk_few_rows(const KvView& kv, const RaggedView& rg, const ChunkView& c) {
 }
 
 // Blocks: two an SM.
-int chunk_few_ctas() { return 2 * num_sms(); }
+int chunk_few_ctas() { return chunk_grid(2); }
 
 ChunkGeo chunk_few_geo(const KvView& kv, const RaggedView& rg, const ChunkView& c, int rows) {
   ChunkGeo g;

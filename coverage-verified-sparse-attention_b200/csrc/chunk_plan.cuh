@@ -272,6 +272,14 @@ __host__ __device__ constexpr size_t chunk_slot_floats(int rows, int d) {
   return (size_t)rows * (d + 2);
 }
 
+// CTAs of a call at most: the workspace has a descriptor for each ahead of the partial slots,
+// and the merges hold a weight for each in shared memory.
+constexpr int kMaxCtas = 320;
+inline int chunk_grid(int per_sm) {
+  const int n = per_sm * num_sms();
+  return n < kMaxCtas ? n : kMaxCtas;
+}
+
 // Whether a call's units fit 31 bits, and whether its items may be split.
 inline bool chunk_fits(const RaggedView& rg, const ChunkGeo& g) {
   const int64_t tiles = ((int64_t)rg.W * g.bs + g.KT - 1) / g.KT + 1;

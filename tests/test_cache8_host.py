@@ -348,3 +348,25 @@ for hq in (2, 16, 18, 32, 64, 66, 128):
             assert lib.cvsa_chunk_attend_q8(*a, None, None, 0, None) == 0
             assert lib.cvsa_chunk_attend_q8_workspace_size(*a) > 0
 """)
+
+
+def test_few_token_grid_fits_its_workspace(tmp_path):
+    """The descriptors ahead of the partial slots, and the merge's weights, hold 320 blocks: a
+    device of more than 160 multiprocessors gets no more. (The library's function that counts
+    them gives way to one of the same name that was loaded before it.)"""
+    src, shim = tmp_path / "sms.cpp", str(tmp_path / "sms.so")
+    src.write_text("int n_sms;\nnamespace cvsa { int num_sms() { return n_sms; } }\n")
+    subprocess.run(["g++", "-shared", "-fPIC", "-o", shim, str(src)], check=True)
+    alone(f"""
+import ctypes
+shim = ctypes.CDLL({shim!r}, ctypes.RTLD_GLOBAL)
+from cvsa import _lib
+from test_ragged_host import chunk, kv, ragged
+lib, blocks = _lib.load(), ctypes.CDLL(_lib.LIB_PATH)._ZN4cvsa14chunk_few_ctasEv
+for sms in (1, 148, 160, 161, 400):
+    ctypes.c_int.in_dll(shim, "n_sms").value = sms
+    assert blocks() == min(2 * sms, 320), (sms, blocks())
+    # two slots of 32 rows a block fit behind the descriptors
+    size = lib.cvsa_chunk_attend_q8_workspace_size(kv(dt={E4M3}), 256, 256, ragged(), chunk())
+    assert size >= 320 * 16 + blocks() * 2 * 32 * (128 + 2) * 4, (sms, size)
+""")
