@@ -22,12 +22,14 @@
 // P' is transposed in registers (movmatrix). K's scale goes to the scores, V's to the
 // widened codes. f16 throughout: queries are scaled by row as in chunk_attend_tc.cu,
 // weights carry 2^11 and the reference maximum follows rises of 2^4, for the reasons
-// given there. The next block's codes are loaded to registers as soon as this block's are
-// operands, so nothing synchronises.
+// given there. Their sum is of the 32-bit weights: rounding one to f16 errs by at most 2^-11 of
+// it, either way, so a row errs by less than that of its values' absolute moment. The next
+// block's codes are loaded to registers as soon as this block's are operands, so nothing
+// synchronises.
 //
 // 32 single tokens of 32 heads at 1 to 8192 keys take 72 us (50 of them the codes at the
 // rate of a copy; the rest goes to the first loads and the join at the end of an item), one
-// token at 128K keys 61 us, 8 drafts of 2 to 8 tokens of 64-wide heads 80 us. Measured and not
+// token at 128K keys 60 us, 8 drafts of 2 to 8 tokens of 64-wide heads 80 us. Measured and not
 // kept: codes through a ring of asynchronous copies in shared memory (91 us), 32 keys a step
 // of 12 warps (89), rows on M (125). The pieces of a split item are joined by a block a
 // row, since 128K keys make 37 pieces (a warp a row: 47 us, now 9).
