@@ -612,8 +612,9 @@ cudaError_t launch_rows(const FewArgs& a, int rows, int ctas, cudaStream_t s) {
 }  // namespace
 
 // Rows of an item, or 0 where the other kernels serve the call: never fewer than one token's.
-// By the batch's mean of rows a sequence, rounded up: longer sequences take several items, which read its cache
-// again each, so batches that hold a prompt are left to the tensor cores. Here against there:
+// By the batch's mean of rows a sequence, rounded up: longer sequences take several items,
+// which read its cache again each, so batches that hold a prompt are left to the tensor cores.
+// Here against there:
 // 32 single tokens 72 and 291 us, 8 drafts of 2 to 8 tokens 80 and 101 us (64-wide heads),
 // 115 and 157 us (128-wide).
 int chunk_few_rows(const KvView& kv, const RaggedView& rg, const ChunkView& c) {

@@ -7,8 +7,8 @@
 // uneven ends (one at 128K keys 59 us, over 8 bits 49). Blocks of 16 keys that no row sees
 // are not read, their weights are decayed beside (with a window of 16 keys: 14 us). As in
 // chunk_attend_few.cu, keys go from memory to the operands of mma.sync in the registers of
-// the lane that loads them: S' = K Q', 16 keys by 8 rows, lane (g, t) with 16-byte pieces of keys g and g + 8 and the same elements of
-// query row g. A key's weights are summed over the two rows of a lane, the row tiles and
+// the lane that loads them: S' = K Q', 16 keys by 8 rows, lane (g, t) with 16-byte pieces
+// of keys g and g + 8 and the same elements of query row g. A key's weights are summed over the two rows of a lane, the row tiles and
 // the four lanes of its row, so nothing else is exchanged and a warp works on its own.
 // 16-bit keys are used as they are; 8-bit ones are widened to f16, with queries scaled by
 // row to fit. A sequence of more rows than a step holds (ROWS) goes over them in turn for

@@ -28,8 +28,9 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tens
     [num_seqs, ceil(keep / block_size)], which no sequence may be using, their
     weights to out_weights [num_seqs, H_kv, >= keep] (None: to the front of
     weights, float32 [num_seqs, H_kv, >= max_pages * block_size], where those behind
-    become 0 up to the old length). Tables and lengths stay as they are. k_scale, v_scale: of an 8-bit cache, whose new
-    pages get the largest scale of their rows.
+    become 0 up to the old length). Tables and lengths stay as they are.
+    k_scale, v_scale: of an 8-bit cache, whose new pages get the largest scale of
+    their rows.
     """
     dev = _lib.same_device(k_cache, v_cache, block_tables, context_lens, weights, new_tables,
                            out_weights, kept, dev_error, k_scale, v_scale)

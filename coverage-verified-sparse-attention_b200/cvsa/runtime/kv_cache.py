@@ -238,8 +238,8 @@ class SequenceKVManager:
         """Cut every sequence longer than `keep` to its `keep` keys of most weight per KV head.
 
         weights [batch_size, num_kv_heads, >= max_pages * block_size] float32
-        (`cvsa.kernels.key_weights`) moves along, 0 where a key went. Of each head the first `sink`
-        and the last `recent` keys stay in any case. Old pages go back to the
+        (`cvsa.kernels.key_weights`) moves along, 0 where a key went. Of each head the
+        first `sink` and the last `recent` keys stay in any case. Old pages go back to the
         pool; pages for the kept keys are taken from it first, and a sequence that it
         has none for stays as it is (`cache.check()` raises). Returns the kept
         keys [batch_size, num_kv_heads, keep], -1 for sequences that were not
